@@ -16,6 +16,9 @@ LIB = os.path.join(HERE, "libunirec_amd.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function"]
 
+# no packed fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong results on this part now and then
+HIP_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 
 # the bounds-checked variant (common.h: UR_ROW): the same sources with -DUR_DEBUG_BOUNDS -> libunirec_amd_dbg.so, loaded by _lib.py when
 # UR_DEBUG_BOUNDS=1.  Only the files that use the macro are recompiled; every other object is shared with the release library.
@@ -24,7 +27,7 @@ DBG_FILES = ("rowops.hip", "loss.hip", "rowchain.hip")
 
 
 def _digest(paths, extra=()):
-    h = hashlib.sha256(" ".join(FLAGS + list(extra)).encode())
+    h = hashlib.sha256(" ".join(FLAGS + HIP_FLAGS + list(extra)).encode())
     for p in sorted(paths):
         with open(p, "rb") as f:
             h.update(f.read())
@@ -49,7 +52,7 @@ def build(verbose=True, force=False, debug_bounds=False):
             for old in os.listdir(OBJ):
                 if old.startswith(stem + "."):
                     os.remove(os.path.join(OBJ, old))
-            lang = ["-x", "hip"] if s.endswith(".hip") else []
+            lang = HIP_FLAGS + ["-x", "hip"] if s.endswith(".hip") else []
             jobs.append((s, [HIPCC] + FLAGS + dbg + lang + ["-c", src, "-o", obj]))
 
     def run(job):
