@@ -19,6 +19,7 @@ UR_SASREC_N_GLOBAL = 3
 UR_SASREC_N_PER_LAYER = 16
 
 ACT_IDS = {"gelu": 0, "relu": 1, "swish": 2, "tanh": 3, "sigmoid": 4}
+DTYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # UR_F32 / UR_F16 / UR_BF16
 LOSS_IDS = {"bce": 0, "bpr": 1, "softmax": 2, "ccl": 3, "fullsoftmax": 4}
 
 
@@ -173,6 +174,11 @@ SIGNATURES = {
     "ur_full_softmax_fwd_shard": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, P, P, P, P, C.c_float, C.c_float, P, P, P]),
     "ur_full_softmax_combine_shards": (C.c_int, [P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, P, P, P]),
     "ur_full_softmax_bwd_shard": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, P, P, P, P, C.c_float, C.c_float, P, P, P, P, P, C.c_int32, P, P]),
+    "ur_full_distill_workspace_bytes": (I64, [C.c_int32, C.c_int32, I64, C.c_int32, C.c_int32]),
+    "ur_full_distill_fwd": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, P, P, C.c_int32, C.c_int32, P, C.c_float, C.c_float, C.c_float, P, P, P, P, P,
+                                      P, P, P]),
+    "ur_full_distill_bwd": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, C.c_int32, P, C.c_float, C.c_float, C.c_float, P, P, P, P, P, P, P, P, P, P,
+                                      P]),
     "ur_rows_scatter_add": (C.c_int, [P, P, I64, P, C.c_int32, P, P]),
     "ur_prof_enable": (C.c_int, [C.c_int]),
     "ur_prof_set_mask": (C.c_int, [C.c_uint32]),

@@ -839,6 +839,83 @@ def full_softmax_bwd_shard(user_emb_all, shard_rows, target_row, lse, ws, d_shar
     return d_user, d_ib
 
 
+# --------------------------------------------------------------------------------------------- distillation from a teacher's top logits
+class DistillSaved:
+    """What a full_distill_fwd(need_grad=True) leaves for its full_distill_bwd (all device tensors)."""
+    __slots__ = ("row_stat", "coef", "entry_id", "d_unit", "ws")
+
+
+def _distill_check(who, user_emb, item_table, item_bias, tau, temperature):
+    _chk(user_emb, torch.float32, "user_emb")
+    _chk(item_table, torch.float32, "item_table")
+    _chk(item_bias, torch.float32, "item_bias", allow_none=True)
+    if user_emb.dim() != 2 or item_table.dim() != 2 or item_table.shape[1] != user_emb.shape[1]:
+        raise _lib.UnirecAmdError(f"{who}: user_emb {tuple(user_emb.shape)} and item_table {tuple(item_table.shape)} do not fit")
+    if item_bias is not None and item_bias.numel() != item_table.shape[0]:
+        raise _lib.UnirecAmdError(f"{who}: item_bias has {item_bias.numel()} entries for {item_table.shape[0]} items")
+    if not (tau > 0 and temperature > 0):
+        raise _lib.UnirecAmdError(f"{who}: tau={tau} and temperature={temperature} must be positive")
+    _same_device(who, user_emb, item_table, item_bias)
+
+
+def _same_device(who, *tensors):
+    """every tensor on the CURRENT device: the kernels run on its current stream"""
+    cur = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.device.index != cur:
+            raise _lib.UnirecAmdError(f"{who}: tensor on {t.device}, the current device is cuda:{cur} (torch.cuda.set_device)")
+
+
+def full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias=None, tau=1.0, score_clip=-1.0, temperature=1.0, need_grad=True):
+    """loss = T^2 mean_b KL(teacher's top-K softmax || softmax over ALL items) -> (loss_out float32[4] = [loss, rows with a teacher, update
+    guard, -], lse float32[B], DistillSaved | None).  teacher_id int64 [B,K] / teacher_score [B,K] (float32, float16 or bfloat16): what
+    full_topk returns; -1 / -inf entries are absent.  See include/unirec_amd.h: ur_full_distill_fwd."""
+    who = "full_distill_fwd"
+    _distill_check(who, user_emb, item_table, item_bias, tau, temperature)
+    _chk(teacher_id, torch.int64, "teacher_id")
+    if teacher_score.dtype not in _lib.DTYPE_IDS:
+        raise _lib.UnirecAmdError(f"teacher_score: expected float32 / float16 / bfloat16, got {teacher_score.dtype}")
+    _chk(teacher_score, teacher_score.dtype, "teacher_score")
+    B, d = user_emb.shape
+    if teacher_id.dim() != 2 or teacher_id.shape[0] != B or teacher_score.shape != teacher_id.shape:
+        raise _lib.UnirecAmdError(f"{who}: teacher_id {tuple(teacher_id.shape)} / teacher_score {tuple(teacher_score.shape)} for {B} rows")
+    _same_device(who, teacher_id, teacher_score)
+    K, N, dev = teacher_id.shape[1], item_table.shape[0], user_emb.device
+    id_guard_check()
+    f32 = dict(dtype=torch.float32, device=dev)
+    lse, loss_out = torch.empty(B, **f32), torch.empty(4, **f32)
+    sv = DistillSaved()
+    sv.row_stat = torch.empty(3 * B, **f32)
+    sv.coef = torch.empty(B, K, **f32) if need_grad else None
+    sv.entry_id = torch.empty(B, K, dtype=torch.int64, device=dev) if need_grad else None
+    sv.d_unit = torch.empty(B, d, **f32) if need_grad else None
+    sv.ws = torch.empty(check(lib.ur_full_distill_workspace_bytes(B, d, N, K, int(need_grad)), "ur_full_distill_workspace_bytes"),
+                        dtype=torch.uint8, device=dev)
+    check(lib.ur_full_distill_fwd(_p(user_emb), _p(item_table), N, B, d, _p(teacher_id), _p(teacher_score), _lib.DTYPE_IDS[teacher_score.dtype], K,
+                                  _p(item_bias), float(tau), float(score_clip if score_clip else -1.0), float(temperature), _p(lse), _p(loss_out),
+                                  _p(sv.row_stat), _p(sv.coef), _p(sv.entry_id), _p(sv.d_unit), _p(sv.ws), _stream()), "ur_full_distill_fwd")
+    return loss_out, lse, (sv if need_grad else None)
+
+
+def full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, saved, item_bias=None, tau=1.0, score_clip=-1.0, temperature=1.0, d_loss=None):
+    """-> (d_user [B,d], d_table [N,d] dense, d_item_bias [N] | None) of a full_distill_fwd(need_grad=True) with the same arguments.
+    See include/unirec_amd.h: ur_full_distill_bwd."""
+    who = "full_distill_bwd"
+    _distill_check(who, user_emb, item_table, item_bias, tau, temperature)
+    _chk(d_loss, torch.float32, "d_loss", allow_none=True)
+    B, d = user_emb.shape
+    if saved is None or saved.d_unit.shape != user_emb.shape or saved.coef.shape != teacher_id.shape or loss_out.numel() != 4 or lse.numel() != B:
+        raise _lib.UnirecAmdError(f"{who}: not the results of a full_distill_fwd(need_grad=True) of these inputs")
+    K, N, dev = teacher_id.shape[1], item_table.shape[0], user_emb.device
+    d_user = torch.empty(B, d, dtype=torch.float32, device=dev)
+    d_table = torch.empty(N, d, dtype=torch.float32, device=dev)
+    d_ib = torch.empty(N, dtype=torch.float32, device=dev) if item_bias is not None else None
+    check(lib.ur_full_distill_bwd(_p(user_emb), _p(item_table), N, B, d, K, _p(item_bias), float(tau), float(score_clip if score_clip else -1.0),
+                                  float(temperature), _p(loss_out), _p(saved.row_stat), _p(saved.coef), _p(saved.entry_id), _p(saved.d_unit),
+                                  _p(d_loss), _p(d_user), _p(d_table), _p(d_ib), _p(saved.ws), _stream()), "ur_full_distill_bwd")
+    return d_user, d_table, d_ib
+
+
 def rows_scatter_add(pl: RowsPlan, rows, dense):
     check(lib.ur_rows_scatter_add(_p(pl.uniq_idx), _p(pl.n_uniq), pl.n, _p(rows), rows.shape[1], _p(dense), _stream()), "ur_rows_scatter_add")
 

@@ -319,6 +319,39 @@ def _(user_emb, item_table, k, user_id, hist_ptr, hist_sorted, user_bias, item_b
     return user_emb.new_empty((B, k)), user_emb.new_empty((B, k), dtype=torch.int64)
 
 
+# ------------------------------------------------------------------------------------------------ distillation from a teacher's top logits
+@custom_op(f"{NS}::full_distill_fwd", mutates_args=())
+def full_distill_fwd(user_emb: torch.Tensor, item_table: torch.Tensor, teacher_id: torch.Tensor, teacher_score: torch.Tensor,
+                     item_bias: Optional[torch.Tensor], tau: float = 1.0, score_clip: float = -1.0, temperature: float = 1.0) -> Tuple[
+                         torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """-> (loss_out, lse, row_stat, coef, entry_id, d_unit, ws): the last five are full_distill_bwd's"""
+    loss_out, lse, sv = ops.full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias, tau, score_clip, temperature)
+    return loss_out, lse, sv.row_stat, sv.coef, sv.entry_id, sv.d_unit, sv.ws
+
+
+@full_distill_fwd.register_fake
+def _(user_emb, item_table, teacher_id, teacher_score, item_bias, tau=1.0, score_clip=-1.0, temperature=1.0):
+    B = user_emb.shape[0]
+    return (user_emb.new_empty((4,)), user_emb.new_empty((B,)), user_emb.new_empty((3 * B,)), user_emb.new_empty(teacher_id.shape),
+            torch.empty_like(teacher_id), torch.empty_like(user_emb), user_emb.new_empty((torch.library.get_ctx().new_dynamic_size(),), dtype=torch.uint8))
+
+
+@custom_op(f"{NS}::full_distill_bwd", mutates_args=("ws",))
+def full_distill_bwd(user_emb: torch.Tensor, item_table: torch.Tensor, loss_out: torch.Tensor, lse: torch.Tensor, row_stat: torch.Tensor,
+                     coef: torch.Tensor, entry_id: torch.Tensor, d_unit: torch.Tensor, ws: torch.Tensor, d_loss: Optional[torch.Tensor],
+                     item_bias: Optional[torch.Tensor], tau: float = 1.0, score_clip: float = -1.0,
+                     temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    sv = ops.DistillSaved()
+    sv.row_stat, sv.coef, sv.entry_id, sv.d_unit, sv.ws = row_stat, coef, entry_id, d_unit, ws
+    d_user, d_table, d_ib = ops.full_distill_bwd(user_emb, item_table, entry_id, lse, loss_out, sv, item_bias, tau, score_clip, temperature, d_loss)
+    return d_user, d_table, d_ib if d_ib is not None else user_emb.new_empty((0,))
+
+
+@full_distill_bwd.register_fake
+def _(user_emb, item_table, loss_out, lse, row_stat, coef, entry_id, d_unit, ws, d_loss, item_bias, tau=1.0, score_clip=-1.0, temperature=1.0):
+    return torch.empty_like(user_emb), torch.empty_like(item_table), user_emb.new_empty((item_table.shape[0] if item_bias is not None else 0,))
+
+
 # ------------------------------------------------------------------------------------------------ header symbol <-> op
 HEADER_TO_OP = {
     "ur_embedding_gather_f32": "embedding_gather",
@@ -343,6 +376,8 @@ HEADER_TO_OP = {
     "ur_dense_adam": "dense_adam",
     "ur_full_rank": "full_rank",
     "ur_full_topk": "full_topk",
+    "ur_full_distill_fwd": "full_distill_fwd",
+    "ur_full_distill_bwd": "full_distill_bwd",
 }
 
 _QUERY = "layout / workspace-size query or error plumbing: plain host function, nothing to dispatch"
@@ -357,7 +392,7 @@ NOT_OPS = {
     "ur_rows_reduce_update_owner": _SHARD,
     "ur_last_error": _QUERY, "ur_version": _QUERY, "ur_id_guard_state": _QUERY, "ur_id_guard_reset": _SWITCH, "ur_trace_ranges_pushed": _QUERY, "ur_sasrec_param_layout": _QUERY, "ur_gru_param_layout": _QUERY,
     "ur_gru_workspace_bytes": _QUERY, "ur_rows_plan_workspace_bytes": _QUERY, "ur_gemm_tn_workspace_floats": _QUERY,
-    "ur_full_topk_workspace_bytes": _QUERY, "ur_full_softmax_workspace_bytes": _QUERY, "ur_convformer_param_layout": _QUERY,
+    "ur_full_topk_workspace_bytes": _QUERY, "ur_full_distill_workspace_bytes": _QUERY, "ur_full_softmax_workspace_bytes": _QUERY, "ur_convformer_param_layout": _QUERY,
     "ur_convformer_workspace_bytes": _QUERY, "ur_atthist_param_layout": _QUERY, "ur_atthist_workspace_bytes": _QUERY,
     "ur_host_sampler_create": _HOST, "ur_host_sampler_destroy": _HOST, "ur_host_sampler_getrandbits": _HOST, "ur_host_sampler_random": _HOST,
     "ur_host_sampler_randint": _HOST, "ur_host_sampler_set_alias": _HOST, "ur_host_build_rows": _HOST, "ur_alias_table_build": _HOST,
