@@ -759,6 +759,25 @@ int ur_full_distill_bwd(const float* user_emb, const float* item_table, int64_t 
                         float* d_user_emb, float* d_item_table, float* d_item_bias, void* ws, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Sampling from scores with temperature, top-k, top-p and min-p, from given random numbers (no counterpart in UniRec; beside
+ * ur_full_topk: answers drawn from the distribution instead of its head).  Row b of scores [B,n] (score_type: UR_F32 / UR_F16 / UR_BF16, rows
+ * ld apart), S draws with replacement from rand[B,S] in [0,1):
+ *   z = (x - max x) / T, w = exp(z); NaN and -inf are never drawn; a row that holds +inf draws among those entries;
+ *   top_k > 0: the first top_k in the order (score descending, index ascending);
+ *   top_p < 1: of those, in that order, every entry before which less than top_p of their weight lies (the first always);
+ *   min_p > 0: w >= min_p;
+ *   the answer to u: the first index n with sum_{j <= n} w_j > u W over the kept entries in INDEX order, W their weight.
+ * temperature = 0: the lowest index among the largest.  *_rows (nullable): per-row values [B] in the place of the scalar (a top_p <= 0 keeps
+ * the first entry, a temperature that is not positive is 0, a min_p that is not below 1 is 1, a top_k <= 0 is off).
+ * out_id[B,S] = ids[b * ld_ids + index] (ids nullable: the index itself), out_logp[B,S] = log of the drawn entry's probability among the kept;
+ * a row without an entry: -1, -inf.  Weights are double, rounded once to multiples of 2^-62, and summed as integers: no result depends on an
+ * order of additions.  n < 2^31. */
+int ur_sample_scores(const void* scores, int32_t score_type, int64_t n, int64_t ld, int32_t B, const float* rand, int32_t S, double temperature,
+                     int32_t top_k, double top_p, double min_p, const float* temperature_rows, const int32_t* top_k_rows,
+                     const float* top_p_rows, const float* min_p_rows, const int64_t* ids, int64_t ld_ids, int64_t* out_id, float* out_logp,
+                     void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * Live profiler (measurement only; no reference counterpart).  While enabled, every launch group is
  * bracketed by HIP events on its stream.  ur_prof_read fills three host arrays of ur_prof_num_classes()
  * entries: summed milliseconds, number of launch groups, and summed algorithmic work (flops for the GEMM

@@ -916,6 +916,50 @@ def full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, saved, ite
     return d_user, d_table, d_ib
 
 
+# --------------------------------------------------------------------------------------------- sampling from scores
+def sample_scores(scores, rand, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ids=None):
+    """Draws from softmax(scores / temperature) under top-k, top-p and min-p, one draw per random number -> (index int64, log-probability
+    float32), both shaped like ``rand``.  scores [B,N] float32 / float16 / bfloat16 (rows may be strided, entries of a row may not);
+    rand float32 [B] or [B,S] in [0,1).  temperature / top_p / min_p (float32) and top_k (int32) may be tensors [B], one value per row.
+    ids: int64 [B,N], returned in the place of the index (e.g. full_topk's item ids).  A row of -inf (or NaN): -1, -inf.
+    See include/unirec_amd.h: ur_sample_scores."""
+    who = "sample_scores"
+    if not torch.is_tensor(scores) or scores.dtype not in _lib.DTYPE_IDS or scores.dim() != 2:
+        raise _lib.UnirecAmdError(f"{who}: scores must be a [B, N] tensor of float32 / float16 / bfloat16")
+    if not scores.is_cuda:
+        raise _lib.UnirecAmdError(f"scores: expected a GPU tensor (unirec_amd has no CPU path), got {scores.device}")
+    B, N = scores.shape
+    if B == 0 or N == 0:
+        raise _lib.UnirecAmdError(f"{who}: scores of shape [{B}, {N}]")
+    if N > 1 and scores.stride(1) != 1 or B > 1 and scores.stride(0) < N:
+        raise _lib.UnirecAmdError(f"{who}: scores with strides {scores.stride()}: the entries of a row must be adjacent, rows must not overlap")
+    ld = scores.stride(0) if B > 1 else N
+    _chk(rand, torch.float32, "rand")
+    if rand.dim() not in (1, 2) or rand.shape[0] != B or rand.numel() == 0:
+        raise _lib.UnirecAmdError(f"{who}: rand of shape {tuple(rand.shape)} for {B} rows")
+    rows = []
+    for name, v, dt in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                        ("min_p", min_p, torch.float32)):
+        t = v if torch.is_tensor(v) else None
+        if t is not None:
+            _chk(t, dt, name)
+            if t.numel() != B:
+                raise _lib.UnirecAmdError(f"{who}: {name} has {t.numel()} values for {B} rows")
+        rows.append(t)
+    if ids is not None:
+        _chk(ids, torch.int64, "ids")
+        if ids.shape != scores.shape:
+            raise _lib.UnirecAmdError(f"{who}: ids of shape {tuple(ids.shape)}, scores of {tuple(scores.shape)}")
+    _same_device(who, scores, rand, ids, *rows)
+    index = torch.empty(rand.shape, dtype=torch.int64, device=scores.device)
+    logp = torch.empty(rand.shape, dtype=torch.float32, device=scores.device)
+    check(lib.ur_sample_scores(_p(scores), _lib.DTYPE_IDS[scores.dtype], N, ld, B, _p(rand), rand.numel() // B,
+                               1.0 if rows[0] is not None else float(temperature), 0 if rows[1] is not None else int(top_k),
+                               1.0 if rows[2] is not None else float(top_p), 0.0 if rows[3] is not None else float(min_p),
+                               _p(rows[0]), _p(rows[1]), _p(rows[2]), _p(rows[3]), _p(ids), N, _p(index), _p(logp), _stream()), "ur_sample_scores")
+    return index, logp
+
+
 def rows_scatter_add(pl: RowsPlan, rows, dense):
     check(lib.ur_rows_scatter_add(_p(pl.uniq_idx), _p(pl.n_uniq), pl.n, _p(rows), rows.shape[1], _p(dense), _stream()), "ur_rows_scatter_add")
 

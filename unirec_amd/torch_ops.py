@@ -352,6 +352,18 @@ def _(user_emb, item_table, loss_out, lse, row_stat, coef, entry_id, d_unit, ws,
     return torch.empty_like(user_emb), torch.empty_like(item_table), user_emb.new_empty((item_table.shape[0] if item_bias is not None else 0,))
 
 
+# ------------------------------------------------------------------------------------------------ sampling from scores
+@custom_op(f"{NS}::sample_scores", mutates_args=())
+def sample_scores(scores: torch.Tensor, rand: torch.Tensor, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0, min_p: float = 0.0,
+                  ids: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    return ops.sample_scores(scores, rand, temperature, top_k, top_p, min_p, ids)
+
+
+@sample_scores.register_fake
+def _(scores, rand, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, ids=None):
+    return rand.new_empty(rand.shape, dtype=torch.int64), torch.empty_like(rand)
+
+
 # ------------------------------------------------------------------------------------------------ header symbol <-> op
 HEADER_TO_OP = {
     "ur_embedding_gather_f32": "embedding_gather",
@@ -378,6 +390,7 @@ HEADER_TO_OP = {
     "ur_full_topk": "full_topk",
     "ur_full_distill_fwd": "full_distill_fwd",
     "ur_full_distill_bwd": "full_distill_bwd",
+    "ur_sample_scores": "sample_scores",
 }
 
 _QUERY = "layout / workspace-size query or error plumbing: plain host function, nothing to dispatch"
