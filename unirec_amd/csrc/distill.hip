@@ -19,12 +19,13 @@
 namespace ur {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
 constexpr float DS_LOG2E = 1.44269504088896340736f, DS_LN2 = 0.69314718055994530942f;
-constexpr int DS_TILE = 32;      // stream rows of a stage
 constexpr int DS_MAX_D = 256;
 
 // ---- fp32 products on the fp16 matrix pipes.  x 2^k = hi + lo with hi = fp16(x 2^k), lo = fp16(x 2^k - hi): 22 bits of every value that
@@ -40,9 +41,10 @@ __device__ __forceinline__ float finite_abs(float x) {   // |x|, 0 for infinitie
   const float a = fabsf(x);
   return a <= 3.402823466e38f ? a : 0.f;
 }
-__device__ __forceinline__ void split2(float x, _Float16& hi, _Float16& lo) {
-  hi = (_Float16)x;
-  lo = (_Float16)(x - (float)hi);
+// two values at a time: v_cvt_pk_f16_f32 and v_fma_mix_f32 (the residual in one instruction), 3 VALU slots a value, 2 without the scale
+__device__ __forceinline__ void split_pair(float x, float y, float up, half2_t& hi, half2_t& lo) {
+  hi = __builtin_convertvector((float2_t){x * up, y * up}, half2_t);
+  lo = __builtin_convertvector((float2_t){fmaf(x, up, -(float)hi[0]), fmaf(y, up, -(float)hi[1])}, half2_t);
 }
 
 struct DistillStream {
@@ -65,22 +67,26 @@ __device__ __forceinline__ float distill_scale(const float* loss_out, const floa
 }
 
 // One wave owns 32 rows of X (lane & 31 = its row, for good: as the B operand of both products and the column of both results), held as
-// split fragments in registers; the workgroup streams tiles of 32 rows of Y through LDS.
+// split fragments in registers; the workgroup streams tiles of 32 rows of Y (64 with eight waves: a wave stages 8 rows) through LDS.
 //   product 1: S^T [32 stream, 32 owner] = Y X^T     -> a lane has 16 stream rows of ONE owner: maximum and sum are lane-local
 //   product 2: O^T [d, 32 owner] += Y^T W            -> W is the B operand as it stands in the registers (the order of the stream rows
 //              inside a K step is free: Y^T is fetched in the same order, transposed on the way out of LDS by ds_read_b64_tr_b16)
-// so the running maximum, the rescale and the final scale are per-lane scalars.
+// so the running maximum, the rescale and the final scale are per-lane scalars.  Two LDS stages, one barrier a tile: the next tile's rows
+// are requested before the products of this one and split into the other stage behind them.
+constexpr int ds_rows(int nw) { return nw == 8 ? 64 : 32; }
+
 template <int D, int NW, bool FWD, bool GRAD, bool CLIP>
-__global__ __launch_bounds__(NW * 64) void distill_stream_kernel(DistillStream a) {
+__global__ __launch_bounds__(NW * 64, D <= 128 && NW >= 4 ? 2 : 1) void distill_stream_kernel(DistillStream a) {
   constexpr int KS = D / 16, DB = D / 32, LS = D + 8;            // LS: row stride in halves, 16 bytes of padding (b128 reads conflict-free)
   constexpr int F4 = D / 4, PER = 2 * D / 64;                    // float4 of a row; float4 a lane stages of 8 rows
-  __shared__ __attribute__((aligned(16))) _Float16 Yh[DS_TILE * LS], Yl[DS_TILE * LS];
-  __shared__ __attribute__((aligned(16))) float rb_s[DS_TILE];
-  __shared__ int ky_s[4];
+  constexpr int TR = ds_rows(NW), GW = TR / 8 / NW;              // stream rows of a stage; groups of 8 rows a wave stages
+  __shared__ __attribute__((aligned(16))) _Float16 Ys[2][2][TR * LS];
+  __shared__ __attribute__((aligned(16))) float rb_s[2][TR];
+  __shared__ int ky_s[2][TR / 8];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
   // all owner blocks of one split sit on one XCD at neighbouring ids: the stream rows they share come from HBM into one L2 once
   int ob = blockIdx.x;
-  long long t0 = 0, t1 = (a.ny + DS_TILE - 1) / DS_TILE;
+  long long t0 = 0, t1 = (a.ny + TR - 1) / TR;
   int split = 0;
   if constexpr (FWD) {
     const int xcd = blockIdx.x & 7, q = blockIdx.x >> 3;
@@ -92,6 +98,52 @@ __global__ __launch_bounds__(NW * 64) void distill_stream_kernel(DistillStream a
   const long long own = ((long long)ob * NW + wave) * 32 + col;
   const bool live = own < a.nx;
 
+  // ---- staging: lane = (row sr of the group, columns sc .. sc + 3), rows sr + p * 64 / F4
+  const int sr = lane / F4, sc = (lane % F4) * 4;
+  const bool son = sc < a.d;
+  float4 v[GW][PER];
+  auto request = [&](long long tile) {
+#pragma unroll
+    for (int g = 0; g < GW; ++g)
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const long long y = min(tile * TR + (g * NW + wave) * 8 + sr + p * (64 / F4), a.ny - 1);   // (behind the end: the last row again, its bias is -inf)
+        v[g][p] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (son) v[g][p] = *(const float4*)(a.Y + y * a.d + sc);
+      }
+  };
+  auto stage = [&](long long tile, int buf) {
+#pragma unroll
+    for (int g = 0; g < GW; ++g) {
+      const int grp = g * NW + wave;
+      float mx = 0.f;
+#pragma unroll
+      for (int p = 0; p < PER; ++p) mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v[g][p].x)), fmaxf(fabsf(v[g][p].y), fabsf(v[g][p].z))), fabsf(v[g][p].w));
+      const int ky = group_exponent(group_max<64>(mx));
+      const float up = pow2i(ky);
+#pragma unroll
+      for (int p = 0; p < PER; ++p) {
+        const int at = (grp * 8 + sr + p * (64 / F4)) * LS + sc;
+        half2_t h0, h1, l0, l1;
+        split_pair(v[g][p].x, v[g][p].y, up, h0, l0);
+        split_pair(v[g][p].z, v[g][p].w, up, h1, l1);
+        *(half4*)(&Ys[buf][0][at]) = (half4){h0[0], h0[1], h1[0], h1[1]};
+        *(half4*)(&Ys[buf][1][at]) = (half4){l0[0], l0[1], l1[0], l1[1]};
+      }
+      if (lane == 0) ky_s[buf][grp] = ky;
+      if (lane < 8) {
+        const long long y = tile * TR + grp * 8 + lane;
+        float rb = -INFINITY;                                    // rows behind the end carry no weight
+        if (y < a.ny) {
+          if constexpr (FWD) rb = a.y_bias ? a.y_bias[y] * a.cz : 0.f;
+          else rb = -a.row_stat[2 * (long long)a.B + y];
+        }
+        rb_s[buf][grp * 8 + lane] = rb;
+      }
+    }
+  };
+  if (t0 < t1) request(t0);
+
   // ---- owner fragments: lane (col, h) holds x[16 t + 8 h .. + 8] of its row for every K step t
   half8 xh[KS], xl[KS];
   float fl;
@@ -100,11 +152,11 @@ __global__ __launch_bounds__(NW * 64) void distill_stream_kernel(DistillStream a
 #pragma unroll
     for (int t = 0; t < KS; ++t) {
       const int c = 16 * t + 8 * h;
-      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
       if (live && c < a.d) u = *(const float4*)(a.X + own * a.d + c);
-      if (live && c + 4 < a.d) v = *(const float4*)(a.X + own * a.d + c + 4);
+      if (live && c + 4 < a.d) w = *(const float4*)(a.X + own * a.d + c + 4);
       mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(u.x), finite_abs(u.y)), fmaxf(finite_abs(u.z), finite_abs(u.w))));
-      mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(v.x), finite_abs(v.y)), fmaxf(finite_abs(v.z), finite_abs(v.w))));
+      mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(w.x), finite_abs(w.y)), fmaxf(finite_abs(w.z), finite_abs(w.w))));
     }
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     const int kx = group_exponent(mx);
@@ -113,16 +165,16 @@ __global__ __launch_bounds__(NW * 64) void distill_stream_kernel(DistillStream a
 #pragma unroll
     for (int t = 0; t < KS; ++t) {
       const int c = 16 * t + 8 * h;
-      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), v = u;
+      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
       if (live && c < a.d) u = *(const float4*)(a.X + own * a.d + c);
-      if (live && c + 4 < a.d) v = *(const float4*)(a.X + own * a.d + c + 4);
-      const float x[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      if (live && c + 4 < a.d) w = *(const float4*)(a.X + own * a.d + c + 4);
+      const float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        _Float16 hi, lo;
-        split2(x[j] * up, hi, lo);
-        xh[t][j] = hi;
-        xl[t][j] = lo;
+      for (int j = 0; j < 8; j += 2) {
+        half2_t hi, lo;
+        split_pair(x[j], x[j + 1], up, hi, lo);
+        xh[t][j] = hi[0]; xh[t][j + 1] = hi[1];
+        xl[t][j] = lo[0]; xl[t][j + 1] = lo[1];
       }
     }
   }
@@ -139,52 +191,9 @@ __global__ __launch_bounds__(NW * 64) void distill_stream_kernel(DistillStream a
       for (int r = 0; r < 16; ++r) O[b][r] = 0.f;
   }
 
-  for (long long tile = t0; tile < t1; ++tile) {
-    const long long y0 = tile * DS_TILE;
-    __syncthreads();
-    // ---- stage: a wave takes groups of 8 rows, one exponent a group
-#pragma unroll
-    for (int gq = 0; gq < 4; ++gq) {
-      if ((gq & (NW - 1)) != (NW >= 4 ? wave & 3 : wave) || wave >= 4) continue;
-      float4 v[PER];
-      float mx = 0.f;
-#pragma unroll
-      for (int p = 0; p < PER; ++p) {
-        const int idx = lane + 64 * p, row = gq * 8 + idx / F4, c = (idx % F4) * 4;
-        v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (y0 + row < a.ny && c < a.d) v[p] = *(const float4*)(a.Y + (y0 + row) * a.d + c);
-        mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(v[p].x), finite_abs(v[p].y)), fmaxf(finite_abs(v[p].z), finite_abs(v[p].w))));
-      }
-      mx = group_max<64>(mx);
-      const int ky = group_exponent(mx);
-      const float up = pow2i(ky);
-#pragma unroll
-      for (int p = 0; p < PER; ++p) {
-        const int idx = lane + 64 * p, row = gq * 8 + idx / F4, c = (idx % F4) * 4;
-        const float x[4] = {v[p].x, v[p].y, v[p].z, v[p].w};
-        half4 hi4, lo4;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          _Float16 hi, lo;
-          split2(x[j] * up, hi, lo);
-          hi4[j] = hi;
-          lo4[j] = lo;
-        }
-        *(half4*)(Yh + row * LS + c) = hi4;
-        *(half4*)(Yl + row * LS + c) = lo4;
-      }
-      if (lane == 0) ky_s[gq] = ky;
-      if (lane < 8) {
-        const long long y = y0 + gq * 8 + lane;
-        float rb = -INFINITY;                                    // rows behind the end carry no weight
-        if (y < a.ny) {
-          if constexpr (FWD) rb = a.y_bias ? a.y_bias[y] * a.cz : 0.f;
-          else rb = -a.row_stat[2 * (long long)a.B + y];
-        }
-        rb_s[gq * 8 + lane] = rb;
-      }
-    }
-    __syncthreads();
+  auto compute = [&](long long tile, int buf, int sub) {
+    const long long y0 = tile * TR + sub * 32;
+    const _Float16 *Yh = &Ys[buf][0][sub * 32 * LS], *Yl = &Ys[buf][1][sub * 32 * LS];
     // ---- product 1
     floatx16 S;
 #pragma unroll
@@ -203,9 +212,9 @@ __global__ __launch_bounds__(NW * 64) void distill_stream_kernel(DistillStream a
     float tmax = -INFINITY;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      ky[q] = ky_s[q];
+      ky[q] = __builtin_amdgcn_readfirstlane(ky_s[buf][sub * 4 + q]);
       const float fq = fl * pow2i(-ky[q]);
-      const float4 rb = *(const float4*)(rb_s + 8 * q + 4 * h);
+      const float4 rb = *(const float4*)(&rb_s[buf][sub * 32 + 8 * q + 4 * h]);
       const float rbv[4] = {rb.x, rb.y, rb.z, rb.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -219,8 +228,8 @@ __global__ __launch_bounds__(NW * 64) void distill_stream_kernel(DistillStream a
           if constexpr (FWD) z[r] = y0 + 8 * q + 4 * h + i < a.ny ? c : -INFINITY;
           else z[r] = c + rbv[i];
         }
-        tmax = fmaxf(tmax, z[r]);
       }
+      tmax = fmaxf(fmaxf(tmax, fmaxf(z[4 * q], z[4 * q + 1])), fmaxf(z[4 * q + 2], z[4 * q + 3]));
     }
     const int kmin = min(min(ky[0], ky[1]), min(ky[2], ky[3])) + 6;
     // ---- a new reference only when a weight would pass 2^8 (or a larger group arrives): weights reach 2^(8 + 6) = fp16's range
@@ -242,22 +251,25 @@ __global__ __launch_bounds__(NW * 64) void distill_stream_kernel(DistillStream a
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float mk = M - (float)(kappa - ky[q]);
-      float lq = 0.f;
+      float w[4], lq = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int r = 4 * q + i;
-        float w = __builtin_amdgcn_exp2f(z[r] - mk);
-        if constexpr (CLIP && !FWD) w = in[r] ? w : 0.f;
-        lq += w;
-        if constexpr (CLIP && FWD) w = in[r] ? w : 0.f;
-        if constexpr (GRAD) {
-          _Float16 hi, lo;
-          split2(w, hi, lo);
-          wh[r >> 3][r & 7] = hi;
-          wl[r >> 3][r & 7] = lo;
-        }
+        w[i] = __builtin_amdgcn_exp2f(z[r] - mk);
+        if constexpr (CLIP && !FWD) w[i] = in[r] ? w[i] : 0.f;
+        lq += w[i];
+        if constexpr (CLIP && FWD) w[i] = in[r] ? w[i] : 0.f;
       }
       l = fmaf(lq, pow2i(ky[q] - kappa), l);
+      if constexpr (GRAD) {
+#pragma unroll
+        for (int i = 0; i < 4; i += 2) {
+          half2_t hi, lo;
+          split_pair(w[i], w[i + 1], 1.f, hi, lo);
+          wh[q >> 1][4 * (q & 1) + i] = hi[0]; wh[q >> 1][4 * (q & 1) + i + 1] = hi[1];
+          wl[q >> 1][4 * (q & 1) + i] = lo[0]; wl[q >> 1][4 * (q & 1) + i + 1] = lo[1];
+        }
+      }
     }
     // ---- product 2
     if constexpr (GRAD) {
@@ -280,6 +292,16 @@ __global__ __launch_bounds__(NW * 64) void distill_stream_kernel(DistillStream a
           O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(yh, wh[t], O[b], 0, 0, 0);
         }
     }
+  };
+  if (t0 < t1) stage(t0, 0);
+  __syncthreads();
+  int buf = 0;
+  for (long long tile = t0; tile < t1; ++tile, buf ^= 1) {
+    if (tile + 1 < t1) request(tile + 1);
+#pragma unroll
+    for (int sub = 0; sub < TR / 32; ++sub) compute(tile, buf, sub);
+    if (tile + 1 < t1) stage(tile + 1, buf ^ 1);                 // (its last readers passed the barrier of the tile before)
+    __syncthreads();
   }
   // ---- out
   l += __shfl_xor(l, 32, 64);
@@ -509,14 +531,14 @@ __global__ __launch_bounds__(256) void distill_apply_kernel(DistillApply a) {
 }
 
 static inline int ds_tpr(int d) { return d <= 64 ? 16 : d <= 128 ? 32 : 64; }
-static inline int ds_nw(int B) { return B <= 32 ? 1 : B <= 64 ? 2 : 4; }
+static inline int ds_nw(int B, int d) { return B <= 32 ? 1 : B <= 64 ? 2 : B <= 128 || d > 128 ? 4 : 8; }
 
 // the catalogue is cut into splits (a multiple of the 8 XCDs) so that about two workgroups per CU are in flight
-static void ds_splits(int B, long long N, int* owner_blocks, int* splits, long long* per) {
-  const int nw = ds_nw(B);
+static void ds_splits(int B, int d, long long N, int* owner_blocks, int* splits, long long* per) {
+  const int nw = ds_nw(B, d);
   *owner_blocks = cdiv(B, 32 * nw);
-  const long long tiles = (N + DS_TILE - 1) / DS_TILE;
-  const long long want = std::max<long long>(1, 512 * (4 / nw) / *owner_blocks);
+  const long long tiles = (N + ds_rows(nw) - 1) / ds_rows(nw);
+  const long long want = std::max<long long>(1, 2048 / nw / *owner_blocks);
   long long s = std::min(want, (tiles + 1) / 2);
   s = std::max<long long>(8, (s + 7) / 8 * 8);
   *per = (tiles + s - 1) / s;
@@ -538,7 +560,7 @@ static DistillWs ds_carve(int B, int d, long long N, int K, int grad, char* base
   };
   int ob, splits;
   long long per;
-  ds_splits(B, N, &ob, &splits, &per);
+  ds_splits(B, d, N, &ob, &splits, &per);
   w.part_m = (float*)take((int64_t)splits * B * 4);
   w.part_l = (float*)take((int64_t)splits * B * 4);
   if (grad) {
@@ -562,10 +584,12 @@ static int ds_launch_stream(const DistillStream& a, bool clip, int grid, hipStre
 }
 template <int D>
 static int ds_launch_fwd(const DistillStream& a, bool grad, bool clip, int nw, int grid, hipStream_t st) {
-  if (grad) return nw == 1 ? ds_launch_stream<D, 1, true, true>(a, clip, grid, st) : nw == 2 ? ds_launch_stream<D, 2, true, true>(a, clip, grid, st)
-                                                                                  : ds_launch_stream<D, 4, true, true>(a, clip, grid, st);
-  return nw == 1 ? ds_launch_stream<D, 1, true, false>(a, clip, grid, st) : nw == 2 ? ds_launch_stream<D, 2, true, false>(a, clip, grid, st)
-                                                                         : ds_launch_stream<D, 4, true, false>(a, clip, grid, st);
+#define GO(W) (grad ? ds_launch_stream<D, W, true, true>(a, clip, grid, st) : ds_launch_stream<D, W, true, false>(a, clip, grid, st))
+  if constexpr (D <= 128) {
+    if (nw == 8) return GO(8);
+  }
+  return nw == 1 ? GO(1) : nw == 2 ? GO(2) : GO(4);
+#undef GO
 }
 
 static int ds_check(const float* user_emb, const float* table, int64_t N, int B, int d, int K, float tau, float T, const char* who) {
@@ -604,9 +628,9 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   DistillStream a{};
   a.X = user_emb; a.nx = B; a.Y = item_table; a.ny = n_items; a.d = d; a.y_bias = item_bias; a.B = B;
   a.cz = DS_LOG2E / (tau * temperature); a.clip2 = score_clip > 0.f ? score_clip / temperature * DS_LOG2E : 0.f;
-  ds_splits(B, n_items, &a.owner_blocks, &a.splits, &a.tiles_per_split);
+  ds_splits(B, d, n_items, &a.owner_blocks, &a.splits, &a.tiles_per_split);
   a.part_m = w.part_m; a.part_l = w.part_l; a.part_o = w.part_o;
-  const int nw = ds_nw(B), grid = a.owner_blocks * a.splits;
+  const int nw = ds_nw(B, d), grid = a.owner_blocks * a.splits;
   const bool clip = score_clip > 0.f;
   rc = d <= 32 ? ds_launch_fwd<32>(a, grad, clip, nw, grid, st) : d <= 64 ? ds_launch_fwd<64>(a, grad, clip, nw, grid, st)
      : d <= 128 ? ds_launch_fwd<128>(a, grad, clip, nw, grid, st) : ds_launch_fwd<256>(a, grad, clip, nw, grid, st);
