@@ -12,13 +12,14 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 #include "kernels.h"
 
 namespace ur {
 
-typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
@@ -47,12 +48,23 @@ __device__ __forceinline__ void split_pair(float x, float y, float up, half2_t& 
   lo = __builtin_convertvector((float2_t){fmaf(x, up, -(float)hi[0]), fmaf(y, up, -(float)hi[1])}, half2_t);
 }
 
+// ---- a tile of 32 stream rows, split: [hi | lo][32][D] halves.  Rows are not padded; the 16-byte units of row r are permuted by XOR with
+// ds_swizzle(r), which keeps both readers free of bank conflicts: the 8 consecutive rows of a b128 read and the 4 rows x 32 bytes of a
+// transposing read land in 8 different 16-byte bank groups.
+constexpr int DS_TILE = 32;
+template <int D>
+__device__ __forceinline__ int ds_swizzle(int r) {
+  return D >= 64 ? ((r & 3) << 1) | ((r >> 2) & 1) : (((r >> 1) & 1) << 1) | ((r >> 2) & 1);
+}
+template <int D>
+__device__ __forceinline__ int ds_at(int r, int c) { return r * D + (((c >> 3) ^ ds_swizzle<D>(r)) << 3) + (c & 7); }
+
 struct DistillStream {
   const float* X; long long nx;        // owner rows [nx, d]
-  const float* Y; long long ny;        // stream rows [ny, d]
+  const float* Y; long long ny;        // stream rows [ny, d] (forward; the backward's come from the image)
   int d;
-  const float* y_bias;                 // added to the log2 score of a stream row (forward: item bias * cz; nullable)
-  const float* row_stat; int B;        // backward: the forward's per-user statistics, row_stat[2 B + b] = log2 sum_n 2^s2 (+inf: no teacher)
+  const float* y_bias;                 // forward: added to the log2 score of a stream row (item bias * cz; nullable)
+  const _Float16* img; const float* rb_img; const int* ky_img;   // backward: the users' rows split tile by tile, their bias, a tile's exponent
   const float* x_bias;                 // backward: item bias of an owner row (* cz; nullable)
   float cz;                            // log2(e) / (tau T): dot + bias -> log2 units
   float clip2;                         // score_clip / T in log2 units
@@ -66,27 +78,32 @@ __device__ __forceinline__ float distill_scale(const float* loss_out, const floa
   return g_num * (d_loss ? d_loss[0] : 1.f) / fmaxf(loss_out[1], 1.f);
 }
 
-// One wave owns 32 rows of X (lane & 31 = its row, for good: as the B operand of both products and the column of both results), held as
-// split fragments in registers; the workgroup streams tiles of 32 rows of Y (64 with eight waves: a wave stages 8 rows) through LDS.
-//   product 1: S^T [32 stream, 32 owner] = Y X^T     -> a lane has 16 stream rows of ONE owner: maximum and sum are lane-local
+// One wave owns 32 rows of X as two column blocks of 16 (lane & 15 = the row of a block, for good: the B operand of both products and the
+// column of both results), held as split fragments in registers; the workgroup streams tiles of 32 rows of Y through LDS.
+//   product 1: S^T [32 stream, 32 owner] = Y X^T     -> a lane has 8 stream rows (16 rb + 4 (lane >> 4) + r) of each of TWO owners
 //   product 2: O^T [d, 32 owner] += Y^T W            -> W is the B operand as it stands in the registers (the order of the stream rows
 //              inside a K step is free: Y^T is fetched in the same order, transposed on the way out of LDS by ds_read_b64_tr_b16)
-// so the running maximum, the rescale and the final scale are per-lane scalars.  Two LDS stages, one barrier a tile: the next tile's rows
-// are requested before the products of this one and split into the other stage behind them.
-constexpr int ds_rows(int nw) { return nw == 8 ? 64 : 32; }
+// so the running maximum, the rescale and the final scale are per-lane.  v_mfma_f32_16x16x32_f16 rather than 32x32x16: the same flops
+// ran at 2 050 - 2 160 TFLOP/s against 1 720 - 1 820 in a loop of nothing else (the part is power-limited there).
+// Three LDS stages, one barrier a tile: while the weights of tile t are made (VALU), product 1 of tile t + 1 runs on the matrix pipe, and
+// tile t + 2 or t + 3 arrives (forward: fp32 rows through registers, split here with one exponent a tile, which the waves agree on a
+// barrier ahead; backward: the image's bytes straight into LDS).
+typedef __attribute__((address_space(1))) const void* ds_gptr;
+typedef __attribute__((address_space(3))) void* ds_lptr;
 
 template <int D, int NW, bool FWD, bool GRAD, bool CLIP>
 __global__ __launch_bounds__(NW * 64, D <= 128 && NW >= 4 ? 2 : 1) void distill_stream_kernel(DistillStream a) {
-  constexpr int KS = D / 16, DB = D / 32, LS = D + 8;            // LS: row stride in halves, 16 bytes of padding (b128 reads conflict-free)
-  constexpr int F4 = D / 4, PER = 2 * D / 64;                    // float4 of a row; float4 a lane stages of 8 rows
-  constexpr int TR = ds_rows(NW), GW = TR / 8 / NW;              // stream rows of a stage; groups of 8 rows a wave stages
-  __shared__ __attribute__((aligned(16))) _Float16 Ys[2][2][TR * LS];
-  __shared__ __attribute__((aligned(16))) float rb_s[2][TR];
-  __shared__ int ky_s[2][TR / 8];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 31, h = lane >> 5;
+  constexpr int KS = D / 32, DB = D / 16;                        // K steps of product 1; 16-column blocks of product 2
+  constexpr int N1 = 2 * KS, N1a = N1 > 4 ? 2 : 1;               // steps of product 1 (K step, row block); those in front of the maximum
+  constexpr int F4 = D / 4, PER = DS_TILE * F4 / (64 * NW);      // float4 of a row; float4 a thread stages of a tile
+  constexpr int HALF = DS_TILE * D;                              // lo plane, in halves behind the hi plane
+  __shared__ __attribute__((aligned(1024))) _Float16 Ys[3][2 * HALF];
+  __shared__ __attribute__((aligned(16))) float rb_s[3][DS_TILE];
+  __shared__ int kw_s[2][NW];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, g = lane >> 4;
   // all owner blocks of one split sit on one XCD at neighbouring ids: the stream rows they share come from HBM into one L2 once
   int ob = blockIdx.x;
-  long long t0 = 0, t1 = (a.ny + TR - 1) / TR;
+  long long t0 = 0, t1 = (a.ny + DS_TILE - 1) / DS_TILE;
   int split = 0;
   if constexpr (FWD) {
     const int xcd = blockIdx.x & 7, q = blockIdx.x >> 3;
@@ -95,247 +112,380 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && NW >= 4 ? 2 : 1) void distill_
     t0 = split * a.tiles_per_split;
     t1 = min(t1, t0 + a.tiles_per_split);
   }
-  const long long own = ((long long)ob * NW + wave) * 32 + col;
-  const bool live = own < a.nx;
+  const long long own0 = ((long long)ob * NW + wave) * 32 + col;   // and own0 + 16
 
-  // ---- staging: lane = (row sr of the group, columns sc .. sc + 3), rows sr + p * 64 / F4
-  const int sr = lane / F4, sc = (lane % F4) * 4;
+  // ---- staging, forward: thread = (row sr + p * 64 NW / F4, columns sc .. sc + 3)
+  const int sr = threadIdx.x / F4, sc = (threadIdx.x % F4) * 4;
   const bool son = sc < a.d;
-  float4 v[GW][PER];
-  auto request = [&](long long tile) {
-#pragma unroll
-    for (int g = 0; g < GW; ++g)
-#pragma unroll
-      for (int p = 0; p < PER; ++p) {
-        const long long y = min(tile * TR + (g * NW + wave) * 8 + sr + p * (64 / F4), a.ny - 1);   // (behind the end: the last row again, its bias is -inf)
-        v[g][p] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (son) v[g][p] = *(const float4*)(a.Y + y * a.d + sc);
-      }
-  };
-  auto stage = [&](long long tile, int buf) {
-#pragma unroll
-    for (int g = 0; g < GW; ++g) {
-      const int grp = g * NW + wave;
-      float mx = 0.f;
-#pragma unroll
-      for (int p = 0; p < PER; ++p) mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v[g][p].x)), fmaxf(fabsf(v[g][p].y), fabsf(v[g][p].z))), fabsf(v[g][p].w));
-      const int ky = group_exponent(group_max<64>(mx));
-      const float up = pow2i(ky);
+  float4 v[FWD ? PER : 1];
+  float rb_next = 0.f;
+  auto request = [&](long long tile, int buf) {
+    if constexpr (FWD) {
 #pragma unroll
       for (int p = 0; p < PER; ++p) {
-        const int at = (grp * 8 + sr + p * (64 / F4)) * LS + sc;
-        half2_t h0, h1, l0, l1;
-        split_pair(v[g][p].x, v[g][p].y, up, h0, l0);
-        split_pair(v[g][p].z, v[g][p].w, up, h1, l1);
-        *(half4*)(&Ys[buf][0][at]) = (half4){h0[0], h0[1], h1[0], h1[1]};
-        *(half4*)(&Ys[buf][1][at]) = (half4){l0[0], l0[1], l1[0], l1[1]};
+        const long long y = min(tile * DS_TILE + sr + p * (64 * NW / F4), a.ny - 1);   // (behind the end: the last row again, its bias is -inf)
+        v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (son) v[p] = *(const float4*)(a.Y + y * a.d + sc);
       }
-      if (lane == 0) ky_s[buf][grp] = ky;
-      if (lane < 8) {
-        const long long y = tile * TR + grp * 8 + lane;
-        float rb = -INFINITY;                                    // rows behind the end carry no weight
-        if (y < a.ny) {
-          if constexpr (FWD) rb = a.y_bias ? a.y_bias[y] * a.cz : 0.f;
-          else rb = -a.row_stat[2 * (long long)a.B + y];
-        }
-        rb_s[buf][grp * 8 + lane] = rb;
+      if (threadIdx.x < DS_TILE) {
+        const long long y = tile * DS_TILE + threadIdx.x;
+        rb_next = y < a.ny ? (a.y_bias ? a.y_bias[y] * a.cz : 0.f) : -INFINITY;        // rows behind the end carry no weight
       }
+    } else {
+      const char* src = (const char*)(a.img + tile * (2 * HALF)) + lane * 16;
+      char* dst = (char*)&Ys[buf][0];
+#pragma unroll
+      for (int i = 0; i < 4 * HALF / 1024 / NW; ++i) {
+        const int piece = (i * NW + wave) * 1024;
+        __builtin_amdgcn_global_load_lds((ds_gptr)(src + piece), (ds_lptr)(dst + piece), 16, 0, 0);
+      }
+      if (threadIdx.x < DS_TILE) rb_next = a.rb_img[tile * DS_TILE + threadIdx.x];
     }
   };
-  if (t0 < t1) request(t0);
+  auto publish = [&](int par) {   // this wave's exponent for the rows it holds
+    float mx = 0.f;
+#pragma unroll
+    for (int p = 0; p < PER; ++p) mx = fmaxf(fmaxf(fmaxf(mx, fabsf(v[p].x)), fmaxf(fabsf(v[p].y), fabsf(v[p].z))), fabsf(v[p].w));
+    mx = group_max<64>(mx);
+    if (lane == 0) kw_s[par][wave] = group_exponent(mx);
+  };
+  auto agreed = [&](int par) {
+    int k = kw_s[par][0];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) k = min(k, kw_s[par][w]);
+    return __builtin_amdgcn_readfirstlane(k);
+  };
+  auto convert = [&](int buf, int ky) {
+    const float up = pow2i(ky);
+#pragma unroll
+    for (int p = 0; p < PER; ++p) {
+      const int at = ds_at<D>(sr + p * (64 * NW / F4), sc);
+      half2_t h0, h1, l0, l1;
+      split_pair(v[p].x, v[p].y, up, h0, l0);
+      split_pair(v[p].z, v[p].w, up, h1, l1);
+      *(half4*)(&Ys[buf][at]) = (half4){h0[0], h0[1], h1[0], h1[1]};
+      *(half4*)(&Ys[buf][HALF + at]) = (half4){l0[0], l0[1], l1[0], l1[1]};
+    }
+  };
+  auto put_bias = [&](int buf) {
+    if (threadIdx.x < DS_TILE) rb_s[buf][threadIdx.x] = rb_next;
+  };
+  auto arrive = [&]() {   // backward: this wave's bytes are in LDS (the barrier speaks for every wave's)
+    if constexpr (!FWD) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  if (t0 < t1) request(t0, 0);
 
-  // ---- owner fragments: lane (col, h) holds x[16 t + 8 h .. + 8] of its row for every K step t
-  half8 xh[KS], xl[KS];
-  float fl;
-  {
+  // ---- owner fragments: lane (col, g) holds x[32 t + 8 g .. + 8] of its two rows for every K step t
+  half8 xh[2][KS], xl[2][KS];
+  float fl[2], xb[2] = {0.f, 0.f};
+#pragma unroll
+  for (int cb = 0; cb < 2; ++cb) {
+    const long long own = own0 + 16 * cb;
+    const bool live = own < a.nx;
+    float4 u[KS], w[KS];
     float mx = 0.f;
 #pragma unroll
     for (int t = 0; t < KS; ++t) {
-      const int c = 16 * t + 8 * h;
-      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
-      if (live && c < a.d) u = *(const float4*)(a.X + own * a.d + c);
-      if (live && c + 4 < a.d) w = *(const float4*)(a.X + own * a.d + c + 4);
-      mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(u.x), finite_abs(u.y)), fmaxf(finite_abs(u.z), finite_abs(u.w))));
-      mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(w.x), finite_abs(w.y)), fmaxf(finite_abs(w.z), finite_abs(w.w))));
+      const int c = 32 * t + 8 * g;
+      u[t] = w[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (live && c < a.d) u[t] = *(const float4*)(a.X + own * a.d + c);
+      if (live && c + 4 < a.d) w[t] = *(const float4*)(a.X + own * a.d + c + 4);
+      mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(u[t].x), finite_abs(u[t].y)), fmaxf(finite_abs(u[t].z), finite_abs(u[t].w))));
+      mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(w[t].x), finite_abs(w[t].y)), fmaxf(finite_abs(w[t].z), finite_abs(w[t].w))));
     }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
     mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
     const int kx = group_exponent(mx);
     const float up = pow2i(kx);
-    fl = a.cz * pow2i(-kx);
+    fl[cb] = a.cz * pow2i(-kx);
 #pragma unroll
     for (int t = 0; t < KS; ++t) {
-      const int c = 16 * t + 8 * h;
-      float4 u = make_float4(0.f, 0.f, 0.f, 0.f), w = u;
-      if (live && c < a.d) u = *(const float4*)(a.X + own * a.d + c);
-      if (live && c + 4 < a.d) w = *(const float4*)(a.X + own * a.d + c + 4);
-      const float x[8] = {u.x, u.y, u.z, u.w, w.x, w.y, w.z, w.w};
+      const float x[8] = {u[t].x, u[t].y, u[t].z, u[t].w, w[t].x, w[t].y, w[t].z, w[t].w};
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
         half2_t hi, lo;
         split_pair(x[j], x[j + 1], up, hi, lo);
-        xh[t][j] = hi[0]; xh[t][j + 1] = hi[1];
-        xl[t][j] = lo[0]; xl[t][j + 1] = lo[1];
+        xh[cb][t][j] = hi[0]; xh[cb][t][j + 1] = hi[1];
+        xl[cb][t][j] = lo[0]; xl[cb][t][j + 1] = lo[1];
       }
     }
+    if constexpr (!FWD) xb[cb] = (live && a.x_bias) ? a.x_bias[own] * a.cz : 0.f;
   }
-  float xb = 0.f;
-  if constexpr (!FWD) xb = (live && a.x_bias) ? a.x_bias[own] * a.cz : 0.f;
 
-  float M = -1e30f, l = 0.f;
-  int kappa = 36;                                                // O is held in units of 2^-kappa: min over the groups seen of k, + 6
-  floatx16 O[GRAD ? DB : 1];
+  float M[2] = {-1e30f, -1e30f}, l[2] = {0.f, 0.f};
+  int kappa = 36;                                                // O is held in units of 2^-kappa: min over the tiles seen of k, + 6
+  floatx4 O[GRAD ? DB : 1][2];
   if constexpr (GRAD) {
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) O[b][r] = 0.f;
+      for (int cb = 0; cb < 2; ++cb) O[b][cb] = (floatx4){0.f, 0.f, 0.f, 0.f};
   }
+  // byte offsets of this lane's fragments inside a tile (K step t: ^ 64 t; row block: + 16 rows; column block b: ^ 32 b)
+  const int frag = 2 * ds_at<D>(col, 8 * g), frag_t = 2 * ds_at<D>(4 * g + (col >> 2), 4 * (col & 3));
 
-  auto compute = [&](long long tile, int buf, int sub) {
-    const long long y0 = tile * TR + sub * 32;
-    const _Float16 *Yh = &Ys[buf][0][sub * 32 * LS], *Yl = &Ys[buf][1][sub * 32 * LS];
-    // ---- product 1
-    floatx16 S;
+  // a fragment pair (hi, lo): step i of product 1 is (K step i >> 1, row block i & 1), step b of product 2 a block of 16 columns
+  auto read1 = [&](int buf, int i, half8& yh, half8& yl) {
+    const char* at = (const char*)&Ys[buf][0] + (frag ^ (64 * (i >> 1))) + (i & 1) * 32 * D;
+    yh = *(const half8*)at;
+    yl = *(const half8*)(at + 2 * HALF);
+  };
+  auto read2 = [&](int buf, int b, half8& yh, half8& yl) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) S[r] = 0.f;
+    for (int rb = 0; rb < 2; ++rb) {
+      const char* at = (const char*)&Ys[buf][0] + (frag_t ^ (32 * b)) + rb * 32 * D;
+      const half4 th = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)at));
+      const half4 tl = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(at + 2 * HALF)));
 #pragma unroll
-    for (int t = 0; t < KS; ++t) {
-      const half8 yh = *(const half8*)(Yh + col * LS + 16 * t + 8 * h), yl = *(const half8*)(Yl + col * LS + 16 * t + 8 * h);
-      S = __builtin_amdgcn_mfma_f32_32x32x16_f16(yl, xh[t], S, 0, 0, 0);
-      S = __builtin_amdgcn_mfma_f32_32x32x16_f16(yh, xl[t], S, 0, 0, 0);
-      S = __builtin_amdgcn_mfma_f32_32x32x16_f16(yh, xh[t], S, 0, 0, 0);
+      for (int j = 0; j < 4; ++j) { yh[4 * rb + j] = th[j]; yl[4 * rb + j] = tl[j]; }
     }
-    // ---- log2 scores: register r is stream row 8 (r >> 2) + 4 h + (r & 3)
-    float z[16];
-    bool in[16];
-    int ky[4];
-    float tmax = -INFINITY;
+  };
+  auto mac = [](floatx4& P0, floatx4& P1, const half8& yh, const half8& yl, const half8& h0, const half8& l0, const half8& h1, const half8& l1) {
+    P0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(yl, h0, P0, 0, 0, 0);
+    P1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(yl, h1, P1, 0, 0, 0);
+    P0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(yh, l0, P0, 0, 0, 0);
+    P1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(yh, l1, P1, 0, 0, 0);
+    P0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(yh, h0, P0, 0, 0, 0);
+    P1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(yh, h1, P1, 0, 0, 0);
+  };
+  struct Scores { floatx4 at[2][2]; };                           // [row block][owner block]
+  auto clear = [](Scores& P) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      ky[q] = __builtin_amdgcn_readfirstlane(ky_s[buf][sub * 4 + q]);
-      const float fq = fl * pow2i(-ky[q]);
-      const float4 rb = *(const float4*)(&rb_s[buf][sub * 32 + 8 * q + 4 * h]);
-      const float rbv[4] = {rb.x, rb.y, rb.z, rb.w};
+    for (int i = 0; i < 4; ++i) P.at[i >> 1][i & 1] = (floatx4){0.f, 0.f, 0.f, 0.f};
+  };
+  auto product1 = [&](Scores& P, int i, const half8& yh, const half8& yl) {
+    mac(P.at[i & 1][0], P.at[i & 1][1], yh, yl, xh[0][i >> 1], xl[0][i >> 1], xh[1][i >> 1], xl[1][i >> 1]);
+  };
+  // one tile: weights of `tile` (exponent ky) from S (stage buf), product 1 of the next one (stage nb, into Sn) beside them, product 2.
+  // Fragments are read one step (six matrix instructions) ahead of their use.
+  auto step = [&](long long tile, int buf, int nb, int ky, Scores& S, Scores& Sn, auto has_next) {
+    constexpr bool NEXT = decltype(has_next)::value;
+    float z[2][8];                                               // [owner block][4 rb + r]: stream row 16 rb + 4 g + r
+    bool in[2][8];
+    float tmax[2] = {-INFINITY, -INFINITY};
+    half8 fh[2], fo[2];                                          // the fragment pair in use and the one on its way
+    if constexpr (NEXT) {
+      read1(nb, 0, fh[0], fo[0]);
+      clear(Sn);
+    }
+    const float down = pow2i(-ky), fq[2] = {fl[0] * down, fl[1] * down};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 4 * q + i;
-        if constexpr (!CLIP) {
-          z[r] = fmaf(S[r], fq, rbv[i]);
-        } else {
-          const float s = fmaf(S[r], fq, FWD ? rbv[i] : xb);
-          const float c = s > a.clip2 ? a.clip2 : (s < -a.clip2 ? -a.clip2 : s);   // (a NaN stays one)
-          in[r] = !(s > a.clip2) && !(s < -a.clip2);
-          if constexpr (FWD) z[r] = y0 + 8 * q + 4 * h + i < a.ny ? c : -INFINITY;
-          else z[r] = c + rbv[i];
+    for (int rb = 0; rb < 2; ++rb) {
+      const float4 rb4 = *(const float4*)(&rb_s[buf][16 * rb + 4 * g]);
+      const float rbv[4] = {rb4.x, rb4.y, rb4.z, rb4.w};
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if constexpr (!CLIP) {
+            z[cb][4 * rb + r] = fmaf(S.at[rb][cb][r], fq[cb], rbv[r]);
+          } else {
+            const float s = fmaf(S.at[rb][cb][r], fq[cb], FWD ? rbv[r] : xb[cb]);
+            const float c = s > a.clip2 ? a.clip2 : (s < -a.clip2 ? -a.clip2 : s);   // (a NaN stays one)
+            in[cb][4 * rb + r] = !(s > a.clip2) && !(s < -a.clip2);
+            if constexpr (FWD) z[cb][4 * rb + r] = tile * DS_TILE + 16 * rb + 4 * g + r < a.ny ? c : -INFINITY;
+            else z[cb][4 * rb + r] = c + rbv[r];
+          }
         }
+        tmax[cb] = fmaxf(fmaxf(tmax[cb], fmaxf(z[cb][4 * rb], z[cb][4 * rb + 1])), fmaxf(z[cb][4 * rb + 2], z[cb][4 * rb + 3]));
       }
-      tmax = fmaxf(fmaxf(tmax, fmaxf(z[4 * q], z[4 * q + 1])), fmaxf(z[4 * q + 2], z[4 * q + 3]));
     }
-    const int kmin = min(min(ky[0], ky[1]), min(ky[2], ky[3])) + 6;
-    // ---- a new reference only when a weight would pass 2^8 (or a larger group arrives): weights reach 2^(8 + 6) = fp16's range
-    if (kmin < kappa || __any(tmax > M + 8.f)) {
-      const float m2 = fmaxf(tmax, __shfl_xor(tmax, 32, 64)), Mn = m2 > M + 8.f ? m2 : M;
-      const int kn = min(kmin, kappa);
-      const float f = __builtin_amdgcn_exp2f(M - Mn), fo = f * exp2f((float)(kn - kappa));
-      l *= f;
-      if constexpr (GRAD) {
+    if constexpr (NEXT) {
 #pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) O[b][r] *= fo;
+      for (int i = 0; i < N1a; ++i) {
+        read1(nb, i + 1, fh[(i + 1) & 1], fo[(i + 1) & 1]);
+        product1(Sn, i, fh[i & 1], fo[i & 1]);
       }
-      M = Mn;
+    }
+    // ---- a new reference only when a weight would pass 2^8 (or a larger tile arrives): weights reach 2^(8 + 6) = fp16's range
+    if (ky + 6 < kappa || __any(fmaxf(tmax[0] - M[0], tmax[1] - M[1]) > 8.f)) {
+      const int kn = min(ky + 6, kappa);
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+        float m2 = fmaxf(tmax[cb], __shfl_xor(tmax[cb], 16, 64));
+        m2 = fmaxf(m2, __shfl_xor(m2, 32, 64));
+        const float Mn = m2 > M[cb] + 8.f ? m2 : M[cb];
+        const float f = __builtin_amdgcn_exp2f(M[cb] - Mn), fk = f * exp2f((float)(kn - kappa));
+        l[cb] *= f;
+        if constexpr (GRAD) {
+#pragma unroll
+          for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[b][cb][r] *= fk;
+        }
+        M[cb] = Mn;
+      }
       kappa = kn;
     }
-    half8 wh[2], wl[2];
+    if constexpr (NEXT) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float mk = M - (float)(kappa - ky[q]);
-      float w[4], lq = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = 4 * q + i;
-        w[i] = __builtin_amdgcn_exp2f(z[r] - mk);
-        if constexpr (CLIP && !FWD) w[i] = in[r] ? w[i] : 0.f;
-        lq += w[i];
-        if constexpr (CLIP && FWD) w[i] = in[r] ? w[i] : 0.f;
+      for (int i = N1a; i < N1; ++i) {
+        if (i + 1 < N1) read1(nb, i + 1, fh[(i + 1) & 1], fo[(i + 1) & 1]);
+        product1(Sn, i, fh[i & 1], fo[i & 1]);
       }
-      l = fmaf(lq, pow2i(ky[q] - kappa), l);
+    }
+    half8 wh[2], wl[2];
+    const float unit = pow2i(ky - kappa);
+#pragma unroll
+    for (int cb = 0; cb < 2; ++cb) {
+      const float mk = M[cb] - (float)(kappa - ky);
+      float w[8], sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        w[j] = __builtin_amdgcn_exp2f(z[cb][j] - mk);
+        if constexpr (CLIP && !FWD) w[j] = in[cb][j] ? w[j] : 0.f;
+        sum += w[j];
+        if constexpr (CLIP && FWD) w[j] = in[cb][j] ? w[j] : 0.f;
+      }
+      l[cb] = fmaf(sum, unit, l[cb]);
       if constexpr (GRAD) {
 #pragma unroll
-        for (int i = 0; i < 4; i += 2) {
+        for (int j = 0; j < 8; j += 2) {
           half2_t hi, lo;
-          split_pair(w[i], w[i + 1], 1.f, hi, lo);
-          wh[q >> 1][4 * (q & 1) + i] = hi[0]; wh[q >> 1][4 * (q & 1) + i + 1] = hi[1];
-          wl[q >> 1][4 * (q & 1) + i] = lo[0]; wl[q >> 1][4 * (q & 1) + i + 1] = lo[1];
+          split_pair(w[j], w[j + 1], 1.f, hi, lo);
+          wh[cb][j] = hi[0]; wh[cb][j + 1] = hi[1];
+          wl[cb][j] = lo[0]; wl[cb][j + 1] = lo[1];
         }
       }
     }
     // ---- product 2
     if constexpr (GRAD) {
-      const int i16 = lane & 15, cg = (lane >> 4) & 1;
+      half8 gh[2], gl[2];
+      read2(buf, 0, gh[0], gl[0]);
 #pragma unroll
-      for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          half8 yh, yl;
-#pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int off = (16 * t + 8 * q + 4 * h + (i16 >> 2)) * LS + 32 * b + 16 * cg + 4 * (i16 & 3);
-            const half4 th = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(Yh + off)));
-            const half4 tl = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)(Yl + off)));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) { yh[4 * q + j] = th[j]; yl[4 * q + j] = tl[j]; }
-          }
-          O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(yl, wh[t], O[b], 0, 0, 0);
-          O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(yh, wl[t], O[b], 0, 0, 0);
-          O[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(yh, wh[t], O[b], 0, 0, 0);
-        }
+      for (int b = 0; b < DB; ++b) {
+        if (b + 1 < DB) read2(buf, b + 1, gh[(b + 1) & 1], gl[(b + 1) & 1]);
+        mac(O[b][0], O[b][1], gh[b & 1], gl[b & 1], wh[0], wl[0], wh[1], wl[1]);
+      }
     }
-  };
-  if (t0 < t1) stage(t0, 0);
-  __syncthreads();
-  int buf = 0;
-  for (long long tile = t0; tile < t1; ++tile, buf ^= 1) {
-    if (tile + 1 < t1) request(tile + 1);
+    // the order the scheduler is asked for, from the branch on: a step's reads, then its six matrix instructions with the weights' VALU
+    // work between them (0x100 LDS reads, 0x8 matrix, 0x2 VALU)
+    if constexpr (NEXT) {
 #pragma unroll
-    for (int sub = 0; sub < TR / 32; ++sub) compute(tile, buf, sub);
-    if (tile + 1 < t1) stage(tile + 1, buf ^ 1);                 // (its last readers passed the barrier of the tile before)
-    __syncthreads();
-  }
-  // ---- out
-  l += __shfl_xor(l, 32, 64);
-  if (!live) return;
-  if constexpr (FWD) {
-    const long long at = (long long)split * a.nx + own;
-    if (h == 0) {
-      a.part_m[at] = M;
-      a.part_l[at] = l;
+      for (int i = N1a; i + 1 < N1; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+#pragma unroll
+        for (int j = 0; j < 6; ++j) {
+          __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+        }
+      }
+      if constexpr (GRAD) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int j = 0; j < 6; ++j) {
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+      }
     }
     if constexpr (GRAD) {
-      const float down = exp2f((float)-kappa);
 #pragma unroll
-      for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int c = 32 * b + 8 * q + 4 * h;
-          if (c < a.d)
-            *(float4*)(a.part_o + at * a.d + c) = make_float4(O[b][4 * q] * down, O[b][4 * q + 1] * down, O[b][4 * q + 2] * down, O[b][4 * q + 3] * down);
-        }
-    }
-  } else {
-    const float g = distill_scale(a.loss_out, a.d_loss, a.g_num), e = CLIP ? 0.f : xb;
-    if (h == 0 && a.d_bias) a.d_bias[own] = l * exp2f(M + e) * g;
-    const float down = own == 0 ? 0.f : exp2f(M + e - (float)kappa) * g;   // padding row: no gradient
-#pragma unroll
-    for (int b = 0; b < DB; ++b)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = 32 * b + 8 * q + 4 * h;
-        if (c < a.d)
-          *(float4*)(a.dX + own * a.d + c) = own == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)
-              : make_float4(O[b][4 * q] * down, O[b][4 * q + 1] * down, O[b][4 * q + 2] * down, O[b][4 * q + 3] * down);
+      for (int b = 0; b + 1 < DB; ++b) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x8, 6, 0);
       }
+    }
+  };
+  if (t0 < t1) {
+    Scores Sa, Sb;
+    int k0 = 0, k1 = 0, k2 = 0, par = 0;                         // exponents of the tile in hand and of the two behind it
+    auto exponent = [&](long long tile) { return FWD ? agreed(par) : a.ky_img[min(tile, t1 - 1)]; };
+    if constexpr (FWD) {
+      publish(0);
+      __syncthreads();
+      k0 = agreed(0);
+      convert(0, k0);
+      put_bias(0);
+      request(t0 + 1, 0);                                        // (behind the last tile: its last row again, never used)
+      publish(1);
+      __syncthreads();
+      k1 = agreed(1);
+      convert(1, k1);
+      put_bias(1);
+      request(t0 + 2, 0);
+      publish(0);
+    } else {
+      put_bias(0);
+      k0 = exponent(t0);
+      if (t0 + 1 < t1) {
+        request(t0 + 1, 1);
+        put_bias(1);
+      }
+      k1 = exponent(t0 + 1);
+    }
+    arrive();
+    clear(Sa);
+#pragma unroll
+    for (int i = 0; i < N1; ++i) {
+      half8 yh, yl;
+      read1(0, i, yh, yl);
+      product1(Sa, i, yh, yl);
+    }
+    int b0 = 0, b1 = 1, b2 = 2;
+    auto advance = [&](long long tile, Scores& S, Scores& Sn) {
+      // (stage b2's last readers passed the barrier of the tile before)
+      if constexpr (FWD) {
+        k2 = agreed(par);
+        par ^= 1;
+        convert(b2, k2);
+        put_bias(b2);
+        request(tile + 3, 0);
+      } else {
+        k2 = exponent(tile + 2);
+        if (tile + 2 < t1) request(tile + 2, b2);
+      }
+      step(tile, b0, b1, k0, S, Sn, std::true_type());
+      if constexpr (FWD) publish(par);
+      else put_bias(b2);
+      arrive();
+      const int b = b0;
+      b0 = b1; b1 = b2; b2 = b;
+      k0 = k1; k1 = k2;
+    };
+    long long tile = t0;
+    for (; tile + 2 < t1; tile += 2) {
+      advance(tile, Sa, Sb);
+      advance(tile + 1, Sb, Sa);
+    }
+    if (tile + 1 < t1) {
+      advance(tile, Sa, Sb);
+      step(tile + 1, b0, b1, k0, Sb, Sa, std::false_type());
+    } else {
+      step(tile, b0, b1, k0, Sa, Sb, std::false_type());
+    }
+  }
+  // ---- out
+#pragma unroll
+  for (int cb = 0; cb < 2; ++cb) {
+    const long long own = own0 + 16 * cb;
+    float lt = l[cb] + __shfl_xor(l[cb], 16, 64);
+    lt += __shfl_xor(lt, 32, 64);
+    if (own >= a.nx) continue;
+    float down;
+    float* out;
+    if constexpr (FWD) {
+      const long long at = (long long)split * a.nx + own;
+      if (g == 0) {
+        a.part_m[at] = M[cb];
+        a.part_l[at] = lt;
+      }
+      down = exp2f((float)-kappa);
+      out = a.part_o + at * a.d;
+    } else {
+      const float gs = distill_scale(a.loss_out, a.d_loss, a.g_num), e = CLIP ? 0.f : xb[cb];
+      if (g == 0 && a.d_bias) a.d_bias[own] = lt * exp2f(M[cb] + e) * gs;
+      down = exp2f(M[cb] + e - (float)kappa) * gs;
+      out = a.dX + own * a.d;
+    }
+    if constexpr (GRAD) {
+#pragma unroll
+      for (int b = 0; b < DB; ++b) {
+        const int c = 16 * b + 4 * g;
+        if (c < a.d)
+          *(float4*)(out + c) = !FWD && own == 0 ? make_float4(0.f, 0.f, 0.f, 0.f)   // padding row: no gradient
+                                                 : make_float4(O[b][cb][0] * down, O[b][cb][1] * down, O[b][cb][2] * down, O[b][cb][3] * down);
+      }
+    }
   }
 }
 
@@ -465,21 +615,57 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
   }
 }
 
-// loss_out = [T^2 / C sum of the rows' losses, C, update guard, -] (single block, fixed order)
-__global__ __launch_bounds__(256) void distill_loss_kernel(const float* __restrict__ stat, int B, float T2, float* __restrict__ loss_out) {
+// Workgroup 0: loss_out = [T^2 / C sum of the rows' losses, C, update guard, -] (fixed order).  The others (a forward pass that will be
+// followed by a backward): the image of one tile of 32 users that every workgroup of the backward streams -- one exponent, [hi | lo][32][D]
+// halves in the swizzled order, the row biases -log2(softmax sum) (-inf without a teacher and behind the last user).
+template <int D>
+__global__ __launch_bounds__(256) void distill_loss_kernel(const float* __restrict__ stat, int B, float T2, float* __restrict__ loss_out,
+                                                           const float* __restrict__ U, int d, _Float16* __restrict__ img,
+                                                           float* __restrict__ rb_img, int* __restrict__ ky_img) {
   __shared__ float red[4];
-  float s = 0.f, c = 0.f;
-  for (int b = threadIdx.x; b < B; b += 256) {
-    s += stat[b];
-    c += stat[B + b];
+  if (blockIdx.x == 0) {
+    float s = 0.f, c = 0.f;
+    for (int b = threadIdx.x; b < B; b += 256) {
+      s += stat[b];
+      c += stat[B + b];
+    }
+    s = ds_block_sum(s, red);
+    c = ds_block_sum(c, red);
+    if (threadIdx.x == 0) {
+      loss_out[0] = T2 * s / fmaxf(c, 1.f);
+      loss_out[1] = c;
+      loss_out[2] = s != s ? -1.f : 1.f;   // update guard (see ur_gather_dot_loss_fwd)
+      loss_out[3] = 0.f;
+    }
+    return;
   }
-  s = ds_block_sum(s, red);
-  c = ds_block_sum(c, red);
-  if (threadIdx.x == 0) {
-    loss_out[0] = T2 * s / fmaxf(c, 1.f);
-    loss_out[1] = c;
-    loss_out[2] = s != s ? -1.f : 1.f;   // update guard (see ur_gather_dot_loss_fwd)
-    loss_out[3] = 0.f;
+  constexpr int F4 = D / 4, PER = DS_TILE * F4 / 256;
+  const int tile = blockIdx.x - 1;
+  float4 v[PER];
+  float mx = 0.f;
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int i = threadIdx.x + 256 * p, b = tile * DS_TILE + i / F4, c = (i % F4) * 4;
+    v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (b < B && c < d) v[p] = *(const float4*)(U + (long long)b * d + c);
+    mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(v[p].x), finite_abs(v[p].y)), fmaxf(finite_abs(v[p].z), finite_abs(v[p].w))));
+  }
+  const int ky = group_exponent(ds_block_max(mx, red));
+  const float up = pow2i(ky);
+  _Float16* out = img + (long long)tile * 2 * DS_TILE * D;
+#pragma unroll
+  for (int p = 0; p < PER; ++p) {
+    const int i = threadIdx.x + 256 * p, at = ds_at<D>(i / F4, (i % F4) * 4);
+    half2_t h0, h1, l0, l1;
+    split_pair(v[p].x, v[p].y, up, h0, l0);
+    split_pair(v[p].z, v[p].w, up, h1, l1);
+    *(half4*)(out + at) = (half4){h0[0], h0[1], h1[0], h1[1]};
+    *(half4*)(out + DS_TILE * D + at) = (half4){l0[0], l0[1], l1[0], l1[1]};
+  }
+  if (threadIdx.x == 0) ky_img[tile] = ky;
+  if (threadIdx.x < DS_TILE) {
+    const int b = tile * DS_TILE + threadIdx.x;
+    rb_img[b] = b < B ? -stat[2 * (long long)B + b] : -INFINITY;
   }
 }
 
@@ -531,13 +717,13 @@ __global__ __launch_bounds__(256) void distill_apply_kernel(DistillApply a) {
 }
 
 static inline int ds_tpr(int d) { return d <= 64 ? 16 : d <= 128 ? 32 : 64; }
-static inline int ds_nw(int B, int d) { return B <= 32 ? 1 : B <= 64 ? 2 : B <= 128 || d > 128 ? 4 : 8; }
+static inline int ds_nw(int B, int d) { return B <= 32 ? 1 : B <= 64 ? 2 : B <= 128 || d <= 32 || d > 128 ? 4 : 8; }
+static inline int ds_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-// the catalogue is cut into splits (a multiple of the 8 XCDs) so that about two workgroups per CU are in flight
 static void ds_splits(int B, int d, long long N, int* owner_blocks, int* splits, long long* per) {
   const int nw = ds_nw(B, d);
   *owner_blocks = cdiv(B, 32 * nw);
-  const long long tiles = (N + ds_rows(nw) - 1) / ds_rows(nw);
+  const long long tiles = (N + DS_TILE - 1) / DS_TILE;
   const long long want = std::max<long long>(1, 2048 / nw / *owner_blocks);
   long long s = std::min(want, (tiles + 1) / 2);
   s = std::max<long long>(8, (s + 7) / 8 * 8);
@@ -548,6 +734,7 @@ static void ds_splits(int B, int d, long long N, int* owner_blocks, int* splits,
 struct DistillWs {
   float *part_m, *part_l, *part_o;                                   // forward
   int *uniq, *seg, *pos, *n_uniq; char* plan;                       // backward
+  _Float16* img; float* rb_img; int* ky_img;                        // from the forward to the backward
   int64_t bytes;
 };
 static DistillWs ds_carve(int B, int d, long long N, int K, int grad, char* base) {
@@ -561,12 +748,17 @@ static DistillWs ds_carve(int B, int d, long long N, int K, int grad, char* base
   int ob, splits;
   long long per;
   ds_splits(B, d, N, &ob, &splits, &per);
+  if (grad) {
+    const int64_t ut = cdiv(B, DS_TILE);
+    w.img = (_Float16*)take(ut * 4 * DS_TILE * ds_width(d)); w.rb_img = (float*)take(ut * DS_TILE * 4); w.ky_img = (int*)take(ut * 4);
+  }
+  const int64_t mark = o;
   w.part_m = (float*)take((int64_t)splits * B * 4);
   w.part_l = (float*)take((int64_t)splits * B * 4);
   if (grad) {
     w.part_o = (float*)take((int64_t)splits * B * d * 4);
     const int64_t n = (int64_t)B * K, fwd = o;
-    o = 0;                                                          // the backward reuses the forward's partials
+    o = mark;                                                       // the backward reuses the forward's partials
     w.uniq = (int*)take(n * 4); w.seg = (int*)take((n + 1) * 4); w.pos = (int*)take(n * 4); w.n_uniq = (int*)take(4);
     w.plan = take(ur_rows_plan_workspace_bytes(n));
     o = std::max(o, fwd);
@@ -585,7 +777,7 @@ static int ds_launch_stream(const DistillStream& a, bool clip, int grid, hipStre
 template <int D>
 static int ds_launch_fwd(const DistillStream& a, bool grad, bool clip, int nw, int grid, hipStream_t st) {
 #define GO(W) (grad ? ds_launch_stream<D, W, true, true>(a, clip, grid, st) : ds_launch_stream<D, W, true, false>(a, clip, grid, st))
-  if constexpr (D <= 128) {
+  if constexpr (D == 64 || D == 128) {
     if (nw == 8) return GO(8);
   }
   return nw == 1 ? GO(1) : nw == 2 ? GO(2) : GO(4);
@@ -626,7 +818,7 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   ProfScope ps(PC_LOSS, st, (grad ? 4.0 : 2.0) * B * (double)n_items * d);
   const DistillWs w = ds_carve(B, d, n_items, K, grad, (char*)ws);
   DistillStream a{};
-  a.X = user_emb; a.nx = B; a.Y = item_table; a.ny = n_items; a.d = d; a.y_bias = item_bias; a.B = B;
+  a.X = user_emb; a.nx = B; a.Y = item_table; a.ny = n_items; a.d = d; a.y_bias = item_bias;
   a.cz = DS_LOG2E / (tau * temperature); a.clip2 = score_clip > 0.f ? score_clip / temperature * DS_LOG2E : 0.f;
   ds_splits(B, d, n_items, &a.owner_blocks, &a.splits, &a.tiles_per_split);
   a.part_m = w.part_m; a.part_l = w.part_l; a.part_o = w.part_o;
@@ -650,7 +842,16 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   }
 #undef GO
   UR_LAUNCH_CHECK();
-  hipLaunchKernelGGL(distill_loss_kernel, dim3(1), dim3(256), 0, st, row_stat, B, temperature * temperature, loss_out);
+  const int tiles = grad ? cdiv(B, DS_TILE) : 0;
+#define GO(W) hipLaunchKernelGGL((distill_loss_kernel<W>), dim3(1 + tiles), dim3(256), 0, st, row_stat, B, temperature * temperature, loss_out, user_emb, d, \
+                                 w.img, w.rb_img, w.ky_img)
+  switch (ds_width(d)) {
+    case 32: GO(32); break;
+    case 64: GO(64); break;
+    case 128: GO(128); break;
+    default: GO(256); break;
+  }
+#undef GO
   UR_LAUNCH_CHECK();
   return UR_OK;
 }
@@ -670,7 +871,7 @@ extern "C" int ur_full_distill_bwd(const float* user_emb, const float* item_tabl
   if (rc) return rc;
   ProfScope ps(PC_LOSS, st, 4.0 * B * (double)n_items * d);
   DistillStream a{};
-  a.X = item_table; a.nx = n_items; a.Y = user_emb; a.ny = B; a.d = d; a.row_stat = row_stat; a.B = B; a.x_bias = item_bias;
+  a.X = item_table; a.nx = n_items; a.ny = B; a.d = d; a.img = w.img; a.rb_img = w.rb_img; a.ky_img = w.ky_img; a.x_bias = item_bias;
   a.cz = DS_LOG2E / (tau * temperature); a.clip2 = score_clip > 0.f ? score_clip / temperature * DS_LOG2E : 0.f;
   a.loss_out = loss_out; a.d_loss = d_loss; a.g_num = temperature / tau; a.dX = d_item_table; a.d_bias = d_item_bias;
   const bool clip = score_clip > 0.f;
