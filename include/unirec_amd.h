@@ -770,11 +770,13 @@ int ur_full_distill_bwd(const float* user_emb, const float* item_table, int64_t 
  * temperature = 0: the lowest index among the largest.  *_rows (nullable): per-row values [B] in the place of the scalar (a top_p <= 0 keeps
  * the first entry, a temperature that is not positive is 0, a min_p that is not below 1 is 1, a top_k <= 0 is off).
  * out_id[B,S] = ids[b * ld_ids + index] (ids nullable: the index itself), out_logp[B,S] = log of the drawn entry's probability among the kept;
- * a row without an entry: -1, -inf.  Weights are double, rounded once to multiples of 2^-62, and summed as integers: no result depends on an
- * order of additions.  n < 2^31. */
+ * a row without an entry: -1, -inf.  Weights are double, rounded down once to multiples of 2^-62 and summed as integers: no result depends on an
+ * order of additions.  n < 2^31.
+ * ws: ur_sample_scores_workspace_bytes (0: rows that fit into a workgroup's LDS need none, ws may be NULL). */
+int64_t ur_sample_scores_workspace_bytes(int32_t score_type, int64_t n, int32_t B);
 int ur_sample_scores(const void* scores, int32_t score_type, int64_t n, int64_t ld, int32_t B, const float* rand, int32_t S, double temperature,
                      int32_t top_k, double top_p, double min_p, const float* temperature_rows, const int32_t* top_k_rows,
-                     const float* top_p_rows, const float* min_p_rows, const int64_t* ids, int64_t ld_ids, int64_t* out_id, float* out_logp,
+                     const float* top_p_rows, const float* min_p_rows, const int64_t* ids, int64_t ld_ids, int64_t* out_id, float* out_logp, void* ws,
                      void* stream);
 
 /* ---------------------------------------------------------------------------------------------

@@ -77,13 +77,16 @@ def test_refusals():
         ops.sample_scores(x.double(), u)
     one = 1 << 20
 
-    def call(t=0, n=8, ld=8, B=2, S=1, T=1.0, k=0, p=1.0, m=0.0, scores=one, ids=None, ld_ids=8):
-        return _lib.lib.ur_sample_scores(scores, t, n, ld, B, one, S, T, k, p, m, None, None, None, None, ids, ld_ids, one, one, None)
+    def call(t=0, n=8, ld=8, B=2, S=1, T=1.0, k=0, p=1.0, m=0.0, scores=one, ids=None, ld_ids=8, ws=one):
+        return _lib.lib.ur_sample_scores(scores, t, n, ld, B, one, S, T, k, p, m, None, None, None, None, ids, ld_ids, one, one, ws, None)
 
     for bad in (dict(t=3), dict(n=0), dict(ld=7), dict(B=0), dict(S=0), dict(T=-1.0), dict(T=math.nan), dict(T=math.inf), dict(k=-1), dict(p=0.0),
-                dict(p=math.nan), dict(m=-0.1), dict(m=1.5), dict(m=math.nan), dict(scores=None), dict(ids=one, ld_ids=3)):
+                dict(p=math.nan), dict(m=-0.1), dict(m=1.5), dict(m=math.nan), dict(scores=None), dict(ids=one, ld_ids=3),
+                dict(n=1 << 20, ld=1 << 20, ws=None)):
         assert call(**bad) == -1, bad
         assert b"ur_sample_scores" in _lib.lib.ur_last_error()
+    assert _lib.lib.ur_sample_scores_workspace_bytes(0, 0, 4) < 0 and _lib.lib.ur_sample_scores_workspace_bytes(9, 100, 4) < 0
+    assert _lib.lib.ur_sample_scores_workspace_bytes(0, 1000, 4) == 0 < _lib.lib.ur_sample_scores_workspace_bytes(0, 1 << 20, 4)
 
 
 # ------------------------------------------------------------------------------------------------ GPU

@@ -180,7 +180,8 @@ SIGNATURES = {
     "ur_full_distill_bwd": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, C.c_int32, P, C.c_float, C.c_float, C.c_float, P, P, P, P, P, P, P, P, P, P,
                                       P]),
     "ur_sample_scores": (C.c_int, [P, C.c_int32, I64, I64, C.c_int32, P, C.c_int32, C.c_double, C.c_int32, C.c_double, C.c_double, P, P, P, P, P, I64,
-                                   P, P, P]),
+                                   P, P, P, P]),
+    "ur_sample_scores_workspace_bytes": (I64, [C.c_int32, I64, C.c_int32]),
     "ur_rows_scatter_add": (C.c_int, [P, P, I64, P, C.c_int32, P, P]),
     "ur_prof_enable": (C.c_int, [C.c_int]),
     "ur_prof_set_mask": (C.c_int, [C.c_uint32]),

@@ -405,7 +405,7 @@ NOT_OPS = {
     "ur_rows_reduce_update_owner": _SHARD,
     "ur_last_error": _QUERY, "ur_version": _QUERY, "ur_id_guard_state": _QUERY, "ur_id_guard_reset": _SWITCH, "ur_trace_ranges_pushed": _QUERY, "ur_sasrec_param_layout": _QUERY, "ur_gru_param_layout": _QUERY,
     "ur_gru_workspace_bytes": _QUERY, "ur_rows_plan_workspace_bytes": _QUERY, "ur_gemm_tn_workspace_floats": _QUERY,
-    "ur_full_topk_workspace_bytes": _QUERY, "ur_full_distill_workspace_bytes": _QUERY, "ur_full_softmax_workspace_bytes": _QUERY, "ur_convformer_param_layout": _QUERY,
+    "ur_full_topk_workspace_bytes": _QUERY, "ur_full_distill_workspace_bytes": _QUERY, "ur_sample_scores_workspace_bytes": _QUERY, "ur_full_softmax_workspace_bytes": _QUERY, "ur_convformer_param_layout": _QUERY,
     "ur_convformer_workspace_bytes": _QUERY, "ur_atthist_param_layout": _QUERY, "ur_atthist_workspace_bytes": _QUERY,
     "ur_host_sampler_create": _HOST, "ur_host_sampler_destroy": _HOST, "ur_host_sampler_getrandbits": _HOST, "ur_host_sampler_random": _HOST,
     "ur_host_sampler_randint": _HOST, "ur_host_sampler_set_alias": _HOST, "ur_host_build_rows": _HOST, "ur_alias_table_build": _HOST,
