@@ -32,18 +32,28 @@ struct SampleArgs {
   long long* out_id; float* out_logp;   // [B, S]
 };
 
-// ascending unsigned order == ascending float order; -0 counts as 0 (equal scores tie), NaN as -inf
-__device__ __forceinline__ unsigned sample_key(float x) {
+// ascending unsigned order == ascending float order; -0 counts as 0 (equal scores tie), NaN and -inf are 0: no entry.
+// Scores of 16 bits keep their own 16-bit image, in the upper half (the last 10-bit round of a selection falls away).
+__device__ __forceinline__ unsigned key_f32(float x) {
   if (!(x > -INFINITY)) return 0u;
   const unsigned u = __float_as_uint(x + 0.f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
-__device__ __forceinline__ float sample_value(unsigned key) { return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key); }
-__device__ __forceinline__ float sample_load(const void* p, int type, long long i) {
-  if (type == UR_F16) return (float)((const _Float16*)p)[i];
-  if (type == UR_BF16) return __uint_as_float((unsigned)((const unsigned short*)p)[i] << 16);
-  return ((const float*)p)[i];
+__device__ __forceinline__ unsigned key_16(unsigned u, int type) {
+  const unsigned mag = u & 0x7FFFu, top = type == UR_F16 ? 0x7C00u : 0x7F80u;   // infinity
+  if (mag > top || u == (0x8000u | top)) return 0u;
+  if (mag == 0u) u = 0u;
+  return ((u & 0x8000u) ? (~u & 0xFFFFu) : (u | 0x8000u)) << 16;
 }
+__device__ __forceinline__ float key_value(unsigned key, int type) {
+  if (type == UR_F32) return __uint_as_float((key & 0x80000000u) ? (key & 0x7FFFFFFFu) : ~key);
+  const unsigned k = key >> 16, u = (k & 0x8000u) ? (k & 0x7FFFu) : (~k & 0xFFFFu);
+  return type == UR_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)u) : __uint_as_float(u << 16);
+}
+__device__ __forceinline__ unsigned sample_key(const void* p, int type, long long i) {
+  return type == UR_F32 ? key_f32(((const float*)p)[i]) : key_16(((const unsigned short*)p)[i], type);
+}
+
 // exp(z) 2^62, rounded down, z <= 0.  r = z - n ln 2 in two pieces, |r| <= ln 2 / 2, the Taylor polynomial of degree 12 (remainder 2 10^-16)
 __device__ __forceinline__ u64 exp_fixed(double z) {
   if (!(z > -43.0)) return 0;                                    // below 2^-62
@@ -69,22 +79,23 @@ __device__ __forceinline__ u64 exp_fixed(double z) {
 }
 // a row's parameters
 struct SampleRow {
-  double inv_T, p, min_z; long long k; bool greedy, flat;
+  double inv_T, p, min_z; long long k; int type; bool greedy, flat;
   float m;
   __device__ __forceinline__ void load(const SampleArgs& a, int b) {
     const double T = a.T_rows ? (double)a.T_rows[b] : a.T;
     double min_p = a.minp_rows ? (double)a.minp_rows[b] : a.min_p;
     p = a.p_rows ? (double)a.p_rows[b] : a.top_p;
     k = a.k_rows ? a.k_rows[b] : a.top_k;
+    type = a.type;
     if (k <= 0) k = a.N;
     greedy = !(T > 1e-300);              // (1 / T stays finite)
     inv_T = greedy ? 1.0 : 1.0 / T;
     if (!(min_p < 1.0)) min_p = 1.0;     // (the largest stays)
     min_z = min_p > 0.0 ? log(min_p) : -INFINITY;
   }
-  __device__ __forceinline__ void set_max(unsigned key) { m = sample_value(key); flat = greedy || m == INFINITY; }
+  __device__ __forceinline__ void set_max(unsigned key) { m = key_value(key, type); flat = greedy || m == INFINITY; }
   __device__ __forceinline__ double z(unsigned key) const {
-    const float x = sample_value(key);
+    const float x = key_value(key, type);
     if (flat) return x == m ? 0.0 : -INFINITY;
     return ((double)x - (double)m) * inv_T;
   }
@@ -105,28 +116,54 @@ struct WSum {   // a sum of weights
   __device__ __forceinline__ void add(const WSum& o) { hi += o.hi; lo += o.lo; }
   __device__ __forceinline__ u128 all() const { return ((u128)hi << 32) + lo; }
 };
-__device__ __forceinline__ u64 shfl_xor64(u64 v, int o) {
-  return ((u64)(unsigned)__shfl_xor((int)(v >> 32), o, 64) << 32) | (unsigned)__shfl_xor((int)(unsigned)v, o, 64);
-}
-__device__ __forceinline__ u64 shfl_up64(u64 v, int o) {
-  return ((u64)(unsigned)__shfl_up((int)(v >> 32), o, 64) << 32) | (unsigned)__shfl_up((int)(unsigned)v, o, 64);
-}
-__device__ __forceinline__ WSum wave_total(WSum v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    v.hi += shfl_xor64(v.hi, o);
-    v.lo += shfl_xor64(v.lo, o);
-  }
+// inclusive sums over the lanes of a wave, in lane order: DPP moves (row_shr 1, 2, 4, 8, then lane 15 / 31 of the rows before), VALU rate
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned dpp_from(unsigned v) { return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false); }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_from(u64 v) { return ((u64)dpp_from<CTRL, ROWS>((unsigned)(v >> 32)) << 32) | dpp_from<CTRL, ROWS>((unsigned)v); }
+template <typename T>
+__device__ __forceinline__ T wave_upto(T v) {
+  v += dpp_from<0x111, 0xF>(v);
+  v += dpp_from<0x112, 0xF>(v);
+  v += dpp_from<0x114, 0xF>(v);
+  v += dpp_from<0x118, 0xF>(v);
+  v += dpp_from<0x142, 0xA>(v);
+  v += dpp_from<0x143, 0xC>(v);
   return v;
 }
-__device__ __forceinline__ WSum wave_upto(WSum v) {   // inclusive, lane order
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ unsigned last_lane(unsigned v) { return (unsigned)__builtin_amdgcn_readlane((int)v, 63); }
+__device__ __forceinline__ u64 last_lane(u64 v) { return ((u64)last_lane((unsigned)(v >> 32)) << 32) | last_lane((unsigned)v); }
+template <typename T>
+__device__ __forceinline__ T wave_total(T v) { return last_lane(wave_upto(v)); }
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 h = shfl_up64(v.hi, o), l = shfl_up64(v.lo, o);
-    if (lane >= o) { v.hi += h; v.lo += l; }
-  }
+  for (int o = 1; o < 64; o <<= 1) v = max(v, (unsigned)__shfl_xor((int)v, o, 64));
   return v;
+}
+// over the workgroup, in thread order: the sum in front of a thread, and the sum of all.  tmp[NT / 64]
+template <int NT, typename T>
+__device__ __forceinline__ T block_before(T v, T* tmp, T* total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const T s = wave_upto(v);
+  __syncthreads();
+  if (lane == 63) tmp[wave] = s;
+  __syncthreads();
+  T base = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < NT / 64; ++w) {
+    const T t = tmp[w];
+    if (w < wave) base += t;
+    all += t;
+  }
+  *total = all;
+  return base + s - v;
+}
+template <int NT>
+__device__ __forceinline__ WSum block_before(const WSum& v, u64* tmp, WSum* total) {
+  WSum r;
+  r.hi = block_before<NT>(v.hi, tmp, &total->hi);
+  r.lo = block_before<NT>(v.lo, tmp, &total->lo);
+  return r;
 }
 __device__ __forceinline__ double wide_to_double(u128 v) { return (double)(u64)(v >> 64) * 18446744073709551616.0 + (double)(u64)v; }
 __device__ __forceinline__ u128 double_to_wide(double v) {   // v >= 0
@@ -150,7 +187,7 @@ __device__ __forceinline__ unsigned ties_within(u64 above, u64 w, double limit, 
 }
 
 // ---- one round of a selection: 2 048 bins over the keys of one prefix
-constexpr int SB = 2048, ROUNDS = 3;
+constexpr int SB = 2048;
 __device__ __forceinline__ int round_shift(int round) { return round == 0 ? 21 : round == 1 ? 10 : 0; }
 __device__ __forceinline__ unsigned round_bin(unsigned key, int round) { return (key >> round_shift(round)) & (round == 2 ? 1023u : 2047u); }
 __device__ __forceinline__ bool round_in(unsigned key, int round, unsigned prefix) {
@@ -161,52 +198,23 @@ struct Select {   // state of a selection (one per row)
   u64 above; double limit;              // top-p: the weight in front of the prefix, p times all of it
   unsigned done;
 };
+// bins lie in the order of the threads that sum them: thread t of NT takes the SB / NT bins from the t SB / NT -th highest on, each at j NT + t
 template <int NT>
-__device__ __forceinline__ unsigned block_before(unsigned v, unsigned* tmp) {   // exclusive sum over the threads; tmp[NT / 64]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  unsigned s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const unsigned t = __shfl_up((int)s, o, 64);
-    if (lane >= o) s += t;
-  }
-  if (lane == 63) tmp[wave] = s;
-  __syncthreads();
-  unsigned base = 0;
-  for (int w = 0; w < wave; ++w) base += tmp[w];
-  __syncthreads();
-  return base + s - v;
+__device__ __forceinline__ int bin_at(unsigned d) {
+  constexpr int PB = SB / NT;
+  const unsigned p = SB - 1 - d;
+  return (int)((p % PB) * NT + p / PB);
 }
+// the bin that the border falls into, found by the whole workgroup (from the highest key down); updates st, sets cut when it is final.
+// `last`: no key of this type has bits below this round's
 template <int NT>
-__device__ __forceinline__ u64 block_before(u64 v, u64* tmp, u64* total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  u64 s = v;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 t = shfl_up64(s, o);
-    if (lane >= o) s += t;
-  }
-  if (lane == 63) tmp[wave] = s;
-  __syncthreads();
-  u64 base = 0, all = 0;
-  for (int w = 0; w < NT / 64; ++w) {
-    if (w < wave) base += tmp[w];
-    all += tmp[w];
-  }
-  __syncthreads();
-  *total = all;
-  return base + s - v;
-}
-// the bin that the border falls into, found by the whole workgroup (bins from the highest key down); updates st, sets cut when it is final.
-// cnt / wgt: the round's histogram (any address space), read through `count` and `weight`
-template <int NT, typename C>
-__device__ __forceinline__ void pick_k(int round, C count, Select* st, SampleCut* cut, unsigned* tmp) {
+__device__ __forceinline__ void pick_k(int round, bool last, const unsigned* hc, Select* st, SampleCut* cut, unsigned* tmp) {
   constexpr int PB = SB / NT;
   const unsigned need = st->need, prefix = st->prefix;
-  unsigned mine[PB], sum = 0;
+  unsigned mine[PB], sum = 0, total;
 #pragma unroll
-  for (int j = 0; j < PB; ++j) { mine[j] = count(SB - 1 - ((int)threadIdx.x * PB + j)); sum += mine[j]; }
-  unsigned before = block_before<NT>(sum, tmp);
+  for (int j = 0; j < PB; ++j) { mine[j] = hc[j * NT + threadIdx.x]; sum += mine[j]; }
+  unsigned before = block_before<NT>(sum, tmp, &total);
   if (before < need && need <= before + sum) {
 #pragma unroll
     for (int j = 0; j < PB; ++j) {
@@ -215,38 +223,37 @@ __device__ __forceinline__ void pick_k(int round, C count, Select* st, SampleCut
         st->prefix = p;
         st->need = rest;
         if (rest == mine[j]) { cut->cut = (p << round_shift(round)) - 1u; cut->ties = 0u; st->done = 1u; }   // all of the bin
-        else if (round == ROUNDS - 1) { cut->cut = p; cut->ties = rest; st->done = 1u; }
+        else if (last) { cut->cut = p << round_shift(round); cut->ties = rest; st->done = 1u; }
       }
       before += mine[j];
     }
-  } else if (threadIdx.x == NT - 1 && before + sum < need) {
+  } else if (threadIdx.x == 0 && total < need) {
     st->done = 1u;                      // fewer entries than k: nothing is cut
   }
   __syncthreads();
 }
-template <int NT, typename C, typename W>
-__device__ __forceinline__ void pick_p(int round, C count, W weight, double p, Select* st, SampleCut* cut, u64* tmp) {
+template <int NT>
+__device__ __forceinline__ void pick_p(int round, bool last, const unsigned* hc, const u64* hw, double p, Select* st, SampleCut* cut, u64* tmp) {
   constexpr int PB = SB / NT;
   const unsigned prefix = st->prefix;
+  const u64 above = st->above;
+  const double given = st->limit;
   u64 mine[PB], sum = 0, total;
 #pragma unroll
-  for (int j = 0; j < PB; ++j) { mine[j] = weight(SB - 1 - ((int)threadIdx.x * PB + j)); sum += mine[j]; }
-  u64 before = block_before<NT>(sum, tmp, &total) + st->above;
-  const double limit = round == 0 ? p * (double)total : st->limit;
-  __syncthreads();
-  // the first entry of exactly one bin is the last whose forerunners weigh less than the limit (p <= 0: the first bin)
-  const bool here = limit > 0.0 ? (double)before < limit && !((double)(before + sum) < limit) : false;
-  if (here) {
+  for (int j = 0; j < PB; ++j) { mine[j] = hw[j * NT + threadIdx.x]; sum += mine[j]; }
+  u64 before = block_before<NT>(sum, tmp, &total) + above;
+  const double limit = round == 0 ? p * (double)total : given;
+  // the first entry of exactly one bin is the last whose forerunners weigh less than the limit
+  if ((double)before < limit && !((double)(before + sum) < limit)) {
 #pragma unroll
     for (int j = 0; j < PB; ++j) {
       if ((double)before < limit && !((double)(before + mine[j]) < limit)) {
-        const unsigned d = SB - 1 - (threadIdx.x * PB + j), q = round == 0 ? d : (prefix << (round == 1 ? 11 : 10)) | d, n = count(d);
+        const unsigned d = SB - 1 - (threadIdx.x * PB + j), q = round == 0 ? d : (prefix << (round == 1 ? 11 : 10)) | d, n = hc[j * NT + threadIdx.x];
         st->prefix = q;
         st->above = before;
         st->limit = limit;
-        st->need = n;
         if (n == 1) { cut->cut = (q << round_shift(round)) - 1u; cut->ties = 0u; st->done = 1u; }
-        else if (round == ROUNDS - 1) { cut->cut = q; cut->ties = ties_within(before, mine[j] / n, limit, n); st->done = 1u; }
+        else if (last) { cut->cut = q << round_shift(round); cut->ties = ties_within(before, mine[j] / n, limit, n); st->done = 1u; }
       }
       before += mine[j];
     }
@@ -255,44 +262,66 @@ __device__ __forceinline__ void pick_p(int round, C count, W weight, double p, S
 }
 
 // ---------------------------------------------------------------------------------------------- rows that fit into LDS
-constexpr int SBLK = 512;               // entries of a block of the kept sums
+constexpr int SLIST = 2048, SPAIRS = 128;
+// Thread t owns the entries [t C, (t + 1) C): sums in index order are one scan over the threads.  When top-k leaves few entries they are
+// copied out, in order, and everything behind it works on the copy; of up to 128 entries the weight in front of each is summed directly.
 template <int NT, bool RAW>
 __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  constexpr int NWV = NT / 64;
-  const int nblk = (int)((a.N + SBLK - 1) / SBLK), N = (int)a.N;
-  u64* hw = (u64*)smem;                                          // [SB]
-  u64* bs = hw + SB;                                             // [2 nblk] block sums, then what lies in front of a block
-  unsigned* hc = (unsigned*)(bs + 2 * nblk);                     // [SB]
-  unsigned* tb = hc + SB;                                        // [nblk] ties in front of a block
-  unsigned* keys = tb + ((nblk + 3) & ~3);                       // [N], or 16-bit scores as they are
-  unsigned short* raw = (unsigned short*)keys;
+  constexpr int NWV = NT / 64, LAST = RAW ? 1 : 2;
+  u64* hw = (u64*)smem;                                          // [SB]; the copied entries on their way
+  unsigned* hc = (unsigned*)(hw + SB);                           // [SB]
+  unsigned* keys = hc + SB;                                      // [N] (RAW: 16 bits each); then the copied entries, keys and indices
+  unsigned short* keys16 = (unsigned short*)keys;
   __shared__ u64 tmp64[NWV];
-  __shared__ unsigned tmp32[NWV], s_max[NWV];
+  __shared__ unsigned tmp32[NWV];
   __shared__ Select st;
   __shared__ SampleCut cut_s;
-  __shared__ WSum s_total;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = blockIdx.x, tid = threadIdx.x, N = (int)a.N;
   const long long base = (long long)b * a.ld;
   SampleRow r;
   r.load(a, b);
+  int n = N;                            // entries in hand
+  bool copied = false;
   auto key_at = [&](int i) -> unsigned {
-    if constexpr (RAW) return sample_key(a.type == UR_F16 ? (float)__builtin_bit_cast(_Float16, raw[i]) : __uint_as_float((unsigned)raw[i] << 16));
-    else return keys[i];
+    if constexpr (RAW) {
+      if (!copied) return (unsigned)keys16[i] << 16;
+    }
+    return keys[i];
   };
   unsigned mk = 0u;
-  for (int i = tid; i < N; i += NT) {
-    const unsigned k = sample_key(sample_load(a.scores, a.type, base + i));
-    if constexpr (RAW) raw[i] = ((const unsigned short*)a.scores)[base + i];
-    else keys[i] = k;
-    mk = max(mk, k);
-  }
+  if constexpr (RAW) {
+    const unsigned short* x = (const unsigned short*)a.scores + base;
+    const int head = (int)min((long long)N, (long long)((8 - (((unsigned long long)x >> 1) & 7)) & 7));   // entries in front of a 16-byte boundary
+    auto put = [&](int i, unsigned u) {
+      const unsigned k = key_16(u, a.type);
+      keys16[i] = (unsigned short)(k >> 16);
+      mk = max(mk, k);
+    };
+    if (tid < head) put(tid, x[tid]);
+    const int wide = (N - head) / 8;
+#pragma unroll 4
+    for (int i = tid; i < wide; i += NT) {
+      const uint4 v = *(const uint4*)(x + head + 8 * i);
+      const unsigned u[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) mk = max(mk, (unsigned)__shfl_xor((int)mk, o, 64));
-  if (lane == 0) s_max[wave] = mk;
+      for (int j = 0; j < 4; ++j) { put(head + 8 * i + 2 * j, u[j] & 0xFFFFu); put(head + 8 * i + 2 * j + 1, u[j] >> 16); }
+    }
+    if (tid < N - head - 8 * wide) put(head + 8 * wide + tid, x[head + 8 * wide + tid]);
+  } else {
+    const float* x = (const float*)a.scores + base;
+#pragma unroll 8
+    for (int i = tid; i < N; i += NT) {
+      const unsigned k = key_f32(x[i]);
+      keys[i] = k;
+      mk = max(mk, k);
+    }
+  }
+  mk = wave_max(mk);
+  if ((tid & 63) == 0) tmp32[tid >> 6] = mk;
   __syncthreads();
-  mk = 0u;
-  for (int w = 0; w < NWV; ++w) mk = max(mk, s_max[w]);
+#pragma unroll
+  for (int w = 0; w < NWV; ++w) mk = max(mk, tmp32[w]);
   if (mk == 0u) {                       // nothing to choose from
     for (int s = tid; s < a.S; s += NT) {
       a.out_id[(long long)b * a.S + s] = -1;
@@ -302,134 +331,137 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
   }
   r.set_max(mk);
   SampleCut c{0u, ALL_TIES};            // (key 0: no entry)
+  auto ranked = [&]() { return c.ties != 0u && c.ties != ALL_TIES; };
+  auto span = [&]() { return ((n + NT - 1) / NT) | 1; };         // (odd: 64 threads a span apart are in 64 banks)
+  auto in_front = [&](int i0, int i1) -> unsigned {              // ties in front of this thread's entries
+    unsigned eq = 0, total;
+    for (int i = i0; i < i1; ++i) eq += key_at(i) == c.cut;
+    return block_before<NT>(eq, tmp32, &total);
+  };
+  auto stays = [&](unsigned k, unsigned& rank) -> bool {         // entries in order; rank = ties so far
+    if (k > c.cut) return true;
+    return k == c.cut && k != 0u && rank++ < c.ties;
+  };
   if (r.greedy) {
     c.cut = mk;
     c.ties = 1u;
   } else {
     if (r.k < N) {
       if (tid == 0) { st = Select{0u, (unsigned)r.k, 0, 0.0, 0u}; cut_s = c; }
-      for (int round = 0; round < ROUNDS; ++round) {
+      for (int round = 0; round <= LAST; ++round) {
         for (int i = tid; i < SB; i += NT) hc[i] = 0u;
         __syncthreads();
         const unsigned prefix = st.prefix;
+#pragma unroll 4
         for (int i = tid; i < N; i += NT) {
           const unsigned k = key_at(i);
-          if (k != 0u && round_in(k, round, prefix)) atomicAdd(&hc[round_bin(k, round)], 1u);
+          if (k != 0u && round_in(k, round, prefix)) atomicAdd(&hc[bin_at<NT>(round_bin(k, round))], 1u);
         }
         __syncthreads();
-        pick_k<NT>(round, [&](int d) { return hc[d]; }, &st, &cut_s, tmp32);
+        pick_k<NT>(round, round == LAST, hc, &st, &cut_s, tmp32);
         if (st.done) break;
       }
       c = cut_s;
       __syncthreads();
+      if (r.k <= SLIST && 4 * r.k <= N && c.cut != 0u) {         // exactly k entries are left: copy them out (through hw: they may overlap the row)
+        const int C = span(), i0 = min(N, tid * C), i1 = min(N, i0 + C);
+        unsigned rank = ranked() ? in_front(i0, i1) : 0u, count = 0, total;
+        const unsigned rank0 = rank;
+        for (int i = i0; i < i1; ++i) count += stays(key_at(i), rank);
+        unsigned at = block_before<NT>(count, tmp32, &total);
+        unsigned* list = (unsigned*)hw;                          // [2 SLIST]: key, index
+        rank = rank0;
+        if (count)
+          for (int i = i0; i < i1; ++i) {
+            const unsigned k = key_at(i);
+            if (stays(k, rank)) { list[2 * at] = k; list[2 * at + 1] = (unsigned)i; ++at; }
+          }
+        __syncthreads();
+        n = (int)total;
+        for (int i = tid; i < n; i += NT) { keys[i] = list[2 * i]; keys[n + i] = list[2 * i + 1]; }
+        copied = true;
+        c = SampleCut{0u, ALL_TIES};
+        __syncthreads();
+      }
     }
-    if (r.p < 1.0) {
+    if (r.p < 1.0 && r.p > 0.0 && copied && n <= SPAIRS) {
+      // the weight in front of every entry; those that go become key 0
+      u64 w = 0, front = 0, total;
+      unsigned mine = 0u;
+      if (tid < n) {
+        mine = key_at(tid);
+        w = r.weight(mine) >> coarse;
+        hw[tid] = w;
+      }
+      block_before<NT>(w, tmp64, &total);                        // (its barriers publish hw)
+      if (tid < n) {
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) {
+          const unsigned k = key_at(j);
+          const u64 wj = hw[j];
+          front += (k > mine || (k == mine && j < tid)) ? wj : 0;
+        }
+      }
+      __syncthreads();
+      if (tid < n && !((double)front < r.p * (double)total)) keys[tid] = 0u;
+      __syncthreads();
+    } else if (r.p < 1.0) {
       if (tid == 0) { st = Select{0u, 0u, 0, 0.0, 0u}; cut_s = SampleCut{mk, 1u}; }   // (p <= 0: the largest alone)
-      for (int round = 0; round < ROUNDS && r.p > 0.0; ++round) {
+      for (int round = 0; round <= LAST && r.p > 0.0; ++round) {
         for (int i = tid; i < SB; i += NT) { hc[i] = 0u; hw[i] = 0; }
         __syncthreads();
         const unsigned prefix = st.prefix;
-        for (int i = tid; i < N; i += NT) {
+        for (int i = tid; i < n; i += NT) {
           const unsigned k = key_at(i);
           if (k <= c.cut || !round_in(k, round, prefix)) continue;
           const u64 w = r.weight(k) >> coarse;
-          const unsigned d = round_bin(k, round);
+          const int d = bin_at<NT>(round_bin(k, round));
           atomicAdd(&hc[d], 1u);
           atomicAdd(&hw[d], w);
         }
         if (tid == 0 && c.cut != 0u && c.ties != 0u && round_in(c.cut, round, prefix)) {   // the ties that top-k left
-          atomicAdd(&hc[round_bin(c.cut, round)], c.ties);
-          atomicAdd(&hw[round_bin(c.cut, round)], (r.weight(c.cut) >> coarse) * c.ties);
+          const int d = bin_at<NT>(round_bin(c.cut, round));
+          atomicAdd(&hc[d], c.ties);
+          atomicAdd(&hw[d], (r.weight(c.cut) >> coarse) * c.ties);
         }
         __syncthreads();
-        pick_p<NT>(round, [&](int d) { return hc[d]; }, [&](int d) { return hw[d]; }, r.p, &st, &cut_s, tmp64);
+        pick_p<NT>(round, round == LAST, hc, hw, r.p, &st, &cut_s, tmp64);
         if (st.done) break;
       }
       __syncthreads();
       c = cut_s;
+      __syncthreads();
     }
   }
-  // ---- ties in front of every block (where some of them go)
-  const bool ranked = c.ties != 0u && c.ties != ALL_TIES;
-  if (ranked) {
-    for (int q = wave; q < nblk; q += NWV) {
-      int n = 0;
-      for (int i = q * SBLK + lane; i < min(N, (q + 1) * SBLK); i += 64) n += key_at(i) == c.cut;
-      for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o, 64);
-      if (lane == 0) tb[q] = (unsigned)n;
-    }
-    __syncthreads();
-    const unsigned v = tid < nblk ? tb[tid] : 0u;               // (nblk <= 128 < NT)
-    const unsigned before = block_before<NT>(v, tmp32);
-    if (tid < nblk) tb[tid] = before;
-    __syncthreads();
+  // ---- the kept weight in front of every thread's entries
+  const int C = span(), i0 = min(n, tid * C), i1 = min(n, i0 + C);
+  const unsigned rank0 = ranked() ? in_front(i0, i1) : 0u;
+  unsigned rank = rank0;
+  WSum mine{0, 0}, all;
+  for (int i = i0; i < i1; ++i) {
+    const unsigned k = key_at(i);
+    if (stays(k, rank)) mine.add(r.kept(k));
   }
-  // whether this lane's entry (one of 64 consecutive ones) stays; `ties` = ties in front of the 64
-  auto stays = [&](unsigned k, unsigned& ties) -> bool {
-    if (!ranked) return k > c.cut || (k == c.cut && k != 0u && c.ties != 0u);
-    const u64 eq = __ballot(k == c.cut);
-    const unsigned rank = ties + __popcll(eq & ((1ull << lane) - 1ull));
-    ties += __popcll(eq);
-    return k > c.cut || (k == c.cut && rank < c.ties);
-  };
-  // ---- the kept weight of every block
-  for (int q = wave; q < nblk; q += NWV) {
-    WSum v{0, 0};
-    unsigned ties = ranked ? tb[q] : 0u;
-#pragma unroll 2
-    for (int j = 0; j < SBLK / 64; ++j) {
-      const int i = q * SBLK + 64 * j + lane;
-      const unsigned k = i < N ? key_at(i) : 0u;
-      if (stays(k, ties)) v.add(r.kept(k));
-    }
-    v = wave_total(v);
-    if (lane == 0) { bs[2 * q] = v.hi; bs[2 * q + 1] = v.lo; }
-  }
-  __syncthreads();
-  if (wave == 0) {                      // prefix over the blocks, 64 at a time
-    WSum run{0, 0};
-    for (int q0 = 0; q0 < nblk; q0 += 64) {
-      const int q = q0 + lane;
-      const WSum v = q < nblk ? WSum{bs[2 * q], bs[2 * q + 1]} : WSum{0, 0};
-      const WSum up = wave_upto(v);
-      if (q < nblk) { bs[2 * q] = run.hi + up.hi - v.hi; bs[2 * q + 1] = run.lo + up.lo - v.lo; }
-      run.hi += ((u64)(unsigned)__shfl((int)(up.hi >> 32), 63, 64) << 32) | (unsigned)__shfl((int)(unsigned)up.hi, 63, 64);
-      run.lo += ((u64)(unsigned)__shfl((int)(up.lo >> 32), 63, 64) << 32) | (unsigned)__shfl((int)(unsigned)up.lo, 63, 64);
-    }
-    if (lane == 0) s_total = run;
-  }
-  __syncthreads();
-  const u128 W = s_total.all();
-  const double log_W = log(wide_to_double(W) * 2.168404344971009e-19);   // 2^-62
-  // ---- a wave a draw: the last block that does not begin behind the goal, its first entry behind it
-  for (int s = wave; s < a.S; s += NWV) {
+  const WSum front = block_before<NT>(mine, tmp64, &all);
+  const u128 W = all.all(), from = front.all(), to = from + mine.all();
+  double log_W = 0.0;
+  bool have = false;
+  for (int s = 0; s < a.S; ++s) {       // the thread that the goal falls to walks its entries
     const u128 goal = sample_goal(a.rand[(long long)b * a.S + s], W);
-    int q = 0;
-    for (int q0 = 0; q0 < nblk; q0 += 64) {
-      const int t = q0 + lane;
-      const bool before = t < nblk && WSum{bs[2 * t], bs[2 * t + 1]}.all() <= goal;
-      q += __popcll(__ballot(before));
-    }
-    q -= 1;
-    u128 run = WSum{bs[2 * q], bs[2 * q + 1]}.all();
-    unsigned ties = ranked ? tb[q] : 0u;
-    for (int j = 0; j < SBLK / 64; ++j) {
-      const int i = q * SBLK + 64 * j + lane;
-      const unsigned k = i < N ? key_at(i) : 0u;
-      WSum v{0, 0};
-      if (stays(k, ties)) v.add(r.kept(k));
-      const WSum up = wave_upto(v);
-      const u64 over = __ballot(run + up.all() > goal);
-      if (over) {
-        if (lane == __ffsll(over) - 1) {
-          a.out_id[(long long)b * a.S + s] = a.ids ? a.ids[(long long)b * a.ld_ids + i] : i;
-          a.out_logp[(long long)b * a.S + s] = r.greedy ? 0.f : (float)(r.z(k) - log_W);
-        }
+    if (!(from <= goal && goal < to)) continue;
+    if (!have) { log_W = log(wide_to_double(W) * 2.168404344971009e-19); have = true; }   // 2^-62
+    u128 run = from;
+    rank = rank0;
+    for (int i = i0; i < i1; ++i) {
+      const unsigned k = key_at(i);
+      if (!stays(k, rank)) continue;
+      run += r.kept(k);
+      if (run > goal) {
+        const long long at = copied ? (long long)keys[n + i] : i;
+        a.out_id[(long long)b * a.S + s] = a.ids ? a.ids[(long long)b * a.ld_ids + at] : at;
+        a.out_logp[(long long)b * a.S + s] = r.greedy ? 0.f : (float)(r.z(k) - log_W);
         break;
       }
-      const u64 th = ((u64)(unsigned)__shfl((int)(up.hi >> 32), 63, 64) << 32) | (unsigned)__shfl((int)(unsigned)up.hi, 63, 64);
-      const u64 tl = ((u64)(unsigned)__shfl((int)(up.lo >> 32), 63, 64) << 32) | (unsigned)__shfl((int)(unsigned)up.lo, 63, 64);
-      run += WSum{th, tl}.all();
     }
   }
 }
@@ -461,31 +493,39 @@ __global__ __launch_bounds__(256) void sample_init_kernel(SampleArgs a, SampleLo
 __device__ __forceinline__ unsigned agent_load(const unsigned* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 __device__ __forceinline__ u64 agent_load(const u64* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// four consecutive entries a thread and step (one wide load where the row's address allows it); entries behind the end are key 0.
-// f(key)
+// four consecutive entries (one wide load where `wide`: the address allows it); entries behind the end are key 0
+struct Four { unsigned k[4]; };
+__device__ __forceinline__ bool sample_wide(const SampleArgs& a, long long first) {
+  return (((unsigned long long)a.scores + (unsigned long long)first * (a.type == UR_F32 ? 4 : 2)) & (a.type == UR_F32 ? 15 : 7)) == 0;
+}
+__device__ __forceinline__ Four sample_four(const SampleArgs& a, long long base, long long i, long long end, bool wide) {
+  Four r;
+  if (wide && i + 4 <= end) {
+    if (a.type == UR_F32) {
+      const float4 v = *(const float4*)((const float*)a.scores + base + i);
+      r.k[0] = key_f32(v.x); r.k[1] = key_f32(v.y); r.k[2] = key_f32(v.z); r.k[3] = key_f32(v.w);
+    } else {
+      const ushort4 v = *(const ushort4*)((const unsigned short*)a.scores + base + i);
+      r.k[0] = key_16(v.x, a.type); r.k[1] = key_16(v.y, a.type); r.k[2] = key_16(v.z, a.type); r.k[3] = key_16(v.w, a.type);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) r.k[j] = i + j < end ? sample_key(a.scores, a.type, base + i + j) : 0u;
+  }
+  return r;
+}
+// a workgroup's entries, f(key); four wide loads of a thread are under way together
 template <typename F>
 __device__ __forceinline__ void sample_walk(const SampleArgs& a, long long base, long long i0, long long i1, F f) {
-  const bool half = a.type != UR_F32;
-  const bool wide = (((unsigned long long)a.scores + (unsigned long long)(base + i0) * (half ? 2 : 4)) & (half ? 7 : 15)) == 0;
-#pragma unroll 2
-  for (long long i = i0 + 4 * threadIdx.x; i < i1; i += 1024) {
-    float x[4];
-    if (wide && i + 4 <= i1) {
-      if (half) {
-        const ushort4 v = *(const ushort4*)((const unsigned short*)a.scores + base + i);
-        const unsigned short u[4] = {v.x, v.y, v.z, v.w};
+  const bool wide = sample_wide(a, base + i0);
+  for (long long i = i0 + 4 * threadIdx.x; i < i1; i += 4096) {
+    Four v[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = a.type == UR_F16 ? (float)__builtin_bit_cast(_Float16, u[j]) : __uint_as_float((unsigned)u[j] << 16);
-      } else {
-        const float4 v = *(const float4*)((const float*)a.scores + base + i);
-        x[0] = v.x; x[1] = v.y; x[2] = v.z; x[3] = v.w;
-      }
-    } else {
+    for (int u = 0; u < 4; ++u) v[u] = sample_four(a, base, i + 1024 * u, i1, wide);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = i + j < i1 ? sample_load(a.scores, a.type, base + i + j) : -INFINITY;
-    }
+    for (int u = 0; u < 4; ++u)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f(sample_key(x[j]));
+      for (int j = 0; j < 4; ++j) f(v[u].k[j]);
   }
 }
 __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a, SampleLong g) {
@@ -493,8 +533,7 @@ __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a, SampleLon
   const long long i0 = (long long)blockIdx.x * LCH, i1 = min(a.N, i0 + LCH);
   unsigned mk = 0u;
   sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) { mk = max(mk, k); });
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) mk = max(mk, (unsigned)__shfl_xor((int)mk, o, 64));
+  mk = wave_max(mk);
   if ((threadIdx.x & 63) == 0 && mk) atomicMax(&g.state[b].maxkey, mk);
 }
 // a round of the top-k (PHASE 0) or top-p (PHASE 1) selection: counts (and weights) of the prefix's entries by bin; the workgroup that
@@ -532,13 +571,14 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
   sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) {
     if (PHASE == 0 ? k == 0u : k <= kc.cut) return;
     if (!round_in(k, round, prefix)) return;
-    const unsigned d = round_bin(k, round);
+    const int d = bin_at<256>(round_bin(k, round));
     atomicAdd(&hc[d], 1u);
     if constexpr (PHASE == 1) atomicAdd(&hw[d], r.weight(k) >> g.coarse);
   });
   if (PHASE == 1 && blockIdx.x == 0 && tid == 0 && kc.cut != 0u && kc.ties != 0u && round_in(kc.cut, round, prefix)) {
-    atomicAdd(&hc[round_bin(kc.cut, round)], kc.ties);
-    atomicAdd(&hw[PHASE == 1 ? round_bin(kc.cut, round) : 0], (r.weight(kc.cut) >> g.coarse) * kc.ties);
+    const int d = bin_at<256>(round_bin(kc.cut, round));
+    atomicAdd(&hc[d], kc.ties);
+    atomicAdd(&hw[PHASE == 1 ? d : 0], (r.weight(kc.cut) >> g.coarse) * kc.ties);
   }
   __syncthreads();
   for (int i = tid; i < SB; i += 256)
@@ -561,8 +601,9 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
     if (PHASE == 1) ghw[i] = 0;
   }
   __syncthreads();
-  if constexpr (PHASE == 0) pick_k<256>(round, [&](int d) { return hc[d]; }, &st, &cut, tmp32);
-  else pick_p<256>(round, [&](int d) { return hc[d]; }, [&](int d) { return hw[d]; }, r.p, &st, &cut, tmp64);
+  const bool last_round = round == (a.type == UR_F32 ? 2 : 1);
+  if constexpr (PHASE == 0) pick_k<256>(round, last_round, hc, &st, &cut, tmp32);
+  else pick_p<256>(round, last_round, hc, hw, r.p, &st, &cut, tmp64);
   if (tid == 0) {
     S->st = st;
     S->cut = cut;
@@ -573,37 +614,35 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
 __device__ __forceinline__ SampleCut final_cut(const SampleState* S, const SampleRow& r) {
   return r.greedy ? SampleCut{S->maxkey, 1u} : S->cut;
 }
+__device__ __forceinline__ bool some_ties(const SampleCut& c) { return c.ties != 0u && c.ties != ALL_TIES; }
 // ties of every block (rows where some of them go)
 __global__ __launch_bounds__(256) void sample_ties_kernel(SampleArgs a, SampleLong g) {
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   SampleRow r;
   r.load(a, b);
   const SampleCut c = final_cut(g.state + b, r);
-  if (c.ties == 0u || c.ties == ALL_TIES) return;
+  if (!some_ties(c)) return;
+  const long long base = (long long)b * a.ld;
   for (int q = blockIdx.x * (LCH / LBLK) + wave; q < min(g.nblk, (int)(blockIdx.x + 1) * (LCH / LBLK)); q += 4) {
-    int n = 0;
-    for (long long i = (long long)q * LBLK + lane; i < min(a.N, (long long)(q + 1) * LBLK); i += 64)
-      n += sample_key(sample_load(a.scores, a.type, (long long)b * a.ld + i)) == c.cut;
-    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o, 64);
-    if (lane == 0) g.tb[(long long)b * g.nblk + q] = (unsigned)n;
+    const long long i0 = (long long)q * LBLK, i1 = min(a.N, i0 + LBLK);
+    const bool wide = sample_wide(a, base + i0);
+    unsigned n = 0;
+#pragma unroll 4
+    for (int j = 0; j < LBLK / 256; ++j) {
+      const Four v = sample_four(a, base, i0 + 256 * j + 4 * lane, i1, wide);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) n += v.k[u] == c.cut;
+    }
+    n = wave_total(n);
+    if (lane == 0) g.tb[(long long)b * g.nblk + q] = n;
   }
 }
-struct TieRank {   // whether this lane's entry (one of 64 consecutive ones) stays
-  SampleCut c; bool ranked; unsigned ties;
-  __device__ __forceinline__ bool stays(unsigned k) {
-    if (!ranked) return k > c.cut || (k == c.cut && k != 0u && c.ties != 0u);
-    const u64 eq = __ballot(k == c.cut);
-    const unsigned rank = ties + __popcll(eq & ((1ull << (threadIdx.x & 63)) - 1ull));
-    ties += __popcll(eq);
-    return k > c.cut || (k == c.cut && rank < c.ties);
-  }
-};
 __device__ __forceinline__ unsigned ties_before(const unsigned* tb, int q) {   // a wave sums what lies in front of block q
   unsigned n = 0;
   for (int t = threadIdx.x & 63; t < q; t += 64) n += tb[t];
-  for (int o = 1; o < 64; o <<= 1) n += (unsigned)__shfl_xor((int)n, o, 64);
-  return n;
+  return wave_total(n);
 }
+// the kept weight of every block: a wave a block of 2 048, four consecutive entries a lane
 __global__ __launch_bounds__(256) void sample_sums_kernel(SampleArgs a, SampleLong g) {
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   SampleRow r;
@@ -611,18 +650,35 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(SampleArgs a, SampleLo
   const SampleState* S = g.state + b;
   if (S->maxkey == 0u) return;
   r.set_max(S->maxkey);
-  TieRank t{final_cut(S, r), false, 0u};
-  t.ranked = t.c.ties != 0u && t.c.ties != ALL_TIES;
+  const SampleCut c = final_cut(S, r);
+  const bool ranked = some_ties(c);
+  const long long base = (long long)b * a.ld;
   for (int q = blockIdx.x * (LCH / LBLK) + wave; q < min(g.nblk, (int)(blockIdx.x + 1) * (LCH / LBLK)); q += 4) {
-    if (t.ranked) t.ties = ties_before(g.tb + (long long)b * g.nblk, q);
+    const long long i0 = (long long)q * LBLK, i1 = min(a.N, i0 + LBLK);
+    const bool wide = sample_wide(a, base + i0);
+    unsigned ties = ranked ? ties_before(g.tb + (long long)b * g.nblk, q) : 0u;
     WSum v{0, 0};
-#pragma unroll 4
-    for (int j = 0; j < LBLK / 64; ++j) {
-      const long long i = (long long)q * LBLK + 64 * j + lane;
-      const unsigned k = i < a.N ? sample_key(sample_load(a.scores, a.type, (long long)b * a.ld + i)) : 0u;
-      if (t.stays(k)) v.add(r.kept(k));
+#pragma unroll 2
+    for (int j = 0; j < LBLK / 256; ++j) {
+      const Four f = sample_four(a, base, i0 + 256 * j + 4 * lane, i1, wide);
+      unsigned rank = 0;
+      if (ranked) {
+        unsigned eq = 0;
+#pragma unroll
+        for (int u = 0; u < 4; ++u) eq += f.k[u] == c.cut;
+        const unsigned upto = wave_upto(eq);
+        rank = ties + upto - eq;
+        ties += last_lane(upto);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const unsigned k = f.k[u];
+        const bool stays = k > c.cut || (k == c.cut && k != 0u && rank++ < c.ties);
+        if (stays) v.add(r.kept(k));
+      }
     }
-    v = wave_total(v);
+    v.hi = wave_total(v.hi);
+    v.lo = wave_total(v.lo);
     if (lane == 0) {
       u64* o = g.bs + ((long long)b * g.nblk + q) * 2;
       o[0] = v.hi;
@@ -630,66 +686,80 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(SampleArgs a, SampleLo
     }
   }
 }
-// a workgroup of one wave a draw
-__global__ __launch_bounds__(64) void sample_draw_kernel(SampleArgs a, SampleLong g) {
-  const int s = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
-  const long long at = (long long)b * a.S + s;
+// a workgroup a draw: the block that the goal falls into (a thread takes a run of blocks), then its entry (a thread takes eight)
+__global__ __launch_bounds__(256) void sample_draw_kernel(SampleArgs a, SampleLong g) {
+  __shared__ u64 tmp64[4];
+  __shared__ unsigned tmp32[4];
+  __shared__ int q_s;
+  __shared__ WSum run_s;
+  const int s = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const long long at = (long long)b * a.S + s, base = (long long)b * a.ld;
   SampleRow r;
   r.load(a, b);
   const SampleState* S = g.state + b;
   if (S->maxkey == 0u) {
-    if (lane == 0) { a.out_id[at] = -1; a.out_logp[at] = -INFINITY; }
+    if (tid == 0) { a.out_id[at] = -1; a.out_logp[at] = -INFINITY; }
     return;
   }
   r.set_max(S->maxkey);
-  TieRank t{final_cut(S, r), false, 0u};
-  t.ranked = t.c.ties != 0u && t.c.ties != ALL_TIES;
+  if (tid == 0) { q_s = 0; run_s = WSum{0, 0}; }
+  const SampleCut c = final_cut(S, r);
   const u64* bs = g.bs + (long long)b * g.nblk * 2;
-  WSum sum{0, 0};
-  for (int q = lane; q < g.nblk; q += 64) sum.add(WSum{bs[2 * q], bs[2 * q + 1]});
-  const u128 W = wave_total(sum).all();
-  const double log_W = log(wide_to_double(W) * 2.168404344971009e-19);   // 2^-62
-  const u128 goal = sample_goal(a.rand[at], W);
-  WSum run{0, 0};                       // in front of the 64 blocks, then of the block, then of the 64 entries
-  int q = 0;
-  for (;; q += 64) {
-    const WSum v = q + lane < g.nblk ? WSum{bs[2 * (q + lane)], bs[2 * (q + lane) + 1]} : WSum{0, 0};
-    const WSum up = wave_upto(v);
-    WSum end = run;
-    end.add(up);
-    const u64 over = __ballot(end.all() > goal);
-    const int from = over ? __ffsll(over) - 1 : 63;
-    const WSum at_end{((u64)(unsigned)__shfl((int)(up.hi >> 32), from, 64) << 32) | (unsigned)__shfl((int)(unsigned)up.hi, from, 64),
-                      ((u64)(unsigned)__shfl((int)(up.lo >> 32), from, 64) << 32) | (unsigned)__shfl((int)(unsigned)up.lo, from, 64)};
-    const WSum last{((u64)(unsigned)__shfl((int)(v.hi >> 32), from, 64) << 32) | (unsigned)__shfl((int)(unsigned)v.hi, from, 64),
-                    ((u64)(unsigned)__shfl((int)(v.lo >> 32), from, 64) << 32) | (unsigned)__shfl((int)(unsigned)v.lo, from, 64)};
-    if (over || q + 64 >= g.nblk) {     // (goal < W: some block passes it)
-      run.hi += at_end.hi - last.hi;
-      run.lo += at_end.lo - last.lo;
-      q = min(q + from, g.nblk - 1);
-      break;
+  const int per = (g.nblk + 255) / 256, q0 = min(g.nblk, tid * per), q1 = min(g.nblk, q0 + per);
+  WSum mine{0, 0}, all;
+  for (int q = q0; q < q1; ++q) mine.add(WSum{bs[2 * q], bs[2 * q + 1]});
+  WSum run = block_before<256>(mine, tmp64, &all);
+  const u128 W = all.all(), goal = sample_goal(a.rand[at], W);
+  WSum end = run;
+  end.add(mine);
+  if (run.all() <= goal && goal < end.all()) {   // one thread (goal < W)
+    for (int q = q0; q < q1; ++q) {
+      end = run;
+      end.add(WSum{bs[2 * q], bs[2 * q + 1]});
+      if (goal < end.all()) { q_s = q; run_s = run; break; }
+      run = end;
     }
-    run.add(at_end);
   }
-  if (t.ranked) t.ties = ties_before(g.tb + (long long)b * g.nblk, q);
-  for (int j = 0; j < LBLK / 64; ++j) {
-    const long long i = (long long)q * LBLK + 64 * j + lane;
-    const unsigned k = i < a.N ? sample_key(sample_load(a.scores, a.type, (long long)b * a.ld + i)) : 0u;
-    WSum v{0, 0};
-    if (t.stays(k)) v.add(r.kept(k));
-    const WSum up = wave_upto(v);
-    WSum end = run;
-    end.add(up);
-    const u64 over = __ballot(end.all() > goal);
-    if (over) {
-      if (lane == __ffsll(over) - 1) {
-        a.out_id[at] = a.ids ? a.ids[(long long)b * a.ld_ids + i] : i;
-        a.out_logp[at] = r.greedy ? 0.f : (float)(r.z(k) - log_W);
+  __syncthreads();
+  const int q = q_s;
+  run = run_s;
+  const long long i0 = (long long)q * LBLK + 8 * tid, i1 = min(a.N, (long long)(q + 1) * LBLK);
+  unsigned k[8];
+  {
+    const bool wide = sample_wide(a, base + i0);
+    const Four f = sample_four(a, base, i0, i1, wide), h = sample_four(a, base, i0 + 4, i1, wide);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { k[u] = f.k[u]; k[4 + u] = h.k[u]; }
+  }
+  unsigned rank = 0;
+  if (some_ties(c)) {
+    unsigned eq = 0, total;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) eq += k[u] == c.cut;
+    rank = block_before<256>(eq, tmp32, &total) + ties_before(g.tb + (long long)b * g.nblk, q);
+  }
+  u64 w[8];
+  mine = WSum{0, 0};
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    const bool stays = k[u] > c.cut || (k[u] == c.cut && k[u] != 0u && rank++ < c.ties);
+    w[u] = stays ? r.kept(k[u]) : 0;
+    mine.add(w[u]);
+  }
+  run.add(block_before<256>(mine, tmp64, &all));
+  u128 sum = run.all();
+  if (sum <= goal && goal < sum + mine.all()) {
+    const double log_W = log(wide_to_double(W) * 2.168404344971009e-19);   // 2^-62
+    bool found = false;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      sum += w[u];
+      if (!found && sum > goal) {
+        found = true;
+        a.out_id[at] = a.ids ? a.ids[(long long)b * a.ld_ids + i0 + u] : i0 + u;
+        a.out_logp[at] = r.greedy ? 0.f : (float)(r.z(k[u]) - log_W);
       }
-      return;
     }
-    run.hi += ((u64)(unsigned)__shfl((int)(up.hi >> 32), 63, 64) << 32) | (unsigned)__shfl((int)(unsigned)up.hi, 63, 64);
-    run.lo += ((u64)(unsigned)__shfl((int)(up.lo >> 32), 63, 64) << 32) | (unsigned)__shfl((int)(unsigned)up.lo, 63, 64);
   }
 }
 
@@ -717,8 +787,7 @@ static size_t sample_long_bytes(long long N, int B, char* base, SampleLong* g) {
 }
 template <int NT, bool RAW>
 static int launch_sample_row(const SampleArgs& a, hipStream_t st) {
-  const int nblk = cdiv(a.N, SBLK);
-  const size_t lds = (size_t)SB * 12 + nblk * 16 + ((nblk + 3) & ~3) * 4 + (size_t)a.N * (RAW ? 2 : 4) + 16;
+  const size_t lds = (size_t)SB * 12 + (size_t)a.N * (RAW ? 2 : 4) + 16;
   static const hipError_t attr = hipFuncSetAttribute((const void*)sample_row_kernel<NT, RAW>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512);
   (void)attr;
   hipLaunchKernelGGL((sample_row_kernel<NT, RAW>), dim3(a.B), dim3(NT), lds, st, a, log2_up(a.N));
@@ -757,8 +826,9 @@ extern "C" int ur_sample_scores(const void* scores, int32_t score_type, int64_t 
   a.ids = (const long long*)ids; a.ld_ids = ld_ids; a.out_id = (long long*)out_id; a.out_logp = out_logp;
   if (lds) {
     // (threads: about 8 entries each for short rows, whose passes are latency; 1 024 where the row is most of a CU's LDS anyway)
-    if (n > 32768) return launch_sample_row<1024, true>(a, st);
-    return n <= 2048 ? launch_sample_row<256, false>(a, st) : n <= 8192 ? launch_sample_row<512, false>(a, st) : launch_sample_row<1024, false>(a, st);
+    if (score_type == UR_F32)
+      return n <= 2048 ? launch_sample_row<256, false>(a, st) : n <= 8192 ? launch_sample_row<512, false>(a, st) : launch_sample_row<1024, false>(a, st);
+    return n <= 2048 ? launch_sample_row<256, true>(a, st) : n <= 8192 ? launch_sample_row<512, true>(a, st) : launch_sample_row<1024, true>(a, st);
   }
   SampleLong g;
   sample_long_bytes(n, B, (char*)ws, &g);
@@ -770,11 +840,12 @@ extern "C" int ur_sample_scores(const void* scores, int32_t score_type, int64_t 
   UR_LAUNCH_CHECK();
   hipLaunchKernelGGL(sample_max_kernel, grid, dim3(256), 0, st, a, g);
   UR_LAUNCH_CHECK();
-  for (int round = 0; round < ROUNDS && g.uses_k; ++round) {
+  const int rounds = score_type == UR_F32 ? 3 : 2;
+  for (int round = 0; round < rounds && g.uses_k; ++round) {
     hipLaunchKernelGGL((sample_round_kernel<0>), grid, dim3(256), 0, st, a, g, round, mode);
     UR_LAUNCH_CHECK();
   }
-  for (int round = 0; round < ROUNDS && g.uses_p; ++round) {
+  for (int round = 0; round < rounds && g.uses_p; ++round) {
     hipLaunchKernelGGL((sample_round_kernel<1>), grid, dim3(256), 0, st, a, g, round, mode);
     UR_LAUNCH_CHECK();
   }
@@ -784,7 +855,7 @@ extern "C" int ur_sample_scores(const void* scores, int32_t score_type, int64_t 
   }
   hipLaunchKernelGGL(sample_sums_kernel, grid, dim3(256), 0, st, a, g);
   UR_LAUNCH_CHECK();
-  hipLaunchKernelGGL(sample_draw_kernel, dim3(S, B), dim3(64), 0, st, a, g);
+  hipLaunchKernelGGL(sample_draw_kernel, dim3(S, B), dim3(256), 0, st, a, g);
   UR_LAUNCH_CHECK();
   return UR_OK;
 }
