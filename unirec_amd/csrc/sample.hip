@@ -3,7 +3,10 @@
 //   z_n = (x_n - max x) / T, weight w_n = exp(z_n); NaN and -inf carry none; a row with +inf: those entries 1, the others 0
 //   top-k: the first k in the order (score descending, index ascending); top-p: of those, in that order, every entry before which less
 //   than p of their weight lies; min-p: w >= min_p.  The answer to u: the first index n, in INDEX order, with sum_{j <= n} kept w_j > u W.
-// No sort: the order only decides a threshold (a key and how many of its ties stay), found by radix selection over 11, 11 and 10 bits.
+// No sort: the order only decides a threshold (a key and how many of its ties stay).  It is found by a histogram over 2 048 equal steps of
+// the score (steps of the key's upper bits put most scores into a few dozen bins, whose LDS atomics then queue: 190 us against 75 us for
+// 64 rows of a million), and inside the step that the border falls into by comparing up to 128 keys directly, or by radix selection over
+// 11, 11 and 10 bits of the key.
 //
 // Arithmetic.  Which entry a sum's border falls on is a whole number, so sums are exact: a weight is exp in double (2 10^-16), rounded down
 // once to a multiple of 2^-62 and added as integers, in two 32-bit limbs summed in 64 bits each (the top-p selection sums multiples of
@@ -15,6 +18,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -186,26 +190,46 @@ __device__ __forceinline__ unsigned ties_within(u64 above, u64 w, double limit, 
   return lo;
 }
 
-// ---- one round of a selection: 2 048 bins over the keys of one prefix
+// ---- a selection: a histogram over equal steps of the score (round -1), then rounds over the bits of the keys of one step
 constexpr int SB = 2048;
+struct Steps {   // step of a score: (max - x) c, monotone in x; double: no difference of two floats overflows
+  double c; float m; int type; bool flat;
+  __device__ __forceinline__ void set(const SampleRow& r, unsigned minkey, bool weights) {
+    m = r.m; type = r.type; flat = r.flat;
+    double range = (double)r.m - (double)key_value(minkey, r.type);
+    if (weights) range = fmin(range, 43.0 / r.inv_T);            // (steps behind that weigh nothing: one bin)
+    c = range > 0.0 ? (double)SB / range : 0.0;
+  }
+  __device__ __forceinline__ int of(unsigned key) const {
+    const float x = key_value(key, type);
+    if (flat) return x == m ? 0 : SB - 1;
+    return (int)fmin(((double)m - (double)x) * c, (double)(SB - 1));
+  }
+};
 __device__ __forceinline__ int round_shift(int round) { return round == 0 ? 21 : round == 1 ? 10 : 0; }
-__device__ __forceinline__ unsigned round_bin(unsigned key, int round) { return (key >> round_shift(round)) & (round == 2 ? 1023u : 2047u); }
+__device__ __forceinline__ int round_place(unsigned key, int round) {   // from the highest key down
+  return SB - 1 - (int)((key >> round_shift(round)) & (round == 2 ? 1023u : 2047u));
+}
+__device__ __forceinline__ unsigned round_prefix(unsigned prefix, int round, int place) {
+  const unsigned d = (unsigned)(SB - 1 - place);
+  return round == 0 ? d : (prefix << (round == 1 ? 11 : 10)) | d;
+}
 __device__ __forceinline__ bool round_in(unsigned key, int round, unsigned prefix) {
   return round == 0 || (round == 1 ? key >> 21 : key >> 10) == prefix;
 }
 struct Select {   // state of a selection (one per row)
-  unsigned prefix; unsigned need;       // top-k: how many of the prefix's entries stay
-  u64 above; double limit;              // top-p: the weight in front of the prefix, p times all of it
+  int step; unsigned prefix; unsigned count;   // the step, the key's bits so far, and the entries that share them
+  unsigned need;                        // top-k: how many of those stay
+  u64 above; double limit;              // top-p: the weight in front of them, p times all of it
   unsigned done;
 };
-// bins lie in the order of the threads that sum them: thread t of NT takes the SB / NT bins from the t SB / NT -th highest on, each at j NT + t
+// bins lie in the order of the threads that sum them: thread t of NT takes places t SB / NT .. , each at j NT + t
 template <int NT>
-__device__ __forceinline__ int bin_at(unsigned d) {
+__device__ __forceinline__ int bin_at(int place) {
   constexpr int PB = SB / NT;
-  const unsigned p = SB - 1 - d;
-  return (int)((p % PB) * NT + p / PB);
+  return (place % PB) * NT + place / PB;
 }
-// the bin that the border falls into, found by the whole workgroup (from the highest key down); updates st, sets cut when it is final.
+// the place that the border falls into, found by the whole workgroup; updates st, sets cut when it is final.
 // `last`: no key of this type has bits below this round's
 template <int NT>
 __device__ __forceinline__ void pick_k(int round, bool last, const unsigned* hc, Select* st, SampleCut* cut, unsigned* tmp) {
@@ -219,11 +243,21 @@ __device__ __forceinline__ void pick_k(int round, bool last, const unsigned* hc,
 #pragma unroll
     for (int j = 0; j < PB; ++j) {
       if (before < need && need <= before + mine[j]) {
-        const unsigned d = SB - 1 - (threadIdx.x * PB + j), p = round == 0 ? d : (prefix << (round == 1 ? 11 : 10)) | d, rest = need - before;
-        st->prefix = p;
+        const int place = (int)threadIdx.x * PB + j;
+        const unsigned rest = need - before;
         st->need = rest;
-        if (rest == mine[j]) { cut->cut = (p << round_shift(round)) - 1u; cut->ties = 0u; st->done = 1u; }   // all of the bin
-        else if (last) { cut->cut = p << round_shift(round); cut->ties = rest; st->done = 1u; }
+        st->count = mine[j];
+        if (round < 0) st->step = place;
+        else {
+          const unsigned q = round_prefix(prefix, round, place);
+          st->prefix = q;
+          if (last) {                   // one key: all of its entries, or the first of them
+            const unsigned key = q << round_shift(round);
+            cut->cut = rest == mine[j] ? key - 1u : key;
+            cut->ties = rest == mine[j] ? 0u : rest;
+            st->done = 1u;
+          }
+        }
       }
       before += mine[j];
     }
@@ -242,29 +276,83 @@ __device__ __forceinline__ void pick_p(int round, bool last, const unsigned* hc,
 #pragma unroll
   for (int j = 0; j < PB; ++j) { mine[j] = hw[j * NT + threadIdx.x]; sum += mine[j]; }
   u64 before = block_before<NT>(sum, tmp, &total) + above;
-  const double limit = round == 0 ? p * (double)total : given;
+  const double limit = round < 0 ? p * (double)total : given;
   // the first entry of exactly one bin is the last whose forerunners weigh less than the limit
   if ((double)before < limit && !((double)(before + sum) < limit)) {
 #pragma unroll
     for (int j = 0; j < PB; ++j) {
       if ((double)before < limit && !((double)(before + mine[j]) < limit)) {
-        const unsigned d = SB - 1 - (threadIdx.x * PB + j), q = round == 0 ? d : (prefix << (round == 1 ? 11 : 10)) | d, n = hc[j * NT + threadIdx.x];
-        st->prefix = q;
+        const int place = (int)threadIdx.x * PB + j;
+        const unsigned n = hc[j * NT + threadIdx.x];
         st->above = before;
         st->limit = limit;
-        if (n == 1) { cut->cut = (q << round_shift(round)) - 1u; cut->ties = 0u; st->done = 1u; }
-        else if (last) { cut->cut = q << round_shift(round); cut->ties = ties_within(before, mine[j] / n, limit, n); st->done = 1u; }
+        st->count = n;
+        if (round < 0) st->step = place;
+        else {
+          const unsigned q = round_prefix(prefix, round, place);
+          st->prefix = q;
+          if (last) {
+            const unsigned key = q << round_shift(round), t = ties_within(before, mine[j] / n, limit, n);
+            cut->cut = t == n ? key - 1u : key;
+            cut->ties = t == n ? 0u : t;
+            st->done = 1u;
+          }
+        }
       }
       before += mine[j];
     }
   }
   __syncthreads();
 }
+// the border among `n` <= DIRECT keys of one step, compared with each other (lists padded with key 0 to a multiple of 8)
+constexpr int DIRECT = 128;
+__device__ __forceinline__ void direct_k(const unsigned* keys, int n, const Select* st, SampleCut* cut) {
+  if ((int)threadIdx.x < n) {
+    const unsigned mine = keys[threadIdx.x], need = st->need;
+    unsigned above = 0, equal = 0;
+    for (int j = 0; j < n; j += 8) {
+      const uint4 u = *(const uint4*)(keys + j), v = *(const uint4*)(keys + j + 4);
+      const unsigned k[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int q = 0; q < 8; ++q) { above += k[q] > mine; equal += k[q] == mine; }
+    }
+    if (above < need && need <= above + equal) {                 // (threads of equal keys write the same)
+      const bool all = need == above + equal;
+      cut->cut = all ? mine - 1u : mine;
+      cut->ties = all ? 0u : need - above;
+    }
+  }
+  __syncthreads();
+}
+__device__ __forceinline__ void direct_p(const unsigned* keys, const u64* wgt, int n, const Select* st, SampleCut* cut) {
+  if ((int)threadIdx.x < n) {
+    const unsigned mine = keys[threadIdx.x];
+    const u64 w = wgt[threadIdx.x];
+    u64 front = st->above;
+    unsigned equal = 0;
+    for (int j = 0; j < n; j += 8) {
+      const uint4 u = *(const uint4*)(keys + j), v = *(const uint4*)(keys + j + 4);
+      const unsigned k[8] = {u.x, u.y, u.z, u.w, v.x, v.y, v.z, v.w};
+      u64 x[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[q] = wgt[j + q];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) { front += k[q] > mine ? x[q] : 0; equal += k[q] == mine; }
+    }
+    const double limit = st->limit;
+    if ((double)front < limit && !((double)(front + w * equal) < limit)) {
+      const unsigned t = ties_within(front, w, limit, equal);
+      cut->cut = t == equal ? mine - 1u : mine;
+      cut->ties = t == equal ? 0u : t;
+    }
+  }
+  __syncthreads();
+}
 
 // ---------------------------------------------------------------------------------------------- rows that fit into LDS
-constexpr int SLIST = 2048, SPAIRS = 128;
+constexpr int SLIST = 2048;
 // Thread t owns the entries [t C, (t + 1) C): sums in index order are one scan over the threads.  When top-k leaves few entries they are
-// copied out, in order, and everything behind it works on the copy; of up to 128 entries the weight in front of each is summed directly.
+// copied out, in order, and everything behind it works on the copy.  A draw falls to one thread's entries; a wave looks at them together.
 template <int NT, bool RAW>
 __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -274,10 +362,15 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
   unsigned* keys = hc + SB;                                      // [N] (RAW: 16 bits each); then the copied entries, keys and indices
   unsigned short* keys16 = (unsigned short*)keys;
   __shared__ u64 tmp64[NWV];
-  __shared__ unsigned tmp32[NWV];
+  __shared__ unsigned tmp32[NWV], s_min[NWV], s_n;
   __shared__ Select st;
   __shared__ SampleCut cut_s;
-  const int b = blockIdx.x, tid = threadIdx.x, N = (int)a.N;
+  __shared__ __attribute__((aligned(16))) unsigned near_k[DIRECT];
+  __shared__ u64 near_w[DIRECT];
+  __shared__ u64 goal_hi[64], goal_lo[64], from_hi[64], from_lo[64];
+  __shared__ int owner[64];
+  __shared__ unsigned owner_rank[64];
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, N = (int)a.N;
   const long long base = (long long)b * a.ld;
   SampleRow r;
   r.load(a, b);
@@ -289,14 +382,18 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
     }
     return keys[i];
   };
-  unsigned mk = 0u;
+  unsigned mk = 0u, least = 0xFFFFFFFFu;
+  auto seen = [&](unsigned k) {
+    mk = max(mk, k);
+    if (k != 0u) least = min(least, k);
+  };
   if constexpr (RAW) {
     const unsigned short* x = (const unsigned short*)a.scores + base;
     const int head = (int)min((long long)N, (long long)((8 - (((unsigned long long)x >> 1) & 7)) & 7));   // entries in front of a 16-byte boundary
     auto put = [&](int i, unsigned u) {
       const unsigned k = key_16(u, a.type);
       keys16[i] = (unsigned short)(k >> 16);
-      mk = max(mk, k);
+      seen(k);
     };
     if (tid < head) put(tid, x[tid]);
     const int wide = (N - head) / 8;
@@ -314,14 +411,15 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
     for (int i = tid; i < N; i += NT) {
       const unsigned k = key_f32(x[i]);
       keys[i] = k;
-      mk = max(mk, k);
+      seen(k);
     }
   }
   mk = wave_max(mk);
-  if ((tid & 63) == 0) tmp32[tid >> 6] = mk;
+  least = ~wave_max(~least);
+  if (lane == 0) { tmp32[wave] = mk; s_min[wave] = least; }
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < NWV; ++w) mk = max(mk, tmp32[w]);
+  for (int w = 0; w < NWV; ++w) { mk = max(mk, tmp32[w]); least = min(least, s_min[w]); }
   if (mk == 0u) {                       // nothing to choose from
     for (int s = tid; s < a.S; s += NT) {
       a.out_id[(long long)b * a.S + s] = -1;
@@ -342,24 +440,41 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
     if (k > c.cut) return true;
     return k == c.cut && k != 0u && rank++ < c.ties;
   };
+  Steps steps;
   if (r.greedy) {
     c.cut = mk;
     c.ties = 1u;
   } else {
     if (r.k < N) {
-      if (tid == 0) { st = Select{0u, (unsigned)r.k, 0, 0.0, 0u}; cut_s = c; }
-      for (int round = 0; round <= LAST; ++round) {
+      steps.set(r, least, false);
+      if (tid == 0) { st = Select{0, 0u, 0u, (unsigned)r.k, 0, 0.0, 0u}; cut_s = c; s_n = 0u; }
+      if (tid < DIRECT) near_k[tid] = 0u;
+      for (int round = -1; round <= LAST; ++round) {
         for (int i = tid; i < SB; i += NT) hc[i] = 0u;
         __syncthreads();
         const unsigned prefix = st.prefix;
+        const int step = st.step;
 #pragma unroll 4
         for (int i = tid; i < N; i += NT) {
           const unsigned k = key_at(i);
-          if (k != 0u && round_in(k, round, prefix)) atomicAdd(&hc[bin_at<NT>(round_bin(k, round))], 1u);
+          if (k == 0u) continue;
+          const int t = steps.of(k);
+          if (round < 0) atomicAdd(&hc[bin_at<NT>(t)], 1u);
+          else if (t == step && round_in(k, round, prefix)) atomicAdd(&hc[bin_at<NT>(round_place(k, round))], 1u);
         }
         __syncthreads();
         pick_k<NT>(round, round == LAST, hc, &st, &cut_s, tmp32);
         if (st.done) break;
+        if (round < 0 && st.count <= DIRECT) {
+          const int at = st.step;
+          for (int i = tid; i < N; i += NT) {
+            const unsigned k = key_at(i);
+            if (k != 0u && steps.of(k) == at) near_k[atomicAdd(&s_n, 1u)] = k;
+          }
+          __syncthreads();
+          direct_k(near_k, (int)st.count, &st, &cut_s);
+          break;
+        }
       }
       c = cut_s;
       __syncthreads();
@@ -384,51 +499,55 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
         __syncthreads();
       }
     }
-    if (r.p < 1.0 && r.p > 0.0 && copied && n <= SPAIRS) {
-      // the weight in front of every entry; those that go become key 0
-      u64 w = 0, front = 0, total;
-      unsigned mine = 0u;
-      if (tid < n) {
-        mine = key_at(tid);
-        w = r.weight(mine) >> coarse;
-        hw[tid] = w;
-      }
-      block_before<NT>(w, tmp64, &total);                        // (its barriers publish hw)
-      if (tid < n) {
-#pragma unroll 4
-        for (int j = 0; j < n; ++j) {
-          const unsigned k = key_at(j);
-          const u64 wj = hw[j];
-          front += (k > mine || (k == mine && j < tid)) ? wj : 0;
-        }
-      }
-      __syncthreads();
-      if (tid < n && !((double)front < r.p * (double)total)) keys[tid] = 0u;
-      __syncthreads();
-    } else if (r.p < 1.0) {
-      if (tid == 0) { st = Select{0u, 0u, 0, 0.0, 0u}; cut_s = SampleCut{mk, 1u}; }   // (p <= 0: the largest alone)
-      for (int round = 0; round <= LAST && r.p > 0.0; ++round) {
+    if (r.p < 1.0) {
+      steps.set(r, least, true);
+      if (tid == 0) { st = Select{0, 0u, 0u, 0u, 0, 0.0, 0u}; cut_s = SampleCut{mk, 1u}; s_n = 0u; }   // (p <= 0: the largest alone)
+      if (tid < DIRECT) { near_k[tid] = 0u; near_w[tid] = 0; }
+      const bool few = n <= DIRECT && copied;                    // no histogram: all of them are compared
+      for (int round = few ? LAST + 1 : -1; round <= LAST && r.p > 0.0; ++round) {
         for (int i = tid; i < SB; i += NT) { hc[i] = 0u; hw[i] = 0; }
         __syncthreads();
         const unsigned prefix = st.prefix;
+        const int step = st.step;
+        auto count = [&](unsigned k, unsigned times) {
+          const int t = steps.of(k);
+          if (round >= 0 && !(t == step && round_in(k, round, prefix))) return;
+          const int d = bin_at<NT>(round < 0 ? t : round_place(k, round));
+          atomicAdd(&hc[d], times);
+          atomicAdd(&hw[d], (r.weight(k) >> coarse) * times);
+        };
         for (int i = tid; i < n; i += NT) {
           const unsigned k = key_at(i);
-          if (k <= c.cut || !round_in(k, round, prefix)) continue;
-          const u64 w = r.weight(k) >> coarse;
-          const int d = bin_at<NT>(round_bin(k, round));
-          atomicAdd(&hc[d], 1u);
-          atomicAdd(&hw[d], w);
+          if (k > c.cut) count(k, 1u);
         }
-        if (tid == 0 && c.cut != 0u && c.ties != 0u && round_in(c.cut, round, prefix)) {   // the ties that top-k left
-          const int d = bin_at<NT>(round_bin(c.cut, round));
-          atomicAdd(&hc[d], c.ties);
-          atomicAdd(&hw[d], (r.weight(c.cut) >> coarse) * c.ties);
-        }
+        if (tid == 0 && c.cut != 0u && c.ties != 0u) count(c.cut, c.ties);   // the ties that top-k left
         __syncthreads();
         pick_p<NT>(round, round == LAST, hc, hw, r.p, &st, &cut_s, tmp64);
-        if (st.done) break;
+        if (st.done || (round < 0 && st.count <= DIRECT)) break;
       }
       __syncthreads();
+      if (r.p > 0.0 && !st.done) {
+        const int at = st.step;
+        auto add = [&](unsigned k) {
+          const unsigned q = atomicAdd(&s_n, 1u);
+          near_k[q] = k;
+          near_w[q] = r.weight(k) >> coarse;
+        };
+        for (int i = tid; i < n; i += NT) {
+          const unsigned k = key_at(i);
+          if (k > c.cut && (few || steps.of(k) == at)) add(k);
+        }
+        if (tid == 0 && c.cut != 0u && c.ties != 0u && (few || steps.of(c.cut) == at))
+          for (unsigned t = 0; t < c.ties; ++t) add(c.cut);
+        __syncthreads();
+        if (few) {                                               // the limit: p times all of it
+          u64 total;
+          block_before<NT>(tid < DIRECT ? near_w[tid] : 0, tmp64, &total);
+          if (tid == 0) { st.limit = r.p * (double)total; st.count = s_n; }
+          __syncthreads();
+        }
+        direct_p(near_k, near_w, (int)st.count, &st, &cut_s);
+      }
       c = cut_s;
       __syncthreads();
     }
@@ -444,23 +563,51 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
   }
   const WSum front = block_before<NT>(mine, tmp64, &all);
   const u128 W = all.all(), from = front.all(), to = from + mine.all();
-  double log_W = 0.0;
-  bool have = false;
-  for (int s = 0; s < a.S; ++s) {       // the thread that the goal falls to walks its entries
-    const u128 goal = sample_goal(a.rand[(long long)b * a.S + s], W);
-    if (!(from <= goal && goal < to)) continue;
-    if (!have) { log_W = log(wide_to_double(W) * 2.168404344971009e-19); have = true; }   // 2^-62
-    u128 run = from;
-    rank = rank0;
-    for (int i = i0; i < i1; ++i) {
-      const unsigned k = key_at(i);
-      if (!stays(k, rank)) continue;
-      run += r.kept(k);
-      if (run > goal) {
-        const long long at = copied ? (long long)keys[n + i] : i;
-        a.out_id[(long long)b * a.S + s] = a.ids ? a.ids[(long long)b * a.ld_ids + at] : at;
-        a.out_logp[(long long)b * a.S + s] = r.greedy ? 0.f : (float)(r.z(k) - log_W);
-        break;
+  const double log_W = log(wide_to_double(W) * 2.168404344971009e-19);   // 2^-62
+  for (int s0 = 0; s0 < a.S; s0 += 64) {
+    const int ns = min(64, a.S - s0);
+    __syncthreads();
+    if (tid < ns) {
+      const u128 goal = sample_goal(a.rand[(long long)b * a.S + s0 + tid], W);
+      goal_hi[tid] = (u64)(goal >> 64);
+      goal_lo[tid] = (u64)goal;
+    }
+    __syncthreads();
+    if (from < to)
+      for (int s = 0; s < ns; ++s) {
+        const u128 goal = ((u128)goal_hi[s] << 64) + goal_lo[s];
+        if (from <= goal && goal < to) {   // one thread
+          owner[s] = tid;
+          owner_rank[s] = rank0;
+          from_hi[s] = (u64)(from >> 64);
+          from_lo[s] = (u64)from;
+        }
+      }
+    __syncthreads();
+    for (int s = wave; s < ns; s += NWV) {   // a wave looks at 64 of the owner's entries at a time
+      const u128 goal = ((u128)goal_hi[s] << 64) + goal_lo[s];
+      u128 run = ((u128)from_hi[s] << 64) + from_lo[s];
+      const int j0 = min(n, owner[s] * C), j1 = min(n, j0 + C);
+      unsigned ties = owner_rank[s];
+      for (int j = j0; j < j1; j += 64) {
+        const int i = j + lane;
+        const unsigned k = i < j1 ? key_at(i) : 0u;
+        const u64 eq = __ballot(k == c.cut && k != 0u);
+        unsigned my_rank = ties + (unsigned)__popcll(eq & ((1ull << lane) - 1ull));
+        ties += (unsigned)__popcll(eq);
+        WSum v{0, 0};
+        if (stays(k, my_rank)) v.add(r.kept(k));
+        const WSum up{wave_upto(v.hi), wave_upto(v.lo)};
+        const u64 over = __ballot(run + up.all() > goal);
+        if (over) {
+          if (lane == __ffsll(over) - 1) {
+            const long long at = copied ? (long long)keys[n + i] : i, o = (long long)b * a.S + s0 + s;
+            a.out_id[o] = a.ids ? a.ids[(long long)b * a.ld_ids + at] : at;
+            a.out_logp[o] = r.greedy ? 0.f : (float)(r.z(k) - log_W);
+          }
+          break;
+        }
+        run += WSum{last_lane(up.hi), last_lane(up.lo)}.all();
       }
     }
   }
@@ -472,11 +619,13 @@ struct SampleState {                      // per row, in the workspace
   Select st;
   SampleCut cut;                          // of the selections so far
   SampleCut kcut;                         // of top-k (the top-p rounds need it)
-  unsigned maxkey, arrived;
+  unsigned maxkey, minkey, arrived, listed;   // listed: entries of the border's step in the list
 };
+constexpr int LLIST = 4096;                   // a row's list
 struct SampleLong {
   SampleState* state; unsigned* hc; u64* hw;   // [B], [B][SB], [B][SB]
   unsigned* tb; u64* bs;                       // [B][nblk] ties of a block, [B][2 nblk] kept weight of a block
+  unsigned* list;                              // [B][LLIST] keys of the border's step
   int nblk, nchunk, coarse;
   int uses_k, uses_p;
 };
@@ -487,6 +636,7 @@ __global__ __launch_bounds__(256) void sample_init_kernel(SampleArgs a, SampleLo
   if (threadIdx.x == 0) {
     SampleState s{};
     s.cut = s.kcut = SampleCut{0u, ALL_TIES};
+    s.minkey = 0xFFFFFFFFu;
     g.state[b] = s;
   }
 }
@@ -531,13 +681,24 @@ __device__ __forceinline__ void sample_walk(const SampleArgs& a, long long base,
 __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a, SampleLong g) {
   const int b = blockIdx.y;
   const long long i0 = (long long)blockIdx.x * LCH, i1 = min(a.N, i0 + LCH);
-  unsigned mk = 0u;
-  sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) { mk = max(mk, k); });
+  unsigned mk = 0u, least = 0xFFFFFFFFu;
+  sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) {
+    mk = max(mk, k);
+    if (k != 0u) least = min(least, k);
+  });
   mk = wave_max(mk);
-  if ((threadIdx.x & 63) == 0 && mk) atomicMax(&g.state[b].maxkey, mk);
+  least = ~wave_max(~least);
+  if ((threadIdx.x & 63) == 0 && mk) {
+    atomicMax(&g.state[b].maxkey, mk);
+    atomicMin(&g.state[b].minkey, least);
+  }
 }
-// a round of the top-k (PHASE 0) or top-p (PHASE 1) selection: counts (and weights) of the prefix's entries by bin; the workgroup that
-// arrives last takes the decision and clears the bins for the next round
+template <int PHASE>
+__device__ __forceinline__ bool sample_active(const SampleArgs& a, const SampleRow& r, unsigned mk) {
+  return mk != 0u && !r.greedy && (PHASE == 0 ? r.k < a.N : r.p < 1.0 && r.p > 0.0);
+}
+// a round of the top-k (PHASE 0) or top-p (PHASE 1) selection: counts (and weights) of the steps (round -1) or of the border's step by bits;
+// the workgroup that arrives last takes the decision and clears the bins for the next round
 template <int PHASE>
 __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleLong g, int round, int mode) {
   __shared__ unsigned hc[SB];
@@ -551,16 +712,18 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
   SampleRow r;
   r.load(a, b);
   const unsigned mk = S->maxkey;
-  const bool active = mk != 0u && !r.greedy && (PHASE == 0 ? r.k < a.N : r.p < 1.0 && r.p > 0.0) && !(round > 0 && S->st.done);
-  if (!active) {
+  if (!sample_active<PHASE>(a, r, mk) || (round >= 0 && S->st.done)) {
     // a row whose p is not positive keeps its largest entry alone
-    if (PHASE == 1 && round == 0 && blockIdx.x == 0 && tid == 0 && mk != 0u && !r.greedy && r.p <= 0.0) S->cut = SampleCut{mk, 1u};
+    if (PHASE == 1 && round < 0 && blockIdx.x == 0 && tid == 0 && mk != 0u && !r.greedy && r.p <= 0.0) S->cut = SampleCut{mk, 1u};
     return;
   }
   r.set_max(mk);
+  Steps steps;
+  steps.set(r, S->minkey, PHASE == 1);
   unsigned* ghc = g.hc + (long long)b * SB;
   u64* ghw = g.hw + (long long)b * SB;
-  const unsigned prefix = round ? S->st.prefix : 0u;
+  const unsigned prefix = round >= 0 ? S->st.prefix : 0u;
+  const int step = round >= 0 ? S->st.step : 0;
   const SampleCut kc = S->kcut;
   for (int i = tid; i < SB; i += 256) {
     hc[i] = 0u;
@@ -568,18 +731,17 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
   }
   __syncthreads();
   const long long i0 = (long long)blockIdx.x * LCH, i1 = min(a.N, i0 + LCH);
+  auto count = [&](unsigned k, unsigned times) {
+    const int t = steps.of(k);
+    if (round >= 0 && !(t == step && round_in(k, round, prefix))) return;
+    const int d = bin_at<256>(round < 0 ? t : round_place(k, round));
+    atomicAdd(&hc[d], times);
+    if constexpr (PHASE == 1) atomicAdd(&hw[d], (r.weight(k) >> g.coarse) * times);
+  };
   sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) {
-    if (PHASE == 0 ? k == 0u : k <= kc.cut) return;
-    if (!round_in(k, round, prefix)) return;
-    const int d = bin_at<256>(round_bin(k, round));
-    atomicAdd(&hc[d], 1u);
-    if constexpr (PHASE == 1) atomicAdd(&hw[d], r.weight(k) >> g.coarse);
+    if (PHASE == 0 ? k != 0u : k > kc.cut) count(k, 1u);
   });
-  if (PHASE == 1 && blockIdx.x == 0 && tid == 0 && kc.cut != 0u && kc.ties != 0u && round_in(kc.cut, round, prefix)) {
-    const int d = bin_at<256>(round_bin(kc.cut, round));
-    atomicAdd(&hc[d], kc.ties);
-    atomicAdd(&hw[PHASE == 1 ? d : 0], (r.weight(kc.cut) >> g.coarse) * kc.ties);
-  }
+  if (PHASE == 1 && blockIdx.x == 0 && tid == 0 && kc.cut != 0u && kc.ties != 0u) count(kc.cut, kc.ties);
   __syncthreads();
   for (int i = tid; i < SB; i += 256)
     if (hc[i]) {
@@ -591,7 +753,7 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
   __syncthreads();
   if (!last) return;
   if (tid == 0) {
-    st = round ? S->st : Select{0u, (unsigned)min((long long)0x7FFFFFFF, r.k), 0, 0.0, 0u};
+    st = round >= 0 ? S->st : Select{0, 0u, 0u, (unsigned)min((long long)0x7FFFFFFF, r.k), 0, 0.0, 0u};
     cut = S->cut;
   }
   for (int i = tid; i < SB; i += 256) {
@@ -604,6 +766,92 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
   const bool last_round = round == (a.type == UR_F32 ? 2 : 1);
   if constexpr (PHASE == 0) pick_k<256>(round, last_round, hc, &st, &cut, tmp32);
   else pick_p<256>(round, last_round, hc, hw, r.p, &st, &cut, tmp64);
+  if (tid == 0) {
+    S->st = st;
+    S->cut = cut;
+    if (PHASE == 0) S->kcut = cut;
+    S->arrived = 0u;
+    S->listed = 0u;
+  }
+}
+// the entries of the border's step, where the list holds them: collected by all, and the border found among them by the last to arrive
+// (radix rounds over the list in LDS).  Rows with more go through the rounds over memory.
+template <int PHASE>
+__global__ __launch_bounds__(256) void sample_near_kernel(SampleArgs a, SampleLong g, int mode) {
+  __shared__ unsigned hc[SB];
+  __shared__ __attribute__((aligned(16))) unsigned lk[LLIST];
+  __shared__ u64 hw[PHASE == 1 ? SB : 1];
+  __shared__ unsigned tmp32[4], last, n_s, at_s;
+  __shared__ u64 tmp64[4];
+  __shared__ Select st;
+  __shared__ SampleCut cut;
+  const int b = blockIdx.y, tid = threadIdx.x;
+  SampleState* S = g.state + b;
+  SampleRow r;
+  r.load(a, b);
+  const unsigned mk = S->maxkey;
+  if (!sample_active<PHASE>(a, r, mk) || S->st.done || S->st.count > LLIST) return;
+  r.set_max(mk);
+  Steps steps;
+  steps.set(r, S->minkey, PHASE == 1);
+  const int step = S->st.step;
+  const SampleCut kc = S->kcut;
+  unsigned* list = g.list + (long long)b * LLIST;
+  if (tid == 0) n_s = 0u;
+  __syncthreads();
+  const long long i0 = (long long)blockIdx.x * LCH, i1 = min(a.N, i0 + LCH);
+  sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) {
+    if ((PHASE == 0 ? k != 0u : k > kc.cut) && steps.of(k) == step) lk[atomicAdd(&n_s, 1u)] = k;   // (at most st.count of them)
+  });
+  __syncthreads();
+  const unsigned n = n_s;
+  if (tid == 0 && n) at_s = atomicAdd(&S->listed, n);
+  __syncthreads();
+  for (unsigned i = tid; i < n; i += 256) __hip_atomic_store(list + at_s + i, lk[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (tid == 0) last = ur_arrive(&S->arrived, mode) == (unsigned)g.nchunk - 1u;
+  __syncthreads();
+  if (!last) return;
+  if (tid == 0) {
+    st = S->st;
+    cut = S->cut;
+    n_s = agent_load(&S->listed);
+  }
+  __syncthreads();
+  const unsigned all = n_s;
+  for (unsigned i = tid; i < all; i += 256) lk[i] = agent_load(list + i);
+  const int rounds = a.type == UR_F32 ? 3 : 2;
+  if (st.count <= DIRECT && st.count == all) {   // few (and no ties that top-k left among them): compared with each other
+    __syncthreads();
+    if (tid >= (int)all && tid < DIRECT) lk[tid] = 0u;
+    if constexpr (PHASE == 1) {
+      if (tid < DIRECT) hw[tid] = tid < (int)all ? r.weight(lk[tid]) >> g.coarse : 0;
+    }
+    __syncthreads();
+    if constexpr (PHASE == 0) direct_k(lk, (int)all, &st, &cut);
+    else direct_p(lk, hw, (int)all, &st, &cut);
+    if (tid == 0) st.done = 1u;
+    __syncthreads();
+  }
+  for (int round = 0; round < rounds && !st.done; ++round) {
+    for (int i = tid; i < SB; i += 256) {
+      hc[i] = 0u;
+      if (PHASE == 1) hw[i] = 0;
+    }
+    __syncthreads();
+    const unsigned prefix = st.prefix;
+    auto count = [&](unsigned k, unsigned times) {
+      if (!round_in(k, round, prefix)) return;
+      const int d = bin_at<256>(round_place(k, round));
+      atomicAdd(&hc[d], times);
+      if constexpr (PHASE == 1) atomicAdd(&hw[d], (r.weight(k) >> g.coarse) * times);
+    };
+    for (unsigned i = tid; i < all; i += 256) count(lk[i], 1u);
+    if (PHASE == 1 && tid == 0 && kc.cut != 0u && kc.ties != 0u && steps.of(kc.cut) == step) count(kc.cut, kc.ties);
+    __syncthreads();
+    if constexpr (PHASE == 0) pick_k<256>(round, round == rounds - 1, hc, &st, &cut, tmp32);
+    else pick_p<256>(round, round == rounds - 1, hc, hw, r.p, &st, &cut, tmp64);
+  }
   if (tid == 0) {
     S->st = st;
     S->cut = cut;
@@ -782,13 +1030,14 @@ static size_t sample_long_bytes(long long N, int B, char* base, SampleLong* g) {
   w.state = (SampleState*)take(sizeof(SampleState) * B);
   w.hc = (unsigned*)take((size_t)B * SB * 4); w.hw = (u64*)take((size_t)B * SB * 8);
   w.tb = (unsigned*)take((size_t)B * w.nblk * 4); w.bs = (u64*)take((size_t)B * w.nblk * 16);
+  w.list = (unsigned*)take((size_t)B * LLIST * 4);
   if (g) *g = w;
   return o;
 }
 template <int NT, bool RAW>
 static int launch_sample_row(const SampleArgs& a, hipStream_t st) {
   const size_t lds = (size_t)SB * 12 + (size_t)a.N * (RAW ? 2 : 4) + 16;
-  static const hipError_t attr = hipFuncSetAttribute((const void*)sample_row_kernel<NT, RAW>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 512);
+  static const hipError_t attr = hipFuncSetAttribute((const void*)sample_row_kernel<NT, RAW>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 6144);
   (void)attr;
   hipLaunchKernelGGL((sample_row_kernel<NT, RAW>), dim3(a.B), dim3(NT), lds, st, a, log2_up(a.N));
   UR_LAUNCH_CHECK();
@@ -841,14 +1090,21 @@ extern "C" int ur_sample_scores(const void* scores, int32_t score_type, int64_t 
   hipLaunchKernelGGL(sample_max_kernel, grid, dim3(256), 0, st, a, g);
   UR_LAUNCH_CHECK();
   const int rounds = score_type == UR_F32 ? 3 : 2;
-  for (int round = 0; round < rounds && g.uses_k; ++round) {
-    hipLaunchKernelGGL((sample_round_kernel<0>), grid, dim3(256), 0, st, a, g, round, mode);
-    UR_LAUNCH_CHECK();
-  }
-  for (int round = 0; round < rounds && g.uses_p; ++round) {
-    hipLaunchKernelGGL((sample_round_kernel<1>), grid, dim3(256), 0, st, a, g, round, mode);
-    UR_LAUNCH_CHECK();
-  }
+  auto select = [&](auto phase) -> int {
+    constexpr int PHASE = decltype(phase)::value;
+    for (int round = -1; round < rounds; ++round) {
+      hipLaunchKernelGGL((sample_round_kernel<PHASE>), grid, dim3(256), 0, st, a, g, round, mode);
+      UR_LAUNCH_CHECK();
+      if (round < 0) {
+        hipLaunchKernelGGL((sample_near_kernel<PHASE>), grid, dim3(256), 0, st, a, g, mode);
+        UR_LAUNCH_CHECK();
+      }
+    }
+    return UR_OK;
+  };
+  int rc = g.uses_k ? select(std::integral_constant<int, 0>()) : UR_OK;
+  if (rc) return rc;
+  if (g.uses_p && (rc = select(std::integral_constant<int, 1>()))) return rc;
   if (g.uses_k || g.uses_p || temperature_rows || temperature == 0.0) {
     hipLaunchKernelGGL(sample_ties_kernel, grid, dim3(256), 0, st, a, g);
     UR_LAUNCH_CHECK();
