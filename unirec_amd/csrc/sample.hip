@@ -13,8 +13,8 @@
 // 2^-(62 - log2 N) in one).  No result depends on an order of additions or on how a row was cut into pieces.
 //
 // Two forms.  A row that fits into LDS (32 768 entries; 65 536 of 16 bits): one workgroup, one read of the row, every pass from LDS.
-// Longer rows: workgroups of 16 384 entries, a pass over memory each for the maximum, every round of a selection and the kept sums, the
-// decisions between the passes taken by the workgroup that arrives last.
+// Longer rows: many workgroups a row, a pass over memory each for the maximum, for a selection's histogram and its border's step, and for the
+// kept sums.
 #include <math.h>
 
 #include <algorithm>
@@ -192,20 +192,39 @@ __device__ __forceinline__ unsigned ties_within(u64 above, u64 w, double limit, 
 
 // ---- a selection: a histogram over equal steps of the score (round -1), then rounds over the bits of the keys of one step
 constexpr int SB = 2048;
-struct Steps {   // step of a score: (max - x) c, monotone in x; double: no difference of two floats overflows
-  double c; float m; int type; bool flat;
+struct Steps {   // step of a score: (max / 2 - x / 2) c, never larger for a larger score (fp32 rounding keeps an order); halves: no difference overflows
+  float half_m, c; float m; int type; bool flat;
   __device__ __forceinline__ void set(const SampleRow& r, unsigned minkey, bool weights) {
     m = r.m; type = r.type; flat = r.flat;
-    double range = (double)r.m - (double)key_value(minkey, r.type);
-    if (weights) range = fmin(range, 43.0 / r.inv_T);            // (steps behind that weigh nothing: one bin)
-    c = range > 0.0 ? (double)SB / range : 0.0;
+    half_m = 0.5f * m;
+    double range = 0.5 * ((double)r.m - (double)key_value(minkey, r.type));
+    if (weights) range = fmin(range, 21.5 / r.inv_T);            // (steps behind 43 T weigh nothing: one bin)
+    c = range > 0.0 ? (float)fmin((double)SB / range, 1e38) : 0.f;
   }
   __device__ __forceinline__ int of(unsigned key) const {
     const float x = key_value(key, type);
     if (flat) return x == m ? 0 : SB - 1;
-    return (int)fmin(((double)m - (double)x) * c, (double)(SB - 1));
+    const float t = fmaf(x, -0.5f, half_m) * c;
+    return t < (float)(SB - 1) ? (int)t : SB - 1;                // (a pattern that is no number: the last)
   }
 };
+// the smallest key whose step is at most s, searched by a wave, 64 keys at a time (mk's step is 0)
+__device__ __forceinline__ unsigned first_key(const Steps& steps, int s, unsigned mk) {
+  const unsigned lane = threadIdx.x & 63;
+  unsigned lo = 1u, hi = mk;
+  while (lo < hi) {
+    const unsigned probe = lo + (unsigned)(((u64)(hi - lo) * lane) >> 6);
+    const u64 in = __ballot(steps.of(probe) <= s);
+    if (in == 0ull) {
+      lo = (unsigned)__builtin_amdgcn_readlane((int)probe, 63) + 1u;
+    } else {
+      const int f = __builtin_amdgcn_readfirstlane(__ffsll(in) - 1);
+      hi = (unsigned)__builtin_amdgcn_readlane((int)probe, f);
+      if (f > 0) lo = (unsigned)__builtin_amdgcn_readlane((int)probe, f - 1) + 1u;
+    }
+  }
+  return hi;
+}
 __device__ __forceinline__ int round_shift(int round) { return round == 0 ? 21 : round == 1 ? 10 : 0; }
 __device__ __forceinline__ int round_place(unsigned key, int round) {   // from the highest key down
   return SB - 1 - (int)((key >> round_shift(round)) & (round == 2 ? 1023u : 2047u));
@@ -218,7 +237,8 @@ __device__ __forceinline__ bool round_in(unsigned key, int round, unsigned prefi
   return round == 0 || (round == 1 ? key >> 21 : key >> 10) == prefix;
 }
 struct Select {   // state of a selection (one per row)
-  int step; unsigned prefix; unsigned count;   // the step, the key's bits so far, and the entries that share them
+  int step; unsigned lo, hi;            // the border's step, its keys [lo, hi]
+  unsigned prefix, count;               // the key's bits so far, and the entries that share them
   unsigned need;                        // top-k: how many of those stay
   u64 above; double limit;              // top-p: the weight in front of them, p times all of it
   unsigned done;
@@ -304,6 +324,18 @@ __device__ __forceinline__ void pick_p(int round, bool last, const unsigned* hc,
   }
   __syncthreads();
 }
+// the keys of the step that the border fell into (two waves, a barrier)
+__device__ __forceinline__ void step_keys(const Steps& steps, unsigned mk, Select* st) {
+  const int wave = threadIdx.x >> 6, at = st->step;
+  if (wave == 0) {
+    const unsigned lo = first_key(steps, at, mk);
+    if (threadIdx.x == 0) st->lo = lo;
+  } else if (wave == 1) {
+    const unsigned above = at > 0 ? first_key(steps, at - 1, mk) : 0u;
+    if (threadIdx.x == 64) st->hi = at > 0 ? above - 1u : mk;
+  }
+  __syncthreads();
+}
 // the border among `n` <= DIRECT keys of one step, compared with each other (lists padded with key 0 to a multiple of 8)
 constexpr int DIRECT = 128;
 __device__ __forceinline__ void direct_k(const unsigned* keys, int n, const Select* st, SampleCut* cut) {
@@ -367,11 +399,10 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
   __shared__ SampleCut cut_s;
   __shared__ __attribute__((aligned(16))) unsigned near_k[DIRECT];
   __shared__ u64 near_w[DIRECT];
-  __shared__ u64 goal_hi[64], goal_lo[64], from_hi[64], from_lo[64];
-  __shared__ int owner[64];
-  __shared__ unsigned owner_rank[64];
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, N = (int)a.N;
   const long long base = (long long)b * a.ld;
+  constexpr int DRAWS = 4;              // draws that a wave takes at a time
+  const float u_first = lane < DRAWS && wave * DRAWS + lane < a.S ? a.rand[(long long)b * a.S + wave * DRAWS + lane] : 0.f;   // asked for early
   SampleRow r;
   r.load(a, b);
   int n = N;                            // entries in hand
@@ -447,29 +478,35 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
   } else {
     if (r.k < N) {
       steps.set(r, least, false);
-      if (tid == 0) { st = Select{0, 0u, 0u, (unsigned)r.k, 0, 0.0, 0u}; cut_s = c; s_n = 0u; }
+      if (tid == 0) { st = Select{0, 0u, 0u, 0u, 0u, (unsigned)r.k, 0, 0.0, 0u}; cut_s = c; s_n = 0u; }
       if (tid < DIRECT) near_k[tid] = 0u;
       for (int round = -1; round <= LAST; ++round) {
         for (int i = tid; i < SB; i += NT) hc[i] = 0u;
         __syncthreads();
-        const unsigned prefix = st.prefix;
-        const int step = st.step;
+        const unsigned prefix = st.prefix, lo = st.lo, hi = st.hi;
+        if (round < 0) {
 #pragma unroll 4
-        for (int i = tid; i < N; i += NT) {
-          const unsigned k = key_at(i);
-          if (k == 0u) continue;
-          const int t = steps.of(k);
-          if (round < 0) atomicAdd(&hc[bin_at<NT>(t)], 1u);
-          else if (t == step && round_in(k, round, prefix)) atomicAdd(&hc[bin_at<NT>(round_place(k, round))], 1u);
+          for (int i = tid; i < N; i += NT) {
+            const unsigned k = key_at(i);
+            if (k != 0u) atomicAdd(&hc[bin_at<NT>(steps.of(k))], 1u);
+          }
+        } else {
+#pragma unroll 4
+          for (int i = tid; i < N; i += NT) {
+            const unsigned k = key_at(i);
+            if (k >= lo && k <= hi && round_in(k, round, prefix)) atomicAdd(&hc[bin_at<NT>(round_place(k, round))], 1u);
+          }
         }
         __syncthreads();
         pick_k<NT>(round, round == LAST, hc, &st, &cut_s, tmp32);
         if (st.done) break;
+        if (round < 0) step_keys(steps, mk, &st);
         if (round < 0 && st.count <= DIRECT) {
-          const int at = st.step;
+          const unsigned lo = st.lo, hi = st.hi;
+#pragma unroll 4
           for (int i = tid; i < N; i += NT) {
             const unsigned k = key_at(i);
-            if (k != 0u && steps.of(k) == at) near_k[atomicAdd(&s_n, 1u)] = k;
+            if (k >= lo && k <= hi) near_k[atomicAdd(&s_n, 1u)] = k;
           }
           __syncthreads();
           direct_k(near_k, (int)st.count, &st, &cut_s);
@@ -501,18 +538,16 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
     }
     if (r.p < 1.0) {
       steps.set(r, least, true);
-      if (tid == 0) { st = Select{0, 0u, 0u, 0u, 0, 0.0, 0u}; cut_s = SampleCut{mk, 1u}; s_n = 0u; }   // (p <= 0: the largest alone)
+      if (tid == 0) { st = Select{0, 1u, mk, 0u, 0u, 0u, 0, 0.0, 0u}; cut_s = SampleCut{mk, 1u}; s_n = 0u; }   // (p <= 0: the largest alone)
       if (tid < DIRECT) { near_k[tid] = 0u; near_w[tid] = 0; }
       const bool few = n <= DIRECT && copied;                    // no histogram: all of them are compared
       for (int round = few ? LAST + 1 : -1; round <= LAST && r.p > 0.0; ++round) {
         for (int i = tid; i < SB; i += NT) { hc[i] = 0u; hw[i] = 0; }
         __syncthreads();
-        const unsigned prefix = st.prefix;
-        const int step = st.step;
+        const unsigned prefix = st.prefix, lo = st.lo, hi = st.hi;
         auto count = [&](unsigned k, unsigned times) {
-          const int t = steps.of(k);
-          if (round >= 0 && !(t == step && round_in(k, round, prefix))) return;
-          const int d = bin_at<NT>(round < 0 ? t : round_place(k, round));
+          if (round >= 0 && !(k >= lo && k <= hi && round_in(k, round, prefix))) return;
+          const int d = bin_at<NT>(round < 0 ? steps.of(k) : round_place(k, round));
           atomicAdd(&hc[d], times);
           atomicAdd(&hw[d], (r.weight(k) >> coarse) * times);
         };
@@ -523,11 +558,12 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
         if (tid == 0 && c.cut != 0u && c.ties != 0u) count(c.cut, c.ties);   // the ties that top-k left
         __syncthreads();
         pick_p<NT>(round, round == LAST, hc, hw, r.p, &st, &cut_s, tmp64);
+        if (round < 0) step_keys(steps, mk, &st);
         if (st.done || (round < 0 && st.count <= DIRECT)) break;
       }
       __syncthreads();
       if (r.p > 0.0 && !st.done) {
-        const int at = st.step;
+        const unsigned lo = st.lo, hi = st.hi;                   // (few: all keys)
         auto add = [&](unsigned k) {
           const unsigned q = atomicAdd(&s_n, 1u);
           near_k[q] = k;
@@ -535,9 +571,9 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
         };
         for (int i = tid; i < n; i += NT) {
           const unsigned k = key_at(i);
-          if (k > c.cut && (few || steps.of(k) == at)) add(k);
+          if (k > c.cut && k >= lo && k <= hi) add(k);
         }
-        if (tid == 0 && c.cut != 0u && c.ties != 0u && (few || steps.of(c.cut) == at))
+        if (tid == 0 && c.cut != 0u && c.ties != 0u && c.cut >= lo && c.cut <= hi)
           for (unsigned t = 0; t < c.ties; ++t) add(c.cut);
         __syncthreads();
         if (few) {                                               // the limit: p times all of it
@@ -562,33 +598,36 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
     if (stays(k, rank)) mine.add(r.kept(k));
   }
   const WSum front = block_before<NT>(mine, tmp64, &all);
-  const u128 W = all.all(), from = front.all(), to = from + mine.all();
+  const u128 W = all.all();
   const double log_W = log(wide_to_double(W) * 2.168404344971009e-19);   // 2^-62
-  for (int s0 = 0; s0 < a.S; s0 += 64) {
-    const int ns = min(64, a.S - s0);
-    __syncthreads();
-    if (tid < ns) {
-      const u128 goal = sample_goal(a.rand[(long long)b * a.S + s0 + tid], W);
-      goal_hi[tid] = (u64)(goal >> 64);
-      goal_lo[tid] = (u64)goal;
+  u64* from_hi = hw;                                             // [NT] (the histograms are done with): what lies in front of a thread's entries
+  u64* from_lo = hw + NT;                                        // [NT]
+  unsigned* ranks = hc;                                          // [NT]
+  from_hi[tid] = front.hi;
+  from_lo[tid] = front.lo;
+  ranks[tid] = rank0;
+  __syncthreads();
+  // a wave takes a few draws, a lane of it finds the thread that a goal falls to (the last that does not begin behind it); then the wave looks
+  // at 64 of that thread's entries at a time, draw after draw
+  for (int s0 = wave * DRAWS; s0 < a.S; s0 += NWV * DRAWS) {
+    const int ns = min(DRAWS, a.S - s0);
+    u128 my_goal = 0;
+    int owner = 0;
+    if (lane < ns) {
+      my_goal = sample_goal(s0 == wave * DRAWS ? u_first : a.rand[(long long)b * a.S + s0 + lane], W);
+#pragma unroll
+      for (int o = NT / 2; o > 0; o >>= 1)
+        if (WSum{from_hi[owner + o], from_lo[owner + o]}.all() <= my_goal) owner += o;
     }
-    __syncthreads();
-    if (from < to)
-      for (int s = 0; s < ns; ++s) {
-        const u128 goal = ((u128)goal_hi[s] << 64) + goal_lo[s];
-        if (from <= goal && goal < to) {   // one thread
-          owner[s] = tid;
-          owner_rank[s] = rank0;
-          from_hi[s] = (u64)(from >> 64);
-          from_lo[s] = (u64)from;
-        }
-      }
-    __syncthreads();
-    for (int s = wave; s < ns; s += NWV) {   // a wave looks at 64 of the owner's entries at a time
-      const u128 goal = ((u128)goal_hi[s] << 64) + goal_lo[s];
-      u128 run = ((u128)from_hi[s] << 64) + from_lo[s];
-      const int j0 = min(n, owner[s] * C), j1 = min(n, j0 + C);
-      unsigned ties = owner_rank[s];
+    for (int s = 0; s < ns; ++s) {
+      const int t = __builtin_amdgcn_readlane(owner, s);
+      const u128 goal = ((u128)(((u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(my_goal >> 96), s) << 32) |
+                                (unsigned)__builtin_amdgcn_readlane((int)(unsigned)(my_goal >> 64), s)) << 64) |
+                        (((u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(my_goal >> 32), s) << 32) |
+                         (unsigned)__builtin_amdgcn_readlane((int)(unsigned)my_goal, s));
+      u128 run = WSum{from_hi[t], from_lo[t]}.all();
+      const int j0 = min(n, t * C), j1 = min(n, j0 + C);
+      unsigned ties = ranks[t];
       for (int j = j0; j < j1; j += 64) {
         const int i = j + lane;
         const unsigned k = i < j1 ? key_at(i) : 0u;
@@ -614,19 +653,20 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
 }
 
 // ---------------------------------------------------------------------------------------------- longer rows
-constexpr int LCH = 16384, LBLK = 2048;   // entries of a workgroup; of a block of the kept sums
+constexpr int LBLK = 2048;                // entries of a block of the kept sums
 struct SampleState {                      // per row, in the workspace
   Select st;
   SampleCut cut;                          // of the selections so far
   SampleCut kcut;                         // of top-k (the top-p rounds need it)
   unsigned maxkey, minkey, arrived, listed;   // listed: entries of the border's step in the list
 };
-constexpr int LLIST = 4096;                   // a row's list
+constexpr int LLIST = 8192;                   // a row's list
 struct SampleLong {
   SampleState* state; unsigned* hc; u64* hw;   // [B], [B][SB], [B][SB]
   unsigned* tb; u64* bs;                       // [B][nblk] ties of a block, [B][2 nblk] kept weight of a block
   unsigned* list;                              // [B][LLIST] keys of the border's step
   int nblk, nchunk, coarse;
+  int chunk;                                   // entries of a workgroup, a multiple of 4 096
   int uses_k, uses_p;
 };
 
@@ -664,23 +704,29 @@ __device__ __forceinline__ Four sample_four(const SampleArgs& a, long long base,
   }
   return r;
 }
-// a workgroup's entries, f(key); four wide loads of a thread are under way together
+// a workgroup's entries, f(key): four wide loads of a thread under way while the four before them are looked at
 template <typename F>
 __device__ __forceinline__ void sample_walk(const SampleArgs& a, long long base, long long i0, long long i1, F f) {
   const bool wide = sample_wide(a, base + i0);
-  for (long long i = i0 + 4 * threadIdx.x; i < i1; i += 4096) {
-    Four v[4];
+  Four v[4];
+  long long i = i0 + 4 * threadIdx.x;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) v[u] = sample_four(a, base, i + 1024 * u, i1, wide);
+  for (int u = 0; u < 4; ++u) v[u] = sample_four(a, base, i + 1024 * u, i1, wide);
+  for (; i < i1; i += 4096) {
+    Four w[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) w[u] = sample_four(a, base, i + 4096 + 1024 * u, i1, wide);
 #pragma unroll
     for (int u = 0; u < 4; ++u)
 #pragma unroll
       for (int j = 0; j < 4; ++j) f(v[u].k[j]);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = w[u];
   }
 }
 __global__ __launch_bounds__(256) void sample_max_kernel(SampleArgs a, SampleLong g) {
   const int b = blockIdx.y;
-  const long long i0 = (long long)blockIdx.x * LCH, i1 = min(a.N, i0 + LCH);
+  const long long i0 = (long long)blockIdx.x * g.chunk, i1 = min(a.N, i0 + g.chunk);
   unsigned mk = 0u, least = 0xFFFFFFFFu;
   sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) {
     mk = max(mk, k);
@@ -697,10 +743,10 @@ template <int PHASE>
 __device__ __forceinline__ bool sample_active(const SampleArgs& a, const SampleRow& r, unsigned mk) {
   return mk != 0u && !r.greedy && (PHASE == 0 ? r.k < a.N : r.p < 1.0 && r.p > 0.0);
 }
-// a round of the top-k (PHASE 0) or top-p (PHASE 1) selection: counts (and weights) of the steps (round -1) or of the border's step by bits;
-// the workgroup that arrives last takes the decision and clears the bins for the next round
+// the top-k (PHASE 0) or top-p (PHASE 1) selection: counts (and weights) of the steps; the workgroup that arrives last finds the border's step
+// and clears the bins
 template <int PHASE>
-__global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleLong g, int round, int mode) {
+__global__ __launch_bounds__(256) void sample_steps_kernel(SampleArgs a, SampleLong g, int mode) {
   __shared__ unsigned hc[SB];
   __shared__ u64 hw[PHASE == 1 ? SB : 1];
   __shared__ unsigned tmp32[4], last;
@@ -712,9 +758,9 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
   SampleRow r;
   r.load(a, b);
   const unsigned mk = S->maxkey;
-  if (!sample_active<PHASE>(a, r, mk) || (round >= 0 && S->st.done)) {
+  if (!sample_active<PHASE>(a, r, mk)) {
     // a row whose p is not positive keeps its largest entry alone
-    if (PHASE == 1 && round < 0 && blockIdx.x == 0 && tid == 0 && mk != 0u && !r.greedy && r.p <= 0.0) S->cut = SampleCut{mk, 1u};
+    if (PHASE == 1 && blockIdx.x == 0 && tid == 0 && mk != 0u && !r.greedy && r.p <= 0.0) S->cut = SampleCut{mk, 1u};
     return;
   }
   r.set_max(mk);
@@ -722,19 +768,15 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
   steps.set(r, S->minkey, PHASE == 1);
   unsigned* ghc = g.hc + (long long)b * SB;
   u64* ghw = g.hw + (long long)b * SB;
-  const unsigned prefix = round >= 0 ? S->st.prefix : 0u;
-  const int step = round >= 0 ? S->st.step : 0;
   const SampleCut kc = S->kcut;
   for (int i = tid; i < SB; i += 256) {
     hc[i] = 0u;
     if (PHASE == 1) hw[i] = 0;
   }
   __syncthreads();
-  const long long i0 = (long long)blockIdx.x * LCH, i1 = min(a.N, i0 + LCH);
+  const long long i0 = (long long)blockIdx.x * g.chunk, i1 = min(a.N, i0 + g.chunk);
   auto count = [&](unsigned k, unsigned times) {
-    const int t = steps.of(k);
-    if (round >= 0 && !(t == step && round_in(k, round, prefix))) return;
-    const int d = bin_at<256>(round < 0 ? t : round_place(k, round));
+    const int d = bin_at<256>(steps.of(k));
     atomicAdd(&hc[d], times);
     if constexpr (PHASE == 1) atomicAdd(&hw[d], (r.weight(k) >> g.coarse) * times);
   };
@@ -753,7 +795,7 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
   __syncthreads();
   if (!last) return;
   if (tid == 0) {
-    st = round >= 0 ? S->st : Select{0, 0u, 0u, (unsigned)min((long long)0x7FFFFFFF, r.k), 0, 0.0, 0u};
+    st = Select{0, 1u, mk, 0u, 0u, (unsigned)min((long long)0x7FFFFFFF, r.k), 0, 0.0, 0u};
     cut = S->cut;
   }
   for (int i = tid; i < SB; i += 256) {
@@ -763,78 +805,81 @@ __global__ __launch_bounds__(256) void sample_round_kernel(SampleArgs a, SampleL
     if (PHASE == 1) ghw[i] = 0;
   }
   __syncthreads();
-  const bool last_round = round == (a.type == UR_F32 ? 2 : 1);
-  if constexpr (PHASE == 0) pick_k<256>(round, last_round, hc, &st, &cut, tmp32);
-  else pick_p<256>(round, last_round, hc, hw, r.p, &st, &cut, tmp64);
+  if constexpr (PHASE == 0) pick_k<256>(-1, false, hc, &st, &cut, tmp32);
+  else pick_p<256>(-1, false, hc, hw, r.p, &st, &cut, tmp64);
+  step_keys(steps, mk, &st);
   if (tid == 0) {
     S->st = st;
-    S->cut = cut;
-    if (PHASE == 0) S->kcut = cut;
     S->arrived = 0u;
     S->listed = 0u;
   }
 }
-// the entries of the border's step, where the list holds them: collected by all, and the border found among them by the last to arrive
-// (radix rounds over the list in LDS).  Rows with more go through the rounds over memory.
+// the keys of the border's step, put together (a list that holds them all)
 template <int PHASE>
-__global__ __launch_bounds__(256) void sample_near_kernel(SampleArgs a, SampleLong g, int mode) {
-  __shared__ unsigned hc[SB];
-  __shared__ __attribute__((aligned(16))) unsigned lk[LLIST];
-  __shared__ u64 hw[PHASE == 1 ? SB : 1];
-  __shared__ unsigned tmp32[4], last, n_s, at_s;
-  __shared__ u64 tmp64[4];
-  __shared__ Select st;
-  __shared__ SampleCut cut;
+__global__ __launch_bounds__(256) void sample_near_kernel(SampleArgs a, SampleLong g) {
+  __shared__ unsigned lk[LLIST], n_s, at_s;
   const int b = blockIdx.y, tid = threadIdx.x;
   SampleState* S = g.state + b;
   SampleRow r;
   r.load(a, b);
-  const unsigned mk = S->maxkey;
-  if (!sample_active<PHASE>(a, r, mk) || S->st.done || S->st.count > LLIST) return;
-  r.set_max(mk);
-  Steps steps;
-  steps.set(r, S->minkey, PHASE == 1);
-  const int step = S->st.step;
-  const SampleCut kc = S->kcut;
-  unsigned* list = g.list + (long long)b * LLIST;
+  if (!sample_active<PHASE>(a, r, S->maxkey) || S->st.done || S->st.count > LLIST) return;
+  const unsigned lo = PHASE == 0 ? S->st.lo : max(S->st.lo, S->kcut.cut + 1u), hi = S->st.hi;
   if (tid == 0) n_s = 0u;
   __syncthreads();
-  const long long i0 = (long long)blockIdx.x * LCH, i1 = min(a.N, i0 + LCH);
+  const long long i0 = (long long)blockIdx.x * g.chunk, i1 = min(a.N, i0 + g.chunk);
   sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) {
-    if ((PHASE == 0 ? k != 0u : k > kc.cut) && steps.of(k) == step) lk[atomicAdd(&n_s, 1u)] = k;   // (at most st.count of them)
+    if (k >= lo && k <= hi) lk[atomicAdd(&n_s, 1u)] = k;         // (at most st.count of them)
   });
   __syncthreads();
   const unsigned n = n_s;
-  if (tid == 0 && n) at_s = atomicAdd(&S->listed, n);
+  if (n == 0u) return;
+  if (tid == 0) at_s = atomicAdd(&S->listed, n);
   __syncthreads();
-  for (unsigned i = tid; i < n; i += 256) __hip_atomic_store(list + at_s + i, lk[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  unsigned* list = g.list + (long long)b * LLIST + at_s;
+  for (unsigned i = tid; i < n; i += 256) list[i] = lk[i];
+}
+// the border among them: compared directly, or radix rounds over the list (over the row where the list could not hold them)
+template <int PHASE>
+__global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, SampleLong g) {
+  constexpr int NT = 1024;
+  __shared__ unsigned hc[SB];
+  __shared__ u64 hw[PHASE == 1 ? SB : 1];
+  __shared__ __attribute__((aligned(16))) unsigned near_k[DIRECT];
+  __shared__ u64 near_w[PHASE == 1 ? DIRECT : 1];
+  __shared__ unsigned tmp32[NT / 64];
+  __shared__ u64 tmp64[NT / 64];
+  __shared__ Select st;
+  __shared__ SampleCut cut;
+  const int b = blockIdx.x, tid = threadIdx.x;
+  SampleState* S = g.state + b;
+  SampleRow r;
+  r.load(a, b);
+  const unsigned mk = S->maxkey;
+  if (!sample_active<PHASE>(a, r, mk) || S->st.done) return;
+  r.set_max(mk);
+  const SampleCut kc = S->kcut;
+  const bool listed = S->st.count <= LLIST;
+  const unsigned n = listed ? S->listed : 0u;
+  const unsigned* list = g.list + (long long)b * LLIST;
+  if (tid == 0) { st = S->st; cut = S->cut; }
   __syncthreads();
-  if (tid == 0) last = ur_arrive(&S->arrived, mode) == (unsigned)g.nchunk - 1u;
-  __syncthreads();
-  if (!last) return;
-  if (tid == 0) {
-    st = S->st;
-    cut = S->cut;
-    n_s = agent_load(&S->listed);
-  }
-  __syncthreads();
-  const unsigned all = n_s;
-  for (unsigned i = tid; i < all; i += 256) lk[i] = agent_load(list + i);
-  const int rounds = a.type == UR_F32 ? 3 : 2;
-  if (st.count <= DIRECT && st.count == all) {   // few (and no ties that top-k left among them): compared with each other
-    __syncthreads();
-    if (tid >= (int)all && tid < DIRECT) lk[tid] = 0u;
-    if constexpr (PHASE == 1) {
-      if (tid < DIRECT) hw[tid] = tid < (int)all ? r.weight(lk[tid]) >> g.coarse : 0;
+  const unsigned lo = st.lo, hi = st.hi;
+  const bool tied = PHASE == 1 && kc.cut != 0u && kc.ties != 0u && kc.cut >= lo && kc.cut <= hi;   // ties that top-k left are among them
+  if (listed && n <= DIRECT && !tied) {
+    if (tid < DIRECT) {
+      const unsigned k = tid < (int)n ? list[tid] : 0u;
+      near_k[tid] = k;
+      if constexpr (PHASE == 1) near_w[tid] = k ? r.weight(k) >> g.coarse : 0;
     }
     __syncthreads();
-    if constexpr (PHASE == 0) direct_k(lk, (int)all, &st, &cut);
-    else direct_p(lk, hw, (int)all, &st, &cut);
+    if constexpr (PHASE == 0) direct_k(near_k, (int)n, &st, &cut);
+    else direct_p(near_k, near_w, (int)n, &st, &cut);
     if (tid == 0) st.done = 1u;
     __syncthreads();
   }
+  const int rounds = a.type == UR_F32 ? 3 : 2;
   for (int round = 0; round < rounds && !st.done; ++round) {
-    for (int i = tid; i < SB; i += 256) {
+    for (int i = tid; i < SB; i += NT) {
       hc[i] = 0u;
       if (PHASE == 1) hw[i] = 0;
     }
@@ -842,21 +887,31 @@ __global__ __launch_bounds__(256) void sample_near_kernel(SampleArgs a, SampleLo
     const unsigned prefix = st.prefix;
     auto count = [&](unsigned k, unsigned times) {
       if (!round_in(k, round, prefix)) return;
-      const int d = bin_at<256>(round_place(k, round));
+      const int d = bin_at<NT>(round_place(k, round));
       atomicAdd(&hc[d], times);
       if constexpr (PHASE == 1) atomicAdd(&hw[d], (r.weight(k) >> g.coarse) * times);
     };
-    for (unsigned i = tid; i < all; i += 256) count(lk[i], 1u);
-    if (PHASE == 1 && tid == 0 && kc.cut != 0u && kc.ties != 0u && steps.of(kc.cut) == step) count(kc.cut, kc.ties);
+    if (listed) {
+      for (unsigned i = tid; i < n; i += NT) count(list[i], 1u);
+    } else {
+      const long long base = (long long)b * a.ld;
+      const unsigned from = PHASE == 0 ? lo : max(lo, kc.cut + 1u);
+      const bool wide = sample_wide(a, base);
+      for (long long i = 4 * tid; i < a.N; i += 4 * NT) {
+        const Four v = sample_four(a, base, i, a.N, wide);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (v.k[j] >= from && v.k[j] <= hi) count(v.k[j], 1u);
+      }
+    }
+    if (tied && tid == 0) count(kc.cut, kc.ties);
     __syncthreads();
-    if constexpr (PHASE == 0) pick_k<256>(round, round == rounds - 1, hc, &st, &cut, tmp32);
-    else pick_p<256>(round, round == rounds - 1, hc, hw, r.p, &st, &cut, tmp64);
+    if constexpr (PHASE == 0) pick_k<NT>(round, round == rounds - 1, hc, &st, &cut, tmp32);
+    else pick_p<NT>(round, round == rounds - 1, hc, hw, r.p, &st, &cut, tmp64);
   }
   if (tid == 0) {
-    S->st = st;
     S->cut = cut;
     if (PHASE == 0) S->kcut = cut;
-    S->arrived = 0u;
   }
 }
 __device__ __forceinline__ SampleCut final_cut(const SampleState* S, const SampleRow& r) {
@@ -871,7 +926,7 @@ __global__ __launch_bounds__(256) void sample_ties_kernel(SampleArgs a, SampleLo
   const SampleCut c = final_cut(g.state + b, r);
   if (!some_ties(c)) return;
   const long long base = (long long)b * a.ld;
-  for (int q = blockIdx.x * (LCH / LBLK) + wave; q < min(g.nblk, (int)(blockIdx.x + 1) * (LCH / LBLK)); q += 4) {
+  for (int q = blockIdx.x * (g.chunk / LBLK) + wave; q < min(g.nblk, (int)(blockIdx.x + 1) * (g.chunk / LBLK)); q += 4) {
     const long long i0 = (long long)q * LBLK, i1 = min(a.N, i0 + LBLK);
     const bool wide = sample_wide(a, base + i0);
     unsigned n = 0;
@@ -901,14 +956,18 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(SampleArgs a, SampleLo
   const SampleCut c = final_cut(S, r);
   const bool ranked = some_ties(c);
   const long long base = (long long)b * a.ld;
-  for (int q = blockIdx.x * (LCH / LBLK) + wave; q < min(g.nblk, (int)(blockIdx.x + 1) * (LCH / LBLK)); q += 4) {
+  for (int q = blockIdx.x * (g.chunk / LBLK) + wave; q < min(g.nblk, (int)(blockIdx.x + 1) * (g.chunk / LBLK)); q += 4) {
     const long long i0 = (long long)q * LBLK, i1 = min(a.N, i0 + LBLK);
     const bool wide = sample_wide(a, base + i0);
     unsigned ties = ranked ? ties_before(g.tb + (long long)b * g.nblk, q) : 0u;
     WSum v{0, 0};
-#pragma unroll 2
+    Four next[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) next[u] = sample_four(a, base, i0 + 256 * u + 4 * lane, i1, wide);
+#pragma unroll
     for (int j = 0; j < LBLK / 256; ++j) {
-      const Four f = sample_four(a, base, i0 + 256 * j + 4 * lane, i1, wide);
+      const Four f = next[j & 3];
+      if (j + 4 < LBLK / 256) next[j & 3] = sample_four(a, base, i0 + 256 * (j + 4) + 4 * lane, i1, wide);
       unsigned rank = 0;
       if (ranked) {
         unsigned eq = 0;
@@ -1026,7 +1085,10 @@ static size_t sample_long_bytes(long long N, int B, char* base, SampleLong* g) {
     return p;
   };
   SampleLong w{};
-  w.nchunk = cdiv(N, LCH); w.nblk = cdiv(N, LBLK); w.coarse = log2_up(N);
+  // about 2 048 workgroups where there is work for them, of 4 096 to 65 536 entries
+  const long long want = (N * (long long)B + 2047) / 2048;
+  w.chunk = (int)std::min<long long>(65536, std::max<long long>(4096, (want + 4095) / 4096 * 4096));
+  w.nchunk = cdiv(N, w.chunk); w.nblk = cdiv(N, LBLK); w.coarse = log2_up(N);
   w.state = (SampleState*)take(sizeof(SampleState) * B);
   w.hc = (unsigned*)take((size_t)B * SB * 4); w.hw = (u64*)take((size_t)B * SB * 8);
   w.tb = (unsigned*)take((size_t)B * w.nblk * 4); w.bs = (u64*)take((size_t)B * w.nblk * 16);
@@ -1089,17 +1151,14 @@ extern "C" int ur_sample_scores(const void* scores, int32_t score_type, int64_t 
   UR_LAUNCH_CHECK();
   hipLaunchKernelGGL(sample_max_kernel, grid, dim3(256), 0, st, a, g);
   UR_LAUNCH_CHECK();
-  const int rounds = score_type == UR_F32 ? 3 : 2;
   auto select = [&](auto phase) -> int {
     constexpr int PHASE = decltype(phase)::value;
-    for (int round = -1; round < rounds; ++round) {
-      hipLaunchKernelGGL((sample_round_kernel<PHASE>), grid, dim3(256), 0, st, a, g, round, mode);
-      UR_LAUNCH_CHECK();
-      if (round < 0) {
-        hipLaunchKernelGGL((sample_near_kernel<PHASE>), grid, dim3(256), 0, st, a, g, mode);
-        UR_LAUNCH_CHECK();
-      }
-    }
+    hipLaunchKernelGGL((sample_steps_kernel<PHASE>), grid, dim3(256), 0, st, a, g, mode);
+    UR_LAUNCH_CHECK();
+    hipLaunchKernelGGL((sample_near_kernel<PHASE>), grid, dim3(256), 0, st, a, g);
+    UR_LAUNCH_CHECK();
+    hipLaunchKernelGGL((sample_border_kernel<PHASE>), dim3(B), dim3(1024), 0, st, a, g);
+    UR_LAUNCH_CHECK();
     return UR_OK;
   };
   int rc = g.uses_k ? select(std::integral_constant<int, 0>()) : UR_OK;
