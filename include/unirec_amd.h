@@ -770,7 +770,7 @@ int ur_full_distill_bwd(const float* user_emb, const float* item_table, int64_t 
  * temperature = 0: the lowest index among the largest.  *_rows (nullable): per-row values [B] in the place of the scalar (a top_p <= 0 keeps
  * the first entry, a temperature that is not positive is 0, a min_p that is not below 1 is 1, a top_k <= 0 is off).
  * out_id[B,S] = ids[b * ld_ids + index] (ids nullable: the index itself), out_logp[B,S] = log of the drawn entry's probability among the kept;
- * a row without an entry: -1, -inf.  Weights are double, rounded down once to multiples of 2^-62 and summed as integers: no result depends on an
+ * a row without an entry: -1, -inf.  Weights are double, rounded down once to multiples of 2^-57 and summed as integers: no result depends on an
  * order of additions.  n < 2^31.
  * ws: ur_sample_scores_workspace_bytes (0: rows that fit into a workgroup's LDS need none, ws may be NULL). */
 int64_t ur_sample_scores_workspace_bytes(int32_t score_type, int64_t n, int32_t B);

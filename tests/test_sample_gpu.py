@@ -137,6 +137,26 @@ def test_ties_stay_in_index_order(N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("N", [60, 5000, 40_000, 70_001])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_a_border_right_below_zero(N, dtype):
+    """zeros of both signs are one tie, and all of them stay where the border lies below them"""
+    g = torch.Generator().manual_seed(N)
+    kind = torch.randint(0, 4, (2, N), generator=g)
+    x = torch.tensor([1.0, 0.0, -0.0, -0.5]).to(getattr(torch, dtype))[kind]
+    u = torch.rand(2, 40, generator=g)
+    kept = (kind < 3).sum(1).to(torch.int32)
+    _check(x, u, T=0.7, k=kept)
+    _check(x, u, T=0.7, k=kept, p=0.999)                         # (the last of the zeros go)
+    one, rest = (kind == 0).sum(1).double(), (kind == 3).sum(1).double()
+    zero = N - one - rest
+    w = [math.exp(-1 / 0.7), math.exp(-1.5 / 0.7)]
+    p = (one + w[0] * zero + 0.3 * w[1]) / (one + w[0] * zero + w[1] * rest)
+    _check(x, u, T=0.7, p=float(p[0]), m=0.0)
+    _check(x, u, T=0.7, m=0.2)                                   # exp(-1 / 0.7) = 0.24 stays, exp(-1.5 / 0.7) = 0.12 goes
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("N", [40, 3000, 50_000])
 def test_infinities_nan_and_empty_rows(N):
     x, u = _scores(9, N, 3, masked=0.0)

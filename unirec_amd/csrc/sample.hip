@@ -4,17 +4,18 @@
 //   top-k: the first k in the order (score descending, index ascending); top-p: of those, in that order, every entry before which less
 //   than p of their weight lies; min-p: w >= min_p.  The answer to u: the first index n, in INDEX order, with sum_{j <= n} kept w_j > u W.
 // No sort: the order only decides a threshold (a key and how many of its ties stay).  It is found by a histogram over 2 048 equal steps of
-// the score (steps of the key's upper bits put most scores into a few dozen bins, whose LDS atomics then queue: 190 us against 75 us for
-// 64 rows of a million), and inside the step that the border falls into by comparing up to 128 keys directly, or by radix selection over
-// 11, 11 and 10 bits of the key.
+// the score (steps of the key's upper bits put most scores into a few dozen bins, whose LDS atomics then queue: with those the whole call
+// took 756 us for 64 rows of a million with top-p, 587 us with these and the comparison), and inside the step that the border falls into by
+// comparing up to 128 keys directly, or by radix selection over 11, 11 and 10 bits of the key.
 //
-// Arithmetic.  Which entry a sum's border falls on is a whole number, so sums are exact: a weight is exp in double (2 10^-16), rounded down
-// once to a multiple of 2^-62 and added as integers, in two 32-bit limbs summed in 64 bits each (the top-p selection sums multiples of
-// 2^-(62 - log2 N) in one).  No result depends on an order of additions or on how a row was cut into pieces.
+// Arithmetic.  Which entry a sum's border falls on is a whole number, so sums are exact: a weight is exp in double, rounded down
+// once to a multiple of 2^-57 (2^-53 is a double's own step) and added as integers: 64 of them in 64 bits, more in two 32-bit limbs (the
+// top-p selection sums multiples of 2^-(63 - log2 N) in 64 bits).  No result depends on an order of additions or on how a row was cut into pieces.
 //
 // Two forms.  A row that fits into LDS (32 768 entries; 65 536 of 16 bits): one workgroup, one read of the row, every pass from LDS.
 // Longer rows: many workgroups a row, a pass over memory each for the maximum, for a selection's histogram and its border's step, and for the
-// kept sums.
+// kept sums.  Bound: short rows by the latency of the passes (1 x 1 000: 16 us, 512 x 1 000: 16 us), long rows with top-p by vector
+// instructions, some 60 an entry for a weight and its place (64 x 1 M fp32: 369 us, without selections 169 us).
 #include <math.h>
 
 #include <algorithm>
@@ -54,36 +55,47 @@ __device__ __forceinline__ float key_value(unsigned key, int type) {
   const unsigned k = key >> 16, u = (k & 0x8000u) ? (k & 0x7FFFu) : (~k & 0xFFFFu);
   return type == UR_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)u) : __uint_as_float(u << 16);
 }
+// a score x (a number) lies above it where x's key lies above `key`; NaN or -inf: every number does.  The place of -0, which no entry
+// has, is read as the number below it: 0 > -0 is false
+__device__ __forceinline__ float cut_value(unsigned key, int type) {
+  const unsigned low = type == UR_F32 ? 0x7FFFFFFFu : 0x7FFF0000u, mask = type == UR_F32 ? 0xFFFFFFFFu : 0xFFFF0000u;
+  const float v = key_value((key & mask) == low ? (type == UR_F32 ? low - 1u : low - 0x10000u) : key, type);
+  return v == v ? v : -INFINITY;
+}
 __device__ __forceinline__ unsigned sample_key(const void* p, int type, long long i) {
   return type == UR_F32 ? key_f32(((const float*)p)[i]) : key_16(((const unsigned short*)p)[i], type);
 }
 
-// exp(z) 2^62, rounded down, z <= 0.  r = z - n ln 2 in two pieces, |r| <= ln 2 / 2, the Taylor polynomial of degree 12 (remainder 2 10^-16)
-__device__ __forceinline__ u64 exp_fixed(double z) {
-  if (!(z > -43.0)) return 0;                                    // below 2^-62
-  const double n = rint(z * 1.4426950408889634);
-  constexpr double LN2_HI = 2977044471.0 / 4294967296.0;         // the first 32 bits of ln 2 (n LN2_HI is exact), and the rest
-  const double r = fma(n, -1.9082149292705877e-10, fma(n, -LN2_HI, z));
-  double p = 1.0 / 479001600.0;
-  p = fma(p, r, 1.0 / 39916800.0);
-  p = fma(p, r, 1.0 / 3628800.0);
-  p = fma(p, r, 1.0 / 362880.0);
-  p = fma(p, r, 1.0 / 40320.0);
-  p = fma(p, r, 1.0 / 5040.0);
-  p = fma(p, r, 1.0 / 720.0);
-  p = fma(p, r, 1.0 / 120.0);
-  p = fma(p, r, 1.0 / 24.0);
-  p = fma(p, r, 1.0 / 6.0);
-  p = fma(p, r, 0.5);
+// 2^(z + 57), rounded down, z <= 0.  r = z - n in [-1/2, 1/2] (exact; n by adding 1.5 2^52), the Taylor polynomial of 2^r of degree 11
+// (remainder 6 10^-15 of it, of the order of the rounding of z itself), 2^n and the fixed point by shifting the result's mantissa
+constexpr int WBITS = 57;
+__device__ __forceinline__ u64 exp2_fixed(double z) {
+  constexpr double L = 0.69314718055994530942, MAGIC = 6755399441055744.0;
+  constexpr double c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5, c6 = c5 * L / 6, c7 = c6 * L / 7, c8 = c7 * L / 8,
+                   c9 = c8 * L / 9, c10 = c9 * L / 10, c11 = c10 * L / 11;
+  z = fmax(z, -100.0);
+  const double t = z + MAGIC;
+  const int n = (int)(unsigned)__double_as_longlong(t);
+  const double r = z - (t - MAGIC);
+  double p = fma(c11, r, c10);
+  p = fma(p, r, c9);
+  p = fma(p, r, c8);
+  p = fma(p, r, c7);
+  p = fma(p, r, c6);
+  p = fma(p, r, c5);
+  p = fma(p, r, c4);
+  p = fma(p, r, c3);
+  p = fma(p, r, c2);
+  p = fma(p, r, L);
   p = fma(p, r, 1.0);
-  p = fma(p, r, 1.0);
-  const double v = ldexp(p, (int)n + 30);                        // <= 2^30 (z <= 0: p 2^n <= 1 up to its rounding)
-  const unsigned hi = (unsigned)v;
-  return ((u64)hi << 32) + (unsigned)((v - (double)hi) * 4294967296.0);
+  const unsigned hi = (unsigned)((u64)__double_as_longlong(p) >> 32), lo = (unsigned)__double_as_longlong(p);   // p in [0.7, 1.5)
+  const unsigned down = min(1023u - (hi >> 20) - (unsigned)n, 63u);                                             // 0 for z = 0; 63: nothing is left
+  const u64 mant = ((u64)((hi & 0xFFFFFu) | 0x100000u) << 32) | lo;
+  return (mant << (WBITS - 52)) >> down;
 }
 // a row's parameters
 struct SampleRow {
-  double inv_T, p, min_z; long long k; int type; bool greedy, flat;
+  double scale, inv_T, p, min_z; long long k; int type; bool greedy, flat;   // scale: log2(e) / T
   float m;
   __device__ __forceinline__ void load(const SampleArgs& a, int b) {
     const double T = a.T_rows ? (double)a.T_rows[b] : a.T;
@@ -94,8 +106,9 @@ struct SampleRow {
     if (k <= 0) k = a.N;
     greedy = !(T > 1e-300);              // (1 / T stays finite)
     inv_T = greedy ? 1.0 : 1.0 / T;
+    scale = greedy ? 1.0 : 1.4426950408889634 / T;
     if (!(min_p < 1.0)) min_p = 1.0;     // (the largest stays)
-    min_z = min_p > 0.0 ? log(min_p) : -INFINITY;
+    min_z = min_p > 0.0 ? log2(min_p) : -INFINITY;
   }
   __device__ __forceinline__ void set_max(unsigned key) { m = key_value(key, type); flat = greedy || m == INFINITY; }
   __device__ __forceinline__ double z(unsigned key) const {
@@ -103,16 +116,37 @@ struct SampleRow {
     if (flat) return x == m ? 0.0 : -INFINITY;
     return ((double)x - (double)m) * inv_T;
   }
-  __device__ __forceinline__ u64 weight(unsigned key) const { return exp_fixed(z(key)); }
-  // of an entry that the selections leave: 0 if min-p takes it
-  __device__ __forceinline__ u64 kept(unsigned key) const {
-    const double v = z(key);
-    return v >= min_z ? exp_fixed(v) : 0;
+  __device__ __forceinline__ double z2(unsigned key) const {     // log2 of the weight
+    const float x = key_value(key, type);
+    if (flat) return x == m ? 0.0 : -INFINITY;
+    return ((double)x - (double)m) * scale;
+  }
+  __device__ __forceinline__ u64 weight(unsigned key) const { return exp2_fixed(z2(key)); }
+  // the smallest key that min-p leaves, searched by a wave, 64 keys at a time
+  __device__ __forceinline__ unsigned min_key(unsigned mk) const {
+    if (!(min_z > -INFINITY)) return 1u;
+    const unsigned lane = threadIdx.x & 63;
+    unsigned lo = 1u, hi = mk;
+    while (lo < hi) {
+      const unsigned probe = lo + (unsigned)(((u64)(hi - lo) * lane) >> 6);
+      const u64 in = __ballot(z2(probe) >= min_z);
+      if (in == 0ull) {
+        lo = (unsigned)__builtin_amdgcn_readlane((int)probe, 63) + 1u;
+      } else {
+        const int f = __builtin_amdgcn_readfirstlane(__ffsll(in) - 1);
+        hi = (unsigned)__builtin_amdgcn_readlane((int)probe, f);
+        if (f > 0) lo = (unsigned)__builtin_amdgcn_readlane((int)probe, f - 1) + 1u;
+      }
+    }
+    return hi;
   }
 };
 // entries above `cut` stay, and of those equal to it the first `ties` in index order
 struct SampleCut { unsigned cut; unsigned ties; };
 constexpr unsigned ALL_TIES = 0xFFFFFFFFu;
+__device__ __forceinline__ SampleCut above_min_p(SampleCut c, unsigned min_key) {   // and what min-p leaves of them
+  return min_key > 1u && min_key > c.cut ? SampleCut{min_key - 1u, 0u} : c;
+}
 
 struct WSum {   // a sum of weights
   u64 hi, lo;
@@ -191,7 +225,7 @@ __device__ __forceinline__ unsigned ties_within(u64 above, u64 w, double limit, 
 }
 
 // ---- a selection: a histogram over equal steps of the score (round -1), then rounds over the bits of the keys of one step
-constexpr int SB = 2048;
+constexpr int SB = 2048, SBP = SB + 8;   // bins; their room in LDS
 struct Steps {   // step of a score: (max / 2 - x / 2) c, never larger for a larger score (fp32 rounding keeps an order); halves: no difference overflows
   float half_m, c; float m; int type; bool flat;
   __device__ __forceinline__ void set(const SampleRow& r, unsigned minkey, bool weights) {
@@ -201,8 +235,8 @@ struct Steps {   // step of a score: (max / 2 - x / 2) c, never larger for a lar
     if (weights) range = fmin(range, 21.5 / r.inv_T);            // (steps behind 43 T weigh nothing: one bin)
     c = range > 0.0 ? (float)fmin((double)SB / range, 1e38) : 0.f;
   }
-  __device__ __forceinline__ int of(unsigned key) const {
-    const float x = key_value(key, type);
+  __device__ __forceinline__ int of(unsigned key) const { return of_value(key_value(key, type)); }
+  __device__ __forceinline__ int of_value(float x) const {
     if (flat) return x == m ? 0 : SB - 1;
     const float t = fmaf(x, -0.5f, half_m) * c;
     return t < (float)(SB - 1) ? (int)t : SB - 1;                // (a pattern that is no number: the last)
@@ -243,11 +277,12 @@ struct Select {   // state of a selection (one per row)
   u64 above; double limit;              // top-p: the weight in front of them, p times all of it
   unsigned done;
 };
-// bins lie in the order of the threads that sum them: thread t of NT takes places t SB / NT .. , each at j NT + t
+// bins lie in the order of the threads that sum them: thread t of NT takes places t SB / NT .. , place j of them at j (NT + 1) + t (a bank apart:
+// scores next to each other fall into places next to each other)
 template <int NT>
 __device__ __forceinline__ int bin_at(int place) {
   constexpr int PB = SB / NT;
-  return (place % PB) * NT + place / PB;
+  return (place % PB) * (NT + 1) + place / PB;
 }
 // the place that the border falls into, found by the whole workgroup; updates st, sets cut when it is final.
 // `last`: no key of this type has bits below this round's
@@ -257,7 +292,7 @@ __device__ __forceinline__ void pick_k(int round, bool last, const unsigned* hc,
   const unsigned need = st->need, prefix = st->prefix;
   unsigned mine[PB], sum = 0, total;
 #pragma unroll
-  for (int j = 0; j < PB; ++j) { mine[j] = hc[j * NT + threadIdx.x]; sum += mine[j]; }
+  for (int j = 0; j < PB; ++j) { mine[j] = hc[j * (NT + 1) + threadIdx.x]; sum += mine[j]; }
   unsigned before = block_before<NT>(sum, tmp, &total);
   if (before < need && need <= before + sum) {
 #pragma unroll
@@ -294,7 +329,7 @@ __device__ __forceinline__ void pick_p(int round, bool last, const unsigned* hc,
   const double given = st->limit;
   u64 mine[PB], sum = 0, total;
 #pragma unroll
-  for (int j = 0; j < PB; ++j) { mine[j] = hw[j * NT + threadIdx.x]; sum += mine[j]; }
+  for (int j = 0; j < PB; ++j) { mine[j] = hw[j * (NT + 1) + threadIdx.x]; sum += mine[j]; }
   u64 before = block_before<NT>(sum, tmp, &total) + above;
   const double limit = round < 0 ? p * (double)total : given;
   // the first entry of exactly one bin is the last whose forerunners weigh less than the limit
@@ -303,12 +338,11 @@ __device__ __forceinline__ void pick_p(int round, bool last, const unsigned* hc,
     for (int j = 0; j < PB; ++j) {
       if ((double)before < limit && !((double)(before + mine[j]) < limit)) {
         const int place = (int)threadIdx.x * PB + j;
-        const unsigned n = hc[j * NT + threadIdx.x];
         st->above = before;
         st->limit = limit;
-        st->count = n;
         if (round < 0) st->step = place;
         else {
+          const unsigned n = hc[j * (NT + 1) + threadIdx.x];
           const unsigned q = round_prefix(prefix, round, place);
           st->prefix = q;
           if (last) {
@@ -389,9 +423,9 @@ template <int NT, bool RAW>
 __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int NWV = NT / 64, LAST = RAW ? 1 : 2;
-  u64* hw = (u64*)smem;                                          // [SB]; the copied entries on their way
-  unsigned* hc = (unsigned*)(hw + SB);                           // [SB]
-  unsigned* keys = hc + SB;                                      // [N] (RAW: 16 bits each); then the copied entries, keys and indices
+  u64* hw = (u64*)smem;                                          // [SBP]; the copied entries on their way
+  unsigned* hc = (unsigned*)(hw + SBP);                          // [SBP]
+  unsigned* keys = hc + SBP;                                     // [N] (RAW: 16 bits each); then the copied entries, keys and indices
   unsigned short* keys16 = (unsigned short*)keys;
   __shared__ u64 tmp64[NWV];
   __shared__ unsigned tmp32[NWV], s_min[NWV], s_n;
@@ -481,7 +515,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
       if (tid == 0) { st = Select{0, 0u, 0u, 0u, 0u, (unsigned)r.k, 0, 0.0, 0u}; cut_s = c; s_n = 0u; }
       if (tid < DIRECT) near_k[tid] = 0u;
       for (int round = -1; round <= LAST; ++round) {
-        for (int i = tid; i < SB; i += NT) hc[i] = 0u;
+        for (int i = tid; i < SBP; i += NT) hc[i] = 0u;
         __syncthreads();
         const unsigned prefix = st.prefix, lo = st.lo, hi = st.hi;
         if (round < 0) {
@@ -541,14 +575,29 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
       if (tid == 0) { st = Select{0, 1u, mk, 0u, 0u, 0u, 0, 0.0, 0u}; cut_s = SampleCut{mk, 1u}; s_n = 0u; }   // (p <= 0: the largest alone)
       if (tid < DIRECT) { near_k[tid] = 0u; near_w[tid] = 0; }
       const bool few = n <= DIRECT && copied;                    // no histogram: all of them are compared
+      auto gather = [&]() {                                      // the keys of the border's step (few: all), as many as can be compared
+        const unsigned lo = st.lo, hi = st.hi;
+        auto add = [&](unsigned k) {
+          const unsigned q = atomicAdd(&s_n, 1u);
+          if (q < DIRECT) { near_k[q] = k; near_w[q] = r.weight(k) >> coarse; }
+        };
+        for (int i = tid; i < n; i += NT) {
+          const unsigned k = key_at(i);
+          if (k > c.cut && k >= lo && k <= hi) add(k);
+        }
+        if (tid == 0 && c.cut != 0u && c.ties != 0u && c.cut >= lo && c.cut <= hi)
+          for (unsigned t = 0; t < min(c.ties, (unsigned)DIRECT + 1u); ++t) add(c.cut);
+        __syncthreads();
+      };
+      if (few) __syncthreads();                                  // (st)
       for (int round = few ? LAST + 1 : -1; round <= LAST && r.p > 0.0; ++round) {
-        for (int i = tid; i < SB; i += NT) { hc[i] = 0u; hw[i] = 0; }
+        for (int i = tid; i < SBP; i += NT) { hc[i] = 0u; hw[i] = 0; }
         __syncthreads();
         const unsigned prefix = st.prefix, lo = st.lo, hi = st.hi;
         auto count = [&](unsigned k, unsigned times) {
           if (round >= 0 && !(k >= lo && k <= hi && round_in(k, round, prefix))) return;
           const int d = bin_at<NT>(round < 0 ? steps.of(k) : round_place(k, round));
-          atomicAdd(&hc[d], times);
+          if (round >= 0) atomicAdd(&hc[d], times);
           atomicAdd(&hw[d], (r.weight(k) >> coarse) * times);
         };
         for (int i = tid; i < n; i += NT) {
@@ -558,48 +607,45 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
         if (tid == 0 && c.cut != 0u && c.ties != 0u) count(c.cut, c.ties);   // the ties that top-k left
         __syncthreads();
         pick_p<NT>(round, round == LAST, hc, hw, r.p, &st, &cut_s, tmp64);
-        if (round < 0) step_keys(steps, mk, &st);
-        if (st.done || (round < 0 && st.count <= DIRECT)) break;
+        if (round < 0) {
+          step_keys(steps, mk, &st);
+          gather();
+          if (s_n <= DIRECT) break;
+        }
+        if (st.done) break;
       }
+      if (few) gather();
       __syncthreads();
       if (r.p > 0.0 && !st.done) {
-        const unsigned lo = st.lo, hi = st.hi;                   // (few: all keys)
-        auto add = [&](unsigned k) {
-          const unsigned q = atomicAdd(&s_n, 1u);
-          near_k[q] = k;
-          near_w[q] = r.weight(k) >> coarse;
-        };
-        for (int i = tid; i < n; i += NT) {
-          const unsigned k = key_at(i);
-          if (k > c.cut && k >= lo && k <= hi) add(k);
-        }
-        if (tid == 0 && c.cut != 0u && c.ties != 0u && c.cut >= lo && c.cut <= hi)
-          for (unsigned t = 0; t < c.ties; ++t) add(c.cut);
-        __syncthreads();
         if (few) {                                               // the limit: p times all of it
           u64 total;
           block_before<NT>(tid < DIRECT ? near_w[tid] : 0, tmp64, &total);
-          if (tid == 0) { st.limit = r.p * (double)total; st.count = s_n; }
+          if (tid == 0) st.limit = r.p * (double)total;
           __syncthreads();
         }
-        direct_p(near_k, near_w, (int)st.count, &st, &cut_s);
+        direct_p(near_k, near_w, (int)s_n, &st, &cut_s);
       }
       c = cut_s;
       __syncthreads();
     }
   }
+  c = above_min_p(c, r.min_key(mk));
   // ---- the kept weight in front of every thread's entries
   const int C = span(), i0 = min(n, tid * C), i1 = min(n, i0 + C);
   const unsigned rank0 = ranked() ? in_front(i0, i1) : 0u;
   unsigned rank = rank0;
   WSum mine{0, 0}, all;
-  for (int i = i0; i < i1; ++i) {
-    const unsigned k = key_at(i);
-    if (stays(k, rank)) mine.add(r.kept(k));
+  {
+    u64 sum = 0;                        // (at most 65 entries of at most 2^57)
+    for (int i = i0; i < i1; ++i) {
+      const unsigned k = key_at(i);
+      if (stays(k, rank)) sum += r.weight(k);
+    }
+    mine.add(sum);
   }
   const WSum front = block_before<NT>(mine, tmp64, &all);
   const u128 W = all.all();
-  const double log_W = log(wide_to_double(W) * 2.168404344971009e-19);   // 2^-62
+  const double log_W = log(wide_to_double(W) * 6.938893903907228e-18);   // 2^-57
   u64* from_hi = hw;                                             // [NT] (the histograms are done with): what lies in front of a thread's entries
   u64* from_lo = hw + NT;                                        // [NT]
   unsigned* ranks = hc;                                          // [NT]
@@ -635,7 +681,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
         unsigned my_rank = ties + (unsigned)__popcll(eq & ((1ull << lane) - 1ull));
         ties += (unsigned)__popcll(eq);
         WSum v{0, 0};
-        if (stays(k, my_rank)) v.add(r.kept(k));
+        if (stays(k, my_rank)) v.add(r.weight(k));
         const WSum up{wave_upto(v.hi), wave_upto(v.lo)};
         const u64 over = __ballot(run + up.all() > goal);
         if (over) {
@@ -662,7 +708,7 @@ struct SampleState {                      // per row, in the workspace
 };
 constexpr int LLIST = 8192;                   // a row's list
 struct SampleLong {
-  SampleState* state; unsigned* hc; u64* hw;   // [B], [B][SB], [B][SB]
+  SampleState* state; unsigned* hc; u64* hw;   // [B], [B][SBP], [B][SBP]
   unsigned* tb; u64* bs;                       // [B][nblk] ties of a block, [B][2 nblk] kept weight of a block
   unsigned* list;                              // [B][LLIST] keys of the border's step
   int nblk, nchunk, coarse;
@@ -672,7 +718,7 @@ struct SampleLong {
 
 __global__ __launch_bounds__(256) void sample_init_kernel(SampleArgs a, SampleLong g) {
   const int b = blockIdx.x;
-  for (int i = threadIdx.x; i < SB; i += 256) { g.hc[(long long)b * SB + i] = 0u; g.hw[(long long)b * SB + i] = 0; }
+  for (int i = threadIdx.x; i < SBP; i += 256) { g.hc[(long long)b * SBP + i] = 0u; g.hw[(long long)b * SBP + i] = 0; }
   if (threadIdx.x == 0) {
     SampleState s{};
     s.cut = s.kcut = SampleCut{0u, ALL_TIES};
@@ -743,12 +789,35 @@ template <int PHASE>
 __device__ __forceinline__ bool sample_active(const SampleArgs& a, const SampleRow& r, unsigned mk) {
   return mk != 0u && !r.greedy && (PHASE == 0 ? r.k < a.N : r.p < 1.0 && r.p > 0.0);
 }
+// four consecutive scores as floats; behind the end: -inf
+struct FourX { float x[4]; };
+template <int TYPE>
+__device__ __forceinline__ FourX four_scores(const SampleArgs& a, long long base, long long i, long long end, bool wide) {
+  FourX r;
+  auto narrow = [](unsigned u) { return TYPE == UR_F16 ? (float)__builtin_bit_cast(_Float16, (unsigned short)u) : __uint_as_float(u << 16); };
+  if (wide && i + 4 <= end) {
+    if constexpr (TYPE == UR_F32) {
+      const float4 v = *(const float4*)((const float*)a.scores + base + i);
+      r.x[0] = v.x; r.x[1] = v.y; r.x[2] = v.z; r.x[3] = v.w;
+    } else {
+      const ushort4 v = *(const ushort4*)((const unsigned short*)a.scores + base + i);
+      r.x[0] = narrow(v.x); r.x[1] = narrow(v.y); r.x[2] = narrow(v.z); r.x[3] = narrow(v.w);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      r.x[j] = -INFINITY;
+      if (i + j < end) r.x[j] = TYPE == UR_F32 ? ((const float*)a.scores)[base + i + j] : narrow(((const unsigned short*)a.scores)[base + i + j]);
+    }
+  }
+  return r;
+}
 // the top-k (PHASE 0) or top-p (PHASE 1) selection: counts (and weights) of the steps; the workgroup that arrives last finds the border's step
 // and clears the bins
-template <int PHASE>
+template <int PHASE, int TYPE>
 __global__ __launch_bounds__(256) void sample_steps_kernel(SampleArgs a, SampleLong g, int mode) {
-  __shared__ unsigned hc[SB];
-  __shared__ u64 hw[PHASE == 1 ? SB : 1];
+  __shared__ unsigned hc[PHASE == 0 ? SBP : 1];
+  __shared__ u64 hw[PHASE == 1 ? SBP : 1];
   __shared__ unsigned tmp32[4], last;
   __shared__ u64 tmp64[4];
   __shared__ Select st;
@@ -766,30 +835,51 @@ __global__ __launch_bounds__(256) void sample_steps_kernel(SampleArgs a, SampleL
   r.set_max(mk);
   Steps steps;
   steps.set(r, S->minkey, PHASE == 1);
-  unsigned* ghc = g.hc + (long long)b * SB;
-  u64* ghw = g.hw + (long long)b * SB;
+  unsigned* ghc = g.hc + (long long)b * SBP;
+  u64* ghw = g.hw + (long long)b * SBP;
   const SampleCut kc = S->kcut;
-  for (int i = tid; i < SB; i += 256) {
-    hc[i] = 0u;
-    if (PHASE == 1) hw[i] = 0;
+  for (int i = tid; i < SBP; i += 256) {
+    if constexpr (PHASE == 0) hc[i] = 0u;
+    else hw[i] = 0;
   }
   __syncthreads();
   const long long i0 = (long long)blockIdx.x * g.chunk, i1 = min(a.N, i0 + g.chunk);
-  auto count = [&](unsigned k, unsigned times) {
-    const int d = bin_at<256>(steps.of(k));
-    atomicAdd(&hc[d], times);
-    if constexpr (PHASE == 1) atomicAdd(&hw[d], (r.weight(k) >> g.coarse) * times);
-  };
-  sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) {
-    if (PHASE == 0 ? k != 0u : k > kc.cut) count(k, 1u);
-  });
-  if (PHASE == 1 && blockIdx.x == 0 && tid == 0 && kc.cut != 0u && kc.ties != 0u) count(kc.cut, kc.ties);
-  __syncthreads();
-  for (int i = tid; i < SB; i += 256)
-    if (hc[i]) {
-      atomicAdd(&ghc[i], hc[i]);
-      if constexpr (PHASE == 1) atomicAdd(&ghw[i], hw[i]);
+  const float above = PHASE == 1 ? cut_value(kc.cut, TYPE) : -INFINITY;
+  const double m = (double)r.m, scale = r.scale;
+  auto count = [&](float x, unsigned times) {
+    const int d = bin_at<256>(steps.of_value(x));
+    if constexpr (PHASE == 0) atomicAdd(&hc[d], times);
+    else {
+      const double z = r.flat ? (x == r.m ? 0.0 : -100.0) : ((double)x - m) * scale;
+      atomicAdd(&hw[d], (exp2_fixed(z) >> g.coarse) * times);
     }
+  };
+  {
+    const long long base = (long long)b * a.ld;
+    const bool wide = sample_wide(a, base + i0);
+    FourX v[4];
+    long long i = i0 + 4 * tid;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = four_scores<TYPE>(a, base, i + 1024 * u, i1, wide);
+    for (; i < i1; i += 4096) {
+      FourX w[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) w[u] = four_scores<TYPE>(a, base, i + 4096 + 1024 * u, i1, wide);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (v[u].x[j] > above) count(v[u].x[j], 1u);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = w[u];
+    }
+  }
+  if (PHASE == 1 && blockIdx.x == 0 && tid == 0 && kc.cut != 0u && kc.ties != 0u) count(above, kc.ties);
+  __syncthreads();
+  for (int i = tid; i < SBP; i += 256) {
+    if constexpr (PHASE == 0) { if (hc[i]) atomicAdd(&ghc[i], hc[i]); }
+    else { if (hw[i]) atomicAdd(&ghw[i], hw[i]); }
+  }
   __syncthreads();
   if (tid == 0) last = ur_arrive(&S->arrived, mode) == (unsigned)g.nchunk - 1u;
   __syncthreads();
@@ -798,15 +888,13 @@ __global__ __launch_bounds__(256) void sample_steps_kernel(SampleArgs a, SampleL
     st = Select{0, 1u, mk, 0u, 0u, (unsigned)min((long long)0x7FFFFFFF, r.k), 0, 0.0, 0u};
     cut = S->cut;
   }
-  for (int i = tid; i < SB; i += 256) {
-    hc[i] = agent_load(ghc + i);
-    if constexpr (PHASE == 1) hw[i] = agent_load(ghw + i);
-    ghc[i] = 0u;
-    if (PHASE == 1) ghw[i] = 0;
+  for (int i = tid; i < SBP; i += 256) {
+    if constexpr (PHASE == 0) { hc[i] = agent_load(ghc + i); ghc[i] = 0u; }
+    else { hw[i] = agent_load(ghw + i); ghw[i] = 0; }
   }
   __syncthreads();
   if constexpr (PHASE == 0) pick_k<256>(-1, false, hc, &st, &cut, tmp32);
-  else pick_p<256>(-1, false, hc, hw, r.p, &st, &cut, tmp64);
+  else pick_p<256>(-1, false, nullptr, hw, r.p, &st, &cut, tmp64);
   step_keys(steps, mk, &st);
   if (tid == 0) {
     S->st = st;
@@ -822,28 +910,31 @@ __global__ __launch_bounds__(256) void sample_near_kernel(SampleArgs a, SampleLo
   SampleState* S = g.state + b;
   SampleRow r;
   r.load(a, b);
-  if (!sample_active<PHASE>(a, r, S->maxkey) || S->st.done || S->st.count > LLIST) return;
+  if (!sample_active<PHASE>(a, r, S->maxkey) || S->st.done) return;
   const unsigned lo = PHASE == 0 ? S->st.lo : max(S->st.lo, S->kcut.cut + 1u), hi = S->st.hi;
   if (tid == 0) n_s = 0u;
   __syncthreads();
   const long long i0 = (long long)blockIdx.x * g.chunk, i1 = min(a.N, i0 + g.chunk);
   sample_walk(a, (long long)b * a.ld, i0, i1, [&](unsigned k) {
-    if (k >= lo && k <= hi) lk[atomicAdd(&n_s, 1u)] = k;         // (at most st.count of them)
+    if (k >= lo && k <= hi) {
+      const unsigned q = atomicAdd(&n_s, 1u);
+      if (q < LLIST) lk[q] = k;
+    }
   });
   __syncthreads();
   const unsigned n = n_s;
   if (n == 0u) return;
   if (tid == 0) at_s = atomicAdd(&S->listed, n);
   __syncthreads();
-  unsigned* list = g.list + (long long)b * LLIST + at_s;
-  for (unsigned i = tid; i < n; i += 256) list[i] = lk[i];
+  unsigned* list = g.list + (long long)b * LLIST;
+  for (unsigned i = tid; at_s + i < LLIST && i < n; i += 256) list[at_s + i] = lk[i];   // (more than the list holds: counted only)
 }
 // the border among them: compared directly, or radix rounds over the list (over the row where the list could not hold them)
 template <int PHASE>
 __global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, SampleLong g) {
   constexpr int NT = 1024;
-  __shared__ unsigned hc[SB];
-  __shared__ u64 hw[PHASE == 1 ? SB : 1];
+  __shared__ unsigned hc[SBP];
+  __shared__ u64 hw[PHASE == 1 ? SBP : 1];
   __shared__ __attribute__((aligned(16))) unsigned near_k[DIRECT];
   __shared__ u64 near_w[PHASE == 1 ? DIRECT : 1];
   __shared__ unsigned tmp32[NT / 64];
@@ -858,8 +949,8 @@ __global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, Sampl
   if (!sample_active<PHASE>(a, r, mk) || S->st.done) return;
   r.set_max(mk);
   const SampleCut kc = S->kcut;
-  const bool listed = S->st.count <= LLIST;
-  const unsigned n = listed ? S->listed : 0u;
+  const unsigned n = S->listed;
+  const bool listed = n <= LLIST;
   const unsigned* list = g.list + (long long)b * LLIST;
   if (tid == 0) { st = S->st; cut = S->cut; }
   __syncthreads();
@@ -879,7 +970,7 @@ __global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, Sampl
   }
   const int rounds = a.type == UR_F32 ? 3 : 2;
   for (int round = 0; round < rounds && !st.done; ++round) {
-    for (int i = tid; i < SB; i += NT) {
+    for (int i = tid; i < SBP; i += NT) {
       hc[i] = 0u;
       if (PHASE == 1) hw[i] = 0;
     }
@@ -914,8 +1005,8 @@ __global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, Sampl
     if (PHASE == 0) S->kcut = cut;
   }
 }
-__device__ __forceinline__ SampleCut final_cut(const SampleState* S, const SampleRow& r) {
-  return r.greedy ? SampleCut{S->maxkey, 1u} : S->cut;
+__device__ __forceinline__ SampleCut final_cut(const SampleState* S, const SampleRow& r) {   // (set_max has been called)
+  return r.greedy ? SampleCut{S->maxkey, 1u} : above_min_p(S->cut, r.min_key(S->maxkey));
 }
 __device__ __forceinline__ bool some_ties(const SampleCut& c) { return c.ties != 0u && c.ties != ALL_TIES; }
 // ties of every block (rows where some of them go)
@@ -923,7 +1014,10 @@ __global__ __launch_bounds__(256) void sample_ties_kernel(SampleArgs a, SampleLo
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   SampleRow r;
   r.load(a, b);
-  const SampleCut c = final_cut(g.state + b, r);
+  const SampleState* S = g.state + b;
+  if (S->maxkey == 0u || (!r.greedy && !some_ties(S->cut))) return;
+  r.set_max(S->maxkey);
+  const SampleCut c = final_cut(S, r);
   if (!some_ties(c)) return;
   const long long base = (long long)b * a.ld;
   for (int q = blockIdx.x * (g.chunk / LBLK) + wave; q < min(g.nblk, (int)(blockIdx.x + 1) * (g.chunk / LBLK)); q += 4) {
@@ -945,7 +1039,9 @@ __device__ __forceinline__ unsigned ties_before(const unsigned* tb, int q) {   /
   for (int t = threadIdx.x & 63; t < q; t += 64) n += tb[t];
   return wave_total(n);
 }
-// the kept weight of every block: a wave a block of 2 048, four consecutive entries a lane
+// the kept weight of every block: a wave a block of 2 048, four consecutive entries a lane.  Scores are compared as floats (a key's order is
+// theirs, the keys in front of the first number are -inf)
+template <int TYPE>
 __global__ __launch_bounds__(256) void sample_sums_kernel(SampleArgs a, SampleLong g) {
   const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   SampleRow r;
@@ -955,35 +1051,41 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(SampleArgs a, SampleLo
   r.set_max(S->maxkey);
   const SampleCut c = final_cut(S, r);
   const bool ranked = some_ties(c);
+  const float above = cut_value(c.cut, TYPE);
+  const double m = (double)r.m, scale = r.scale;
   const long long base = (long long)b * a.ld;
   for (int q = blockIdx.x * (g.chunk / LBLK) + wave; q < min(g.nblk, (int)(blockIdx.x + 1) * (g.chunk / LBLK)); q += 4) {
     const long long i0 = (long long)q * LBLK, i1 = min(a.N, i0 + LBLK);
     const bool wide = sample_wide(a, base + i0);
     unsigned ties = ranked ? ties_before(g.tb + (long long)b * g.nblk, q) : 0u;
-    WSum v{0, 0};
-    Four next[4];
+    u64 sum = 0;                        // (32 entries of at most 2^57)
+    FourX next[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) next[u] = sample_four(a, base, i0 + 256 * u + 4 * lane, i1, wide);
+    for (int u = 0; u < 4; ++u) next[u] = four_scores<TYPE>(a, base, i0 + 256 * u + 4 * lane, i1, wide);
 #pragma unroll
     for (int j = 0; j < LBLK / 256; ++j) {
-      const Four f = next[j & 3];
-      if (j + 4 < LBLK / 256) next[j & 3] = sample_four(a, base, i0 + 256 * (j + 4) + 4 * lane, i1, wide);
+      const FourX f = next[j & 3];
+      if (j + 4 < LBLK / 256) next[j & 3] = four_scores<TYPE>(a, base, i0 + 256 * (j + 4) + 4 * lane, i1, wide);
       unsigned rank = 0;
       if (ranked) {
         unsigned eq = 0;
 #pragma unroll
-        for (int u = 0; u < 4; ++u) eq += f.k[u] == c.cut;
+        for (int u = 0; u < 4; ++u) eq += f.x[u] == above;
         const unsigned upto = wave_upto(eq);
         rank = ties + upto - eq;
         ties += last_lane(upto);
       }
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        const unsigned k = f.k[u];
-        const bool stays = k > c.cut || (k == c.cut && k != 0u && rank++ < c.ties);
-        if (stays) v.add(r.kept(k));
+        const float x = f.x[u];
+        bool stays = x > above;
+        if (ranked) stays |= x == above && rank++ < c.ties;
+        const double z = r.flat ? (x == r.m ? 0.0 : -100.0) : ((double)x - m) * scale;
+        sum += stays ? exp2_fixed(z) : 0;
       }
     }
+    WSum v{0, 0};
+    v.add(sum);
     v.hi = wave_total(v.hi);
     v.lo = wave_total(v.lo);
     if (lane == 0) {
@@ -1050,13 +1152,13 @@ __global__ __launch_bounds__(256) void sample_draw_kernel(SampleArgs a, SampleLo
 #pragma unroll
   for (int u = 0; u < 8; ++u) {
     const bool stays = k[u] > c.cut || (k[u] == c.cut && k[u] != 0u && rank++ < c.ties);
-    w[u] = stays ? r.kept(k[u]) : 0;
+    w[u] = stays ? r.weight(k[u]) : 0;
     mine.add(w[u]);
   }
   run.add(block_before<256>(mine, tmp64, &all));
   u128 sum = run.all();
   if (sum <= goal && goal < sum + mine.all()) {
-    const double log_W = log(wide_to_double(W) * 2.168404344971009e-19);   // 2^-62
+    const double log_W = log(wide_to_double(W) * 6.938893903907228e-18);   // 2^-57
     bool found = false;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
@@ -1076,6 +1178,7 @@ static inline int log2_up(long long n) {
   while ((1LL << k) < n) ++k;
   return k;
 }
+static inline int coarse_bits(long long n) { return std::max(0, log2_up(n) - 6); }   // sums of n weights stay below 2^63
 static inline bool sample_in_lds(long long N, int type) { return N <= (type == UR_F32 ? 32768 : 65536); }
 static size_t sample_long_bytes(long long N, int B, char* base, SampleLong* g) {
   size_t o = 0;
@@ -1088,9 +1191,9 @@ static size_t sample_long_bytes(long long N, int B, char* base, SampleLong* g) {
   // about 2 048 workgroups where there is work for them, of 4 096 to 65 536 entries
   const long long want = (N * (long long)B + 2047) / 2048;
   w.chunk = (int)std::min<long long>(65536, std::max<long long>(4096, (want + 4095) / 4096 * 4096));
-  w.nchunk = cdiv(N, w.chunk); w.nblk = cdiv(N, LBLK); w.coarse = log2_up(N);
+  w.nchunk = cdiv(N, w.chunk); w.nblk = cdiv(N, LBLK); w.coarse = coarse_bits(N);
   w.state = (SampleState*)take(sizeof(SampleState) * B);
-  w.hc = (unsigned*)take((size_t)B * SB * 4); w.hw = (u64*)take((size_t)B * SB * 8);
+  w.hc = (unsigned*)take((size_t)B * SBP * 4); w.hw = (u64*)take((size_t)B * SBP * 8);
   w.tb = (unsigned*)take((size_t)B * w.nblk * 4); w.bs = (u64*)take((size_t)B * w.nblk * 16);
   w.list = (unsigned*)take((size_t)B * LLIST * 4);
   if (g) *g = w;
@@ -1098,10 +1201,10 @@ static size_t sample_long_bytes(long long N, int B, char* base, SampleLong* g) {
 }
 template <int NT, bool RAW>
 static int launch_sample_row(const SampleArgs& a, hipStream_t st) {
-  const size_t lds = (size_t)SB * 12 + (size_t)a.N * (RAW ? 2 : 4) + 16;
+  const size_t lds = (size_t)SBP * 12 + (size_t)a.N * (RAW ? 2 : 4) + 16;
   static const hipError_t attr = hipFuncSetAttribute((const void*)sample_row_kernel<NT, RAW>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 6144);
   (void)attr;
-  hipLaunchKernelGGL((sample_row_kernel<NT, RAW>), dim3(a.B), dim3(NT), lds, st, a, log2_up(a.N));
+  hipLaunchKernelGGL((sample_row_kernel<NT, RAW>), dim3(a.B), dim3(NT), lds, st, a, coarse_bits(a.N));
   UR_LAUNCH_CHECK();
   return UR_OK;
 }
@@ -1153,7 +1256,9 @@ extern "C" int ur_sample_scores(const void* scores, int32_t score_type, int64_t 
   UR_LAUNCH_CHECK();
   auto select = [&](auto phase) -> int {
     constexpr int PHASE = decltype(phase)::value;
-    hipLaunchKernelGGL((sample_steps_kernel<PHASE>), grid, dim3(256), 0, st, a, g, mode);
+    if (score_type == UR_F32) hipLaunchKernelGGL((sample_steps_kernel<PHASE, UR_F32>), grid, dim3(256), 0, st, a, g, mode);
+    else if (score_type == UR_F16) hipLaunchKernelGGL((sample_steps_kernel<PHASE, UR_F16>), grid, dim3(256), 0, st, a, g, mode);
+    else hipLaunchKernelGGL((sample_steps_kernel<PHASE, UR_BF16>), grid, dim3(256), 0, st, a, g, mode);
     UR_LAUNCH_CHECK();
     hipLaunchKernelGGL((sample_near_kernel<PHASE>), grid, dim3(256), 0, st, a, g);
     UR_LAUNCH_CHECK();
@@ -1168,7 +1273,9 @@ extern "C" int ur_sample_scores(const void* scores, int32_t score_type, int64_t 
     hipLaunchKernelGGL(sample_ties_kernel, grid, dim3(256), 0, st, a, g);
     UR_LAUNCH_CHECK();
   }
-  hipLaunchKernelGGL(sample_sums_kernel, grid, dim3(256), 0, st, a, g);
+  if (score_type == UR_F32) hipLaunchKernelGGL((sample_sums_kernel<UR_F32>), grid, dim3(256), 0, st, a, g);
+  else if (score_type == UR_F16) hipLaunchKernelGGL((sample_sums_kernel<UR_F16>), grid, dim3(256), 0, st, a, g);
+  else hipLaunchKernelGGL((sample_sums_kernel<UR_BF16>), grid, dim3(256), 0, st, a, g);
   UR_LAUNCH_CHECK();
   hipLaunchKernelGGL(sample_draw_kernel, dim3(S, B), dim3(256), 0, st, a, g);
   UR_LAUNCH_CHECK();
