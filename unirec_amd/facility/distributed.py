@@ -142,6 +142,8 @@ class ShardedSparseDenseAdam(SparseDenseAdam):
         initialised per rank): nothing is broadcast or cut for them -- how a 100 M-row table is brought up without ever
         existing in one piece (bench.py); by default the model's full tables are broadcast from rank 0 and cut here.
         cap_slack: capacity per (source, owner) pair = cap_slack x lookups / world (uniform ids need ~1.1)."""
+        if getattr(model, "loss_type", None) == "distill":
+            raise NotImplementedError("loss_type='distill' over a row-sharded table: the loss runs on one GPU")
         self.rank, self.world = rank, world
         self.xchg = RowExchange(world, rank, group)
         self.full_rows = {}

@@ -17,6 +17,7 @@ import os
 import torch
 
 from .. import ops
+from ..constants import DENSE_LOSSES
 
 
 class SparseDenseAdam:
@@ -56,8 +57,8 @@ class SparseDenseAdam:
                 w = getattr(model, name).weight.data
                 st = dict(w=w, m=torch.zeros_like(w), v=torch.zeros_like(w))
                 st["last"] = torch.zeros(w.shape[0], dtype=torch.int32, device=dev) if table_mode == "lazy_dense" else None
-                if name == "item_embedding" and getattr(model, "loss_type", None) == "fullsoftmax":
-                    st["last"] = None      # fullsoftmax: a dense [N,d] gradient every step -> plain dense Adam on this table
+                if name == "item_embedding" and getattr(model, "loss_type", None) in DENSE_LOSSES:
+                    st["last"] = None      # a dense [N,d] gradient every step -> plain dense Adam on this table
                 self.tables[name] = st
         self._plans = {}
         # dense_side: "" = per call (step(late_join=...) -> "late" / "join"); "late" / "join" / "0" force one mode ("0": the dense half on
@@ -304,7 +305,7 @@ class SparseDenseAdam:
                 ops.rows_reduce_update(cfg, st["w"], st["m"], st["v"], pl, rows, coef, vec, G, st["last"], guard, next_split=split)
                 continue
             reduced[name] = (pl, ops.rows_reduce(pl, rows, coef, vec, G, d, zero_tail=self.grad_clip is not None))
-        # fullsoftmax: the table's gradient is dense; the encoder's row-sparse part is folded into it
+        # fullsoftmax, distill: the table's gradient is dense; the encoder's row-sparse part is folded into it
         dense_tables = dict(model.dense_table_grads)
         for name, dg in dense_tables.items():
             if name in reduced:

@@ -253,6 +253,7 @@ class Trainer(object):
         self.scheduler = self._build_scheduler(config.get("scheduler", "off"), config.get("scheduler_factor", 0.1))
         self.best_valid_score, self.cur_step, self.start_epoch = None, 1, 0
         self.step_losses = []
+        self.teacher, self.teacher_k = None, 0
 
     def _build_optimizer(self, opt_type):
         """Trainer._build_optimizer (unirec/facility/trainer.py:134-152): same names, same fall-back."""
@@ -289,8 +290,19 @@ class Trainer(object):
         self.eval_protocol = eval_protocol
 
     # ------------------------------------------------------------------ the step (trainer.py:327-357)
+    def set_teacher(self, teacher, k):
+        """loss_type='distill': the model whose ``topk(batch, k)`` a step is trained on.  A batch that brings its own list (``teacher_id``
+        [B,K] and ``teacher_score`` [B,K], e.g. stored ones) is trained on that."""
+        if self.model.loss_type != "distill":
+            raise ValueError(f"set_teacher: loss_type={self.model.loss_type!r} learns from labels (loss_type='distill')")
+        if teacher is self.model or teacher.n_items != self.model.n_items:
+            raise ValueError("set_teacher: the teacher is another model of the same catalogue")
+        if not 1 <= int(k) <= 1024:
+            raise ValueError(f"set_teacher: k={k} (1 to 1024 items of the teacher's list)")
+        self.teacher, self.teacher_k = teacher, int(k)
+
     def _plan_ids(self, batch):
-        return dict(item_seq=batch.get("item_seq"), item_id=batch["item_id"],
+        return dict(item_seq=batch.get("item_seq"), item_id=batch.get("item_id") if self.model.loss_type == "distill" else batch["item_id"],
                     user_id=batch.get("user_id") if hasattr(self.model, "user_embedding") else None)
 
     def train_step(self, batch, next_batch=None):
@@ -304,7 +316,13 @@ class Trainer(object):
         opt.plan_batch(**self._plan_ids(batch))
         if next_batch is not None:
             opt.prefetch_plan(**self._plan_ids(next_batch))
-        kw = {k: batch[k] for k in ("user_id", "item_id", "label", "item_seq", "item_seq_len") if k in batch}
+        kw = {k: batch[k] for k in ("user_id", "item_id", "label", "item_seq", "item_seq_len", "teacher_id", "teacher_score") if k in batch}
+        if model.loss_type == "distill" and "teacher_id" not in kw:
+            if self.teacher is None:
+                raise ValueError("loss_type='distill': no teacher (set_teacher) and no teacher_id / teacher_score in the batch")
+            if self.teacher.training:
+                self.teacher.eval()
+            kw["teacher_score"], kw["teacher_id"] = self.teacher.topk(batch, self.teacher_k)
         if self.config.get("fused_step", True):
             loss = model.forward_backward(**kw)       # same launches as forward + backward, no autograd graph
         else:

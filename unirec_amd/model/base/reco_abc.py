@@ -17,7 +17,7 @@ import torch
 import torch.nn as nn
 
 from ... import ops
-from ...constants import LOSS_TYPES
+from ...constants import DENSE_LOSSES, LOSS_TYPES
 
 
 class SparseTable(nn.Module):
@@ -51,7 +51,7 @@ class AbstractRecommender(nn.Module):
         self.__optimized_by_SGD__ = True
         self.config = config
         self.sparse_grads = []     # filled by backward: dicts consumed by facility.optimizer
-        self.dense_table_grads = {}  # fullsoftmax: {table name: dense [N,d] gradient} (every row moves)
+        self.dense_table_grads = {}  # DENSE_LOSSES: {table name: dense [N,d] gradient} (every row moves)
         self._init_attributes()
         self._init_modules()
         self.annotations = []
@@ -93,12 +93,15 @@ class AbstractRecommender(nn.Module):
         self.SCORE_CLIP = config.get("score_clip_value", -1) or -1
         self.has_user_bias = bool(config.get("has_user_bias", False))
         self.has_item_bias = bool(config.get("has_item_bias", False))
-        if self.loss_type == "fullsoftmax" and self.has_user_bias and self.SCORE_CLIP > 0:
-            # the fullsoftmax kernels take d loss / d user_bias as exactly 0 (a per-user shift cancels in the softmax over n); a score clamp
+        if self.loss_type in DENSE_LOSSES and self.has_user_bias and self.SCORE_CLIP > 0:
+            # these losses' kernels take d loss / d user_bias as exactly 0 (a per-user shift cancels in the softmax over n); a score clamp
             # (recommender.py:94-95) breaks that invariance wherever it saturates, and that term is not computed: refuse instead of drifting
-            raise NotImplementedError("loss_type='fullsoftmax' with has_user_bias and score_clip_value > 0: the user-bias gradient under an "
+            raise NotImplementedError(f"loss_type={self.loss_type!r} with has_user_bias and score_clip_value > 0: the user-bias gradient under an "
                                       "active score clamp is not implemented (drop the clamp or the user bias)")
         self.tau = config.get("tau", 1.0)
+        self.distill_temperature = float(config.get("distill_temperature", 1.0))
+        if not self.distill_temperature > 0:
+            raise ValueError(f"distill_temperature={self.distill_temperature} must be positive")
 
     def _init_modules(self):  # reco_abc.py:159-208
         dev = self.device

@@ -11,6 +11,7 @@ import numpy as np
 import torch
 
 from ... import ops
+from ...constants import DENSE_LOSSES
 from .reco_abc import AbstractRecommender
 
 
@@ -80,6 +81,24 @@ class _FullSoftmaxFn(torch.autograd.Function):
         return model._fs_d_user, None, None, None
 
 
+class _DistillFn(torch.autograd.Function):
+    """loss = T^2 mean_b KL(teacher's top list || softmax over ALL items), the scores those of fullsoftmax"""
+
+    @staticmethod
+    def forward(ctx, user_emb, model, teacher_id, teacher_score):
+        user_emb = user_emb.contiguous()
+        loss_out, lse, saved = model._distill_forward(user_emb, teacher_id, teacher_score)
+        ctx.model, ctx.saved = model, saved
+        ctx.save_for_backward(user_emb, teacher_id, lse, loss_out)
+        object.__setattr__(model, "loss_guard", loss_out[2:3])
+        return loss_out[0]
+
+    @staticmethod
+    def backward(ctx, d_loss):
+        user_emb, teacher_id, lse, loss_out = ctx.saved_tensors
+        return ctx.model._distill_backward(user_emb, teacher_id, lse, loss_out, ctx.saved, d_loss.contiguous().view(1).float()), None, None, None
+
+
 class _TableLookupFn(torch.autograd.Function):
     """user_emb = U[user_id] with a row-sparse gradient (MF: recommender.py:42-44)."""
 
@@ -132,7 +151,14 @@ class BaseRecommender(AbstractRecommender):
 
     # ---- forward ----------------------------------------------------------------------------
     def forward(self, user_id=None, item_id=None, label=None, item_features=None, item_seq=None, item_seq_len=None,
-                item_seq_features=None, time_seq=None, session_id=None, reduction=True, return_loss_only=True, max_len=None):
+                item_seq_features=None, time_seq=None, session_id=None, reduction=True, return_loss_only=True, max_len=None,
+                teacher_id=None, teacher_score=None):
+        if self.loss_type == "distill" and self.training:
+            if not (reduction and return_loss_only):
+                raise NotImplementedError("distill: the [B, n_items] score matrix is never materialised (reduction / return_loss_only)")
+            teacher_id, teacher_score = self._teacher_list(teacher_id, teacher_score)
+            user_emb = self.forward_user_emb(user_id, item_seq, item_seq_len, item_seq_features, time_seq)
+            return _DistillFn.apply(user_emb, self, teacher_id, teacher_score), None, None, None
         if self.loss_type == "fullsoftmax" and self.training:
             # label = item_id, candidates = every item (recommender.py:47-50)
             if getattr(self, "_fs_shard_step", None) is not None:
@@ -179,12 +205,35 @@ class BaseRecommender(AbstractRecommender):
             self.user_bias.grad = torch.zeros_like(self.user_bias)   # softmax is shift invariant along n: exactly 0
         object.__setattr__(self, "_fs_d_user", d_user)
 
+    @staticmethod
+    def _teacher_list(teacher_id, teacher_score):
+        if teacher_id is None or teacher_score is None:
+            raise ValueError("loss_type='distill' trains on teacher_id [B,K] and teacher_score [B,K] (what a teacher's topk returns)")
+        return teacher_id.contiguous(), teacher_score.detach().contiguous()
+
+    def _distill_args(self):
+        return dict(item_bias=self.item_bias.data if self.has_item_bias else None, tau=self.tau, score_clip=self.SCORE_CLIP,
+                    temperature=self.distill_temperature)
+
+    def _distill_forward(self, user_emb, teacher_id, teacher_score):
+        return ops.full_distill_fwd(user_emb, self.item_embedding.weight.data, teacher_id, teacher_score, **self._distill_args())
+
+    def _distill_backward(self, user_emb, teacher_id, lse, loss_out, saved, d_loss):
+        d_user, d_table, d_ib = ops.full_distill_bwd(user_emb, self.item_embedding.weight.data, teacher_id, lse, loss_out, saved, d_loss=d_loss,
+                                                     **self._distill_args())
+        self.dense_table_grads["item_embedding"] = d_table
+        if self.has_item_bias:
+            self.item_bias.grad = d_ib
+        if self.has_user_bias:
+            self.user_bias.grad = torch.zeros_like(self.user_bias)   # the softmax is shift invariant along n: exactly 0
+        return d_user
+
     def lookup_tables(self):
         """Which batch field indexes which row-sparse table: {table: (explicit-row ids, scorer candidate ids)}; the optimizer
         plans the batch's id sort from it.  Default: MF-style (user table <- user_id, item table <- scorer candidates);
         sequence models add item_seq to the item table."""
-        # fullsoftmax TRAINING: every item is a candidate, their gradient is dense; evaluation scores item_id like every other loss
-        cand = None if (self.loss_type == "fullsoftmax" and self.training) else "item_id"
+        # fullsoftmax / distill TRAINING: every item is a candidate, their gradient is dense; evaluation scores item_id like every other loss
+        cand = None if (self.loss_type in DENSE_LOSSES and self.training) else "item_id"
         spec = {"item_embedding": ("item_seq" if "SeqRecBase" in self.annotations else None, cand)}
         if hasattr(self, "user_embedding"):
             spec["user_embedding"] = ("user_id", None)
@@ -256,7 +305,8 @@ class BaseRecommender(AbstractRecommender):
             self.dense_flat.grad = g
             object.__setattr__(self, "_deferred_dense_grad", None)
 
-    def forward_backward(self, user_id=None, item_id=None, label=None, item_seq=None, item_seq_len=None, **_unused):
+    def forward_backward(self, user_id=None, item_id=None, label=None, item_seq=None, item_seq_len=None, teacher_id=None,
+                         teacher_score=None, **_unused):
         """``loss = model(...); loss.backward()`` (unirec/facility/trainer.py:340-346) as one straight-line sequence of
         the same HIP launches, without building/walking an autograd graph: leaves ``dense_flat.grad``, the bias
         gradients and ``sparse_grads`` exactly as ``backward()`` would, and returns the (detached) loss.
@@ -264,6 +314,14 @@ class BaseRecommender(AbstractRecommender):
         this step size; the trainer therefore uses this entry point (config ``fused_step``, default on)."""
         if not self.training:
             raise RuntimeError("forward_backward is a training-mode entry point")
+        if self.loss_type == "distill":
+            teacher_id, teacher_score = self._teacher_list(teacher_id, teacher_score)
+            user_emb, state = self._encode_train(user_id, item_seq, item_seq_len)
+            user_emb = user_emb.contiguous()
+            loss_out, lse, saved = self._distill_forward(user_emb, teacher_id, teacher_score)
+            self._encode_backward(state, self._distill_backward(user_emb, teacher_id, lse, loss_out, saved, None))
+            object.__setattr__(self, "loss_guard", loss_out[2:3])
+            return loss_out[0]
         if self.loss_type == "fullsoftmax":
             user_emb, state = self._encode_train(user_id, item_seq, item_seq_len)
             user_emb = user_emb.contiguous()
@@ -382,3 +440,11 @@ class BaseRecommender(AbstractRecommender):
         return ops.full_topk(user_emb, self.item_embedding.weight.data, k, hist_uid if (hp is not None or self.has_user_bias) else None,
                              hp, hs, self.user_bias.data if self.has_user_bias else None,
                              self.item_bias.data if self.has_item_bias else None, self.tau)
+
+    def sample(self, interaction, rand, k=100, temperature=1.0, top_p=1.0, min_p=0.0, user_hist=None):
+        """Items drawn from the softmax over the k best of a batch of users (k <= 1024; topk's scores, candidates and user_hist), one for
+        every random number in [0, 1): rand float32 [B] or [B, S].  temperature 0: always the best item; top_p: of the k, best first, every
+        item before which less than top_p of the weight lies; min_p: items with at least min_p of the best one's weight.  Each of the three
+        may be a tensor [B].  -> (ids int64, log-probabilities float32), shaped like rand; (-1, -inf) for a user with no item left."""
+        scores, ids = self.topk(interaction, k, user_hist=user_hist)
+        return ops.sample_scores(scores, rand, temperature=temperature, top_p=top_p, min_p=min_p, ids=ids)
