@@ -740,23 +740,22 @@ int ur_rows_scatter_add(const int32_t* uniq_idx, const int32_t* n_uniq_dev, int6
  *   pads with; the padding row) or its score is -inf or NaN; an id outside [-1,n_items) raises the id guard and is absent too; an item
  *   listed twice has both entries' mass;
  *   loss = T^2 / C * sum_b sum_k p_bk (log p_bk - s(b, id_bk) / T + lse[b]), C = rows with a present entry (the others count for nothing).
- * teacher_id, entry_id: int64[B,K]; teacher_score: [B,K] of score_type (UR_F32 / UR_F16 / UR_BF16; the softmax is fp32).
- *   fwd: lse[B], loss_out[4] = [loss, C, update guard, -], row_stat[3B] (what the backward needs of a row); with coef[B,K], entry_id[B,K] and
- *        d_unit[B,d] (all three or none) the pass also leaves what the backward needs: p, the items, sum_n q E - sum_k p E.
+ * teacher_id: int64[B,K]; teacher_score: [B,K] of score_type (UR_F32 / UR_F16 / UR_BF16; the softmax is fp32).
+ *   fwd: lse[B], loss_out[4] = [loss, C, update guard, -]; need_grad: the pass also leaves in ws what the backward needs (the teacher's
+ *        entries by item, sum_n q E - sum_k p E, the users' rows as its matrix operand).
  *   bwd: d_user_emb[B,d]; d_item_table [n_items,d] DENSE and overwritten (row 0 = 0: padding_idx); d_item_bias [n_items] (required iff
  *        item_bias); a per-user bias would cancel in q: it has none.  d_loss: device scalar (nullable = 1).  No gradient where the score was clipped.
  * tau, temperature > 0; d % 4 == 0, d <= 256.  Nothing of size [B, n_items] exists; results are bit-reproducible.
- * ws: ur_full_distill_workspace_bytes, for one call (need_grad: also the backward's). */
+ * A score within rounding of +-score_clip may be taken as cut or as not.
+ * ws: ur_full_distill_workspace_bytes of the same sizes and need_grad, from the forward to its backward, which only reads it. */
 enum { UR_F32 = 0, UR_F16 = 1, UR_BF16 = 2 }; /* element types of teacher_score and of ur_sample_scores' scores */
 int64_t ur_full_distill_workspace_bytes(int32_t B, int32_t d, int64_t n_items, int32_t K, int32_t need_grad);
 int ur_full_distill_fwd(const float* user_emb, const float* item_table, int64_t n_items, int32_t B, int32_t d, const int64_t* teacher_id,
                         const void* teacher_score, int32_t score_type, int32_t K, const float* item_bias, float tau, float score_clip,
-                        float temperature, float* lse, float* loss_out, float* row_stat, float* coef, int64_t* entry_id, float* d_unit,
-                        void* ws, void* stream);
+                        float temperature, float* lse, float* loss_out, int32_t need_grad, void* ws, void* stream);
 int ur_full_distill_bwd(const float* user_emb, const float* item_table, int64_t n_items, int32_t B, int32_t d, int32_t K,
-                        const float* item_bias, float tau, float score_clip, float temperature, const float* loss_out,
-                        const float* row_stat, const float* coef, const int64_t* entry_id, const float* d_unit, const float* d_loss,
-                        float* d_user_emb, float* d_item_table, float* d_item_bias, void* ws, void* stream);
+                        const float* item_bias, float tau, float score_clip, float temperature, const float* loss_out, const float* d_loss, float* d_user_emb,
+                        float* d_item_table, float* d_item_bias, const void* ws, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
  * Sampling from scores with temperature, top-k, top-p and min-p, from given random numbers (no counterpart in UniRec; beside

@@ -5,7 +5,7 @@ The tolerances are arithmetic, element by element.  With eps = 2^-24 (half a ste
   of 2^-36 of the largest |x| |y|, and its fp32 sum over D by D eps more: the log score is off by  ds = (2^-21 + (D + 8) eps) A / (tau T) + 8 eps |s|,
   A = sum |u| |E|;
   q = exp(s - lse) is then off by a factor 1 + dq,  dq = 2 ds + 16 eps (|log q| <= 100) + 2^-21 (its own split), and sums over n terms add n eps;
-  the split weights have a floor of 2^-30 of the largest weight of a row (forward) or column (backward)."""
+  the split weights have a floor of 2^-30 of the largest weight of a row (forward) or column (backward; a weight there is q - p)."""
 import math
 
 import pytest
@@ -92,7 +92,7 @@ def _check(r, U, E, loss_out, lse, grads, d_loss=1.0):
     Qt = r["Q"] * (dq + N * EPS) + 2.0 ** -30 * r["Q"].amax(1, keepdim=True)
     Pt = r["P"] * (40 * EPS + 4 * EPS * 40)
     _close(du, r["dU"] * d_loss, g * ((Qt + Pt) @ Ea) + 4 * EPS * (r["dU"] * d_loss).abs() + 1e-37, "d_user")
-    Qt = r["Q"] * (dq + B * EPS) + 2.0 ** -30 * r["Q"].amax(0, keepdim=True)
+    Qt = r["Q"] * (dq + B * EPS) + 2.0 ** -30 * torch.maximum(r["Q"], r["P"]).amax(0, keepdim=True)
     _close(dt, r["dE"] * d_loss, g * ((Qt + Pt).t() @ Ua) + 4 * EPS * (r["dE"] * d_loss).abs() + 1e-37, "d_table")
     assert (dt[0] == 0).all()
     if dib is not None:
@@ -125,14 +125,14 @@ def test_refusals():
     assert lib.ur_full_distill_workspace_bytes(400, 64, 1682, 20, 1) > lib.ur_full_distill_workspace_bytes(400, 64, 1682, 20, 0) > 0
     one = 1 << 20                                                                         # never read: every call below is refused first
 
-    def fwd(B=4, d=16, N=20, K=3, t=0, tau=1.0, T=1.0, coef=one, tid=one, unit=one, U=one):
-        return lib.ur_full_distill_fwd(U, one, N, B, d, one, one, t, K, None, tau, -1.0, T, one, one, one, coef, tid, unit, one, None)
+    def fwd(B=4, d=16, N=20, K=3, t=0, tau=1.0, T=1.0, U=one, ws=one):
+        return lib.ur_full_distill_fwd(U, one, N, B, d, one, one, t, K, None, tau, -1.0, T, one, one, 1, ws, None)
 
     for bad, msg in ((dict(U=None), b"null pointer"), (dict(d=18), b"shape"), (dict(N=1), b"shape"), (dict(K=0), b"shape"), (dict(d=260), b"d=260"),
                      (dict(t=7), b"score_type"), (dict(tau=0.0), b"positive"), (dict(T=-1.0), b"positive"), (dict(T=math.nan), b"positive"),
-                     (dict(T=math.inf), b"positive"), (dict(coef=None), b"go together"), (dict(unit=None), b"go together")):
+                     (dict(T=math.inf), b"positive"), (dict(ws=None), b"null pointer")):
         assert fwd(**bad) in (-1, -3) and msg in lib.ur_last_error(), bad
-    rc = lib.ur_full_distill_bwd(one, one, 20, 4, 16, 3, one, 1.0, -1.0, 1.0, one, one, one, one, one, None, one, one, None, one, None)
+    rc = lib.ur_full_distill_bwd(one, one, 20, 4, 16, 3, one, 1.0, -1.0, 1.0, one, None, one, one, None, one, None)
     assert rc == -1 and b"d_item_bias" in lib.ur_last_error()
 
 
@@ -213,6 +213,31 @@ def test_masks_duplicates_and_absent_entries():
     loss_out, lse, grads = _run(U, E, ids, score, None, 1.0, 0.0, 1.0)
     r["loss"] = loss
     _check(r, U, E, loss_out, lse, grads)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,N,d,K", [(3, 40, 16, 30), (40, 300, 64, 1500), (70, 5000, 128, 260), (33, 1_200_000, 32, 40), (33, 1_200_000, 32, 160)])
+def test_lists_that_fall_on_few_items(B, N, d, K):
+    """every user lists the same few items, some of them over and over: one block of items has all entries, a cell has many"""
+    U, E, ids, score, ib = _inputs(B, N, d, K, seed=13, bias=True)
+    ids = torch.where(ids > 0, ids % min(N - 1, 50) + 1, ids)
+    if N > 10_000:                                              # lists' blocks are wider than a workgroup's items there
+        ids = torch.where(ids > 0, ids + N - 60, ids)
+    r = _reference(U, E, ids, score, ib, 1.0, 0.0, 1.5)
+    a = _run(U, E, ids, score, ib, 1.0, 0.0, 1.5)
+    _check(r, U, E, *a)
+    b = _run(U, E, ids, score, ib, 1.0, 0.0, 1.5)
+    assert torch.equal(a[0], b[0]) and all(torch.equal(x, y) for x, y in zip(a[2], b[2]))
+
+
+@pytest.mark.gpu
+def test_a_forward_serves_more_than_one_backward():
+    from unirec_amd import ops
+    U, E, ids, score, ib = (x.cuda() for x in _inputs(50, 700, 64, 9, seed=14, bias=True))
+    loss_out, lse, sv = ops.full_distill_fwd(U, E, ids, score, item_bias=ib)
+    a = ops.full_distill_bwd(U, E, ids, lse, loss_out, sv, item_bias=ib)
+    b = ops.full_distill_bwd(U, E, ids, lse, loss_out, sv, item_bias=ib, d_loss=torch.tensor([2.0], device="cuda"))
+    assert all(torch.equal(2 * x, y) for x, y in zip(a, b))
 
 
 def _loss64(r, ids, score):
@@ -355,7 +380,7 @@ def test_table_offsets_beyond_32_bits():
     p = torch.softmax(score.double(), 1)
     grad = q.scatter_add(1, ids - lo, -p) / B
     want = grad.t() @ U.double()
-    bound = (2 * tol + 2.0 ** -18) * (q.scatter_add(1, ids - lo, p) / B).t() @ U.double().abs() + 2.0 ** -28 * (q.amax(0) / B)[:, None] * U.double().abs().sum(0)
+    bound = (2 * tol + 2.0 ** -18) * (q.scatter_add(1, ids - lo, p) / B).t() @ U.double().abs() + 2.0 ** -28 * (q.scatter_add(1, ids - lo, p).amax(0) / B)[:, None] * U.double().abs().sum(0)
     assert ((dt[lo:].double() - want).abs() <= bound).all()
     mid = dt[N // 2: N // 2 + 1000]
     qm = torch.exp(U.double() @ E[N // 2: N // 2 + 1000].double().t() - ref[:, None]) / B
@@ -370,5 +395,5 @@ def test_torch_ops():
     a = _run(U, E, ids, score, ib, 0.9, 0.0, 1.5)
     U, E, ids, score, ib = (x.cuda() for x in (U, E, ids, score, ib))
     o = torch.ops.unirec_amd.full_distill_fwd(U, E, ids, score, ib, 0.9, -1.0, 1.5)
-    g = torch.ops.unirec_amd.full_distill_bwd(U, E, o[0], o[1], o[2], o[3], o[4], o[5], o[6], None, ib, 0.9, -1.0, 1.5)
+    g = torch.ops.unirec_amd.full_distill_bwd(U, E, ids, o[0], o[1], o[2], None, ib, 0.9, -1.0, 1.5)
     assert torch.equal(a[0], o[0]) and torch.equal(a[1], o[1]) and all(torch.equal(x, y) for x, y in zip(a[2], g))

@@ -175,10 +175,9 @@ SIGNATURES = {
     "ur_full_softmax_combine_shards": (C.c_int, [P, C.c_int32, C.c_int32, C.c_int32, C.c_int32, P, P, P]),
     "ur_full_softmax_bwd_shard": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, P, P, P, P, C.c_float, C.c_float, P, P, P, P, P, C.c_int32, P, P]),
     "ur_full_distill_workspace_bytes": (I64, [C.c_int32, C.c_int32, I64, C.c_int32, C.c_int32]),
-    "ur_full_distill_fwd": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, P, P, C.c_int32, C.c_int32, P, C.c_float, C.c_float, C.c_float, P, P, P, P, P,
-                                      P, P, P]),
-    "ur_full_distill_bwd": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, C.c_int32, P, C.c_float, C.c_float, C.c_float, P, P, P, P, P, P, P, P, P, P,
-                                      P]),
+    "ur_full_distill_fwd": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, P, P, C.c_int32, C.c_int32, P, C.c_float, C.c_float, C.c_float, P, P, C.c_int32,
+                                      P, P]),
+    "ur_full_distill_bwd": (C.c_int, [P, P, I64, C.c_int32, C.c_int32, C.c_int32, P, C.c_float, C.c_float, C.c_float, P, P, P, P, P, P, P]),
     "ur_sample_scores": (C.c_int, [P, C.c_int32, I64, I64, C.c_int32, P, C.c_int32, C.c_double, C.c_int32, C.c_double, C.c_double, P, P, P, P, P, I64,
                                    P, P, P, P]),
     "ur_sample_scores_workspace_bytes": (I64, [C.c_int32, I64, C.c_int32]),

@@ -8,7 +8,10 @@
 // STREAM of rows y, weights exp2(z - M), a sum l of the weights and a weighted sum of the stream's rows, one pass, nothing of size
 // B x N written.  The forward finds its maximum M on the way (online softmax); the backward knows q's denominator from the forward
 // pass (it rides in the stream rows' bias as -log2 of it), its M is a per-item reference that keeps q in fp16's range.
-// The teacher's K entries a row are sparse: gathered once in the forward, added to the table gradient through a row plan (rows.hip).
+// The teacher's K entries a row are sparse: gathered once in the forward, which leaves them as short lists by (tile of 32 users, bucket of
+// items); a workgroup per bucket adds them to the table gradient, in the order of the users.  Nothing is sorted over the whole batch (that
+// took 6 launches and 32 of 115 us at 60 K items, 512 users x 50 entries); taking the lists inside the stream kernel cost more than it saved
+// (35 -> 47 - 55 us there, its one barrier a tile waits for the wave that has entries, and D = 128 has no register left for it).
 #include <math.h>
 
 #include <algorithm>
@@ -504,7 +507,7 @@ struct DistillRow {
   float inv_tau, inv_T, clip;
   float* lse;
   float* stat;                         // [0, B) loss of the row, [B, 2B) 1 = has a teacher, [2B, 3B) log2 of the softmax sum (+inf without a teacher)
-  float* coef; long long* tid;         // [B, K]: p (0 where the gradient is cut), item (0 = absent)
+  float* coef; int* tid;               // [B, K]: p (0 where the gradient is cut), item (0: absent; negative: a second time)
   float* d_unit;                       // [B, d]: O_b - sum_k p E
   IdGuard guard;
 };
@@ -531,6 +534,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
   constexpr int G = 256 / TPR;
   __shared__ float red[4];
   __shared__ __attribute__((aligned(16))) float4 acc_s[256];
+  __shared__ __attribute__((aligned(16))) int items_s[GRAD ? 1024 : 4];
   const int b = blockIdx.x, tid = threadIdx.x, g = tid / TPR, t = tid % TPR, d4 = a.d / 4;
   const bool on = t < d4;
   float m = -INFINITY;
@@ -582,7 +586,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
     }
     if (GRAD && t == 0) {
       a.coef[i] = p;
-      a.tid[i] = there ? id : 0;
+      a.tid[i] = there ? (int)id : 0;
     }
   }
   loss = ds_block_sum(loss, red);
@@ -593,6 +597,36 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
     a.stat[2 * (long long)a.B + b] = some ? lse2 : INFINITY;
   }
   if constexpr (GRAD) {
+    // ---- an item listed again: the first of its entries takes their mass (in order)
+    float* coef = a.coef + (long long)b * a.K;
+    int* items = a.tid + (long long)b * a.K;
+    for (int k0 = 0; k0 < a.K; k0 += 256) {
+      const int k = k0 + tid, mine = k < a.K ? abs(items[k]) : 0;
+      bool before = false, after = false;
+      for (int c0 = 0; c0 < a.K; c0 += 1024) {
+        const int n = min(1024, a.K - c0);
+        __syncthreads();
+        for (int i = tid; i < 1024; i += 256) items_s[i] = i < n ? abs(items[c0 + i]) : -1;
+        __syncthreads();
+        if (mine)
+          for (int j = 0; j < n; j += 4) {
+            const int4 v = *(const int4*)(items_s + j);
+            const int q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              before |= q[e] == mine && c0 + j + e < k;
+              after |= q[e] == mine && c0 + j + e > k;
+            }
+          }
+      }
+      if (before) items[k] = -mine;
+      else if (after) {
+        float p = coef[k];
+        for (int j = k + 1; j < a.K; ++j)
+          if (abs(items[j]) == mine) p += coef[j];
+        coef[k] = p;
+      }
+    }
     for (int s = g; s < a.splits; s += G) {
       const long long at = (long long)s * a.B + b;
       const float f = exp2f(a.part_m[at] - lse2);
@@ -615,27 +649,35 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
   }
 }
 
+struct DistillLoss {
+  const float* stat; int B, d, K; float T2; float* loss_out;
+  const float* U; _Float16* img; float* rb_img; int* ky_img;
+  const float* coef; const int* tid; int buckets, shift; int* offs; uint2* list;
+};
 // Workgroup 0: loss_out = [T^2 / C sum of the rows' losses, C, update guard, -] (fixed order).  The others (a forward pass that will be
-// followed by a backward): the image of one tile of 32 users that every workgroup of the backward streams -- one exponent, [hi | lo][32][D]
-// halves in the swizzled order, the row biases -log2(softmax sum) (-inf without a teacher and behind the last user).
+// followed by a backward): what the backward needs of a tile of 32 users.  Its image, that every workgroup streams: one exponent, [hi | lo][32][D]
+// halves in the swizzled order, the row biases -log2(softmax sum) (-inf without a teacher and behind the last user).  And its teacher's
+// entries (item - first item of the bucket, user; p) by bucket of 2^shift items, a counting sort in LDS: the order inside a bucket is free.
 template <int D>
-__global__ __launch_bounds__(256) void distill_loss_kernel(const float* __restrict__ stat, int B, float T2, float* __restrict__ loss_out,
-                                                           const float* __restrict__ U, int d, _Float16* __restrict__ img,
-                                                           float* __restrict__ rb_img, int* __restrict__ ky_img) {
+__global__ __launch_bounds__(256) void distill_loss_kernel(DistillLoss a) {
   __shared__ float red[4];
+  __shared__ unsigned wave_s[4];
+  extern __shared__ unsigned count_s[];                          // [buckets]
+  const float* stat = a.stat;
+  const int B = a.B, d = a.d, tid = threadIdx.x;
   if (blockIdx.x == 0) {
     float s = 0.f, c = 0.f;
-    for (int b = threadIdx.x; b < B; b += 256) {
+    for (int b = tid; b < B; b += 256) {
       s += stat[b];
       c += stat[B + b];
     }
     s = ds_block_sum(s, red);
     c = ds_block_sum(c, red);
-    if (threadIdx.x == 0) {
-      loss_out[0] = T2 * s / fmaxf(c, 1.f);
-      loss_out[1] = c;
-      loss_out[2] = s != s ? -1.f : 1.f;   // update guard (see ur_gather_dot_loss_fwd)
-      loss_out[3] = 0.f;
+    if (tid == 0) {
+      a.loss_out[0] = a.T2 * s / fmaxf(c, 1.f);
+      a.loss_out[1] = c;
+      a.loss_out[2] = s != s ? -1.f : 1.f;   // update guard (see ur_gather_dot_loss_fwd)
+      a.loss_out[3] = 0.f;
     }
     return;
   }
@@ -647,12 +689,12 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(const float* __restri
   for (int p = 0; p < PER; ++p) {
     const int i = threadIdx.x + 256 * p, b = tile * DS_TILE + i / F4, c = (i % F4) * 4;
     v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (b < B && c < d) v[p] = *(const float4*)(U + (long long)b * d + c);
+    if (b < B && c < d) v[p] = *(const float4*)(a.U + (long long)b * d + c);
     mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(v[p].x), finite_abs(v[p].y)), fmaxf(finite_abs(v[p].z), finite_abs(v[p].w))));
   }
   const int ky = group_exponent(ds_block_max(mx, red));
   const float up = pow2i(ky);
-  _Float16* out = img + (long long)tile * 2 * DS_TILE * D;
+  _Float16* out = a.img + (long long)tile * 2 * DS_TILE * D;
 #pragma unroll
   for (int p = 0; p < PER; ++p) {
     const int i = threadIdx.x + 256 * p, at = ds_at<D>(i / F4, (i % F4) * 4);
@@ -662,57 +704,208 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(const float* __restri
     *(half4*)(out + at) = (half4){h0[0], h0[1], h1[0], h1[1]};
     *(half4*)(out + DS_TILE * D + at) = (half4){l0[0], l0[1], l1[0], l1[1]};
   }
-  if (threadIdx.x == 0) ky_img[tile] = ky;
-  if (threadIdx.x < DS_TILE) {
-    const int b = tile * DS_TILE + threadIdx.x;
-    rb_img[b] = b < B ? -stat[2 * (long long)B + b] : -INFINITY;
+  if (tid == 0) a.ky_img[tile] = ky;
+  if (tid < DS_TILE) {
+    const int b = tile * DS_TILE + tid;
+    a.rb_img[b] = b < B ? -stat[2 * (long long)B + b] : -INFINITY;
+  }
+  // ---- the lists
+  const int rows = min(DS_TILE, B - tile * DS_TILE);
+  const unsigned n = (unsigned)rows * (unsigned)a.K;
+  const long long e0 = (long long)tile * DS_TILE * a.K;
+  const int* items = a.tid + e0;
+  const float* coef = a.coef + e0;
+  for (int i = tid; i < a.buckets; i += 256) count_s[i] = 0u;
+  __syncthreads();
+#pragma unroll 4
+  for (unsigned i = tid; i < n; i += 256) {
+    const int item = items[i];
+    if (item > 0 && coef[i] != 0.f) atomicAdd(&count_s[item >> a.shift], 1u);
+  }
+  __syncthreads();
+  const int per = (a.buckets + 255) / 256, i0 = min(a.buckets, tid * per), i1 = min(a.buckets, i0 + per);
+  unsigned mine = 0u;
+  for (int i = i0; i < i1; ++i) mine += count_s[i];
+  unsigned upto = mine;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const unsigned v = (unsigned)__shfl_up((int)upto, o, 64);
+    if ((tid & 63) >= o) upto += v;
+  }
+  if ((tid & 63) == 63) wave_s[tid >> 6] = upto;
+  __syncthreads();
+  unsigned at = upto - mine;
+#pragma unroll
+  for (int w = 0; w < 3; ++w)
+    if (w < (tid >> 6)) at += wave_s[w];
+  int* offs = a.offs + (long long)tile * (a.buckets + 1);
+  for (int i = i0; i < i1; ++i) {
+    const unsigned c = count_s[i];
+    count_s[i] = at;
+    offs[i] = (int)at;
+    at += c;
+  }
+  if (tid == 255) offs[a.buckets] = (int)at;
+  __syncthreads();
+  uint2* list = a.list + e0;
+#pragma unroll 4
+  for (unsigned i = tid; i < n; i += 256) {
+    const int item = items[i];
+    const float p = coef[i];
+    if (item > 0 && p != 0.f)
+      list[atomicAdd(&count_s[item >> a.shift], 1u)] = make_uint2(((unsigned)item & ((1u << a.shift) - 1u)) << 5 | i / (unsigned)a.K, __float_as_uint(p));
   }
 }
 
 struct DistillApply {
-  const int *uniq, *seg, *pos, *n_uniq;
-  const float *coef, *U, *d_unit;
+  const int* offs; const uint2* list; int buckets, shift;
+  const float *U, *d_unit;
   int B, d, K;
   const float* loss_out; const float* d_loss; float g_num;
   float *d_user, *d_table, *d_bias;
-  int user_blocks;
 };
-// the first user_blocks workgroups: d_user = g d_unit; the others: a group of TPR lanes per distinct teacher item,
-// dE[item] -= g sum p u (the plan's order: bit-reproducible), d_bias[item] -= g sum p
+// A workgroup per bucket: dE[item] -= g sum p u, d_bias[item] -= g sum p over its lists of up to 16 tiles of users (512 users) at a time, put
+// in the order of (item, user) by a bitonic sort in LDS.  Lists longer than the room there: one tile at a time, 32 items (32 x 32 entries at
+// the most) at a time.  TPR lanes hold a row; a group of them takes an item, all groups one that many list (a popular item).  The
+// workgroups behind: d_user = g d_unit.  Latency bound: a chain of range, entries, rows, gradient.
 template <int TPR>
-__global__ __launch_bounds__(256) void distill_apply_kernel(DistillApply a) {
-  constexpr int G = 256 / TPR;
-  const float g = distill_scale(a.loss_out, a.d_loss, a.g_num);
-  const int d4 = a.d / 4;
-  if ((int)blockIdx.x < a.user_blocks) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+__global__ __launch_bounds__(128) void distill_apply_kernel(DistillApply a) {
+  constexpr int NT = 128, G = NT / TPR, ROOM = 1024, WINDOW = ROOM / DS_TILE, LONG = 32;
+  typedef unsigned long long u64;
+  __shared__ u64 entry_s[ROOM];                                  // item of the bucket << 41 | user of the 512 << 32 | p
+  __shared__ unsigned short run_s[ROOM + 1], long_s[ROOM];       // where an item's entries begin
+  __shared__ int first_s[16], count_s[16], n_s, runs_s, nlong_s;
+  __shared__ __attribute__((aligned(16))) float4 acc_s[NT];
+  __shared__ float accp_s[G];
+  const float gs = distill_scale(a.loss_out, a.d_loss, a.g_num);
+  const int d4 = a.d / 4, tid = threadIdx.x, grp = tid / TPR, t = tid % TPR;
+  if ((int)blockIdx.x >= a.buckets) {
+    const long long i = (long long)(blockIdx.x - a.buckets) * NT + tid;
     if (i < (long long)a.B * d4) {
       const float4 v = ((const float4*)a.d_unit)[i];
-      ((float4*)a.d_user)[i] = make_float4(g * v.x, g * v.y, g * v.z, g * v.w);
+      ((float4*)a.d_user)[i] = make_float4(gs * v.x, gs * v.y, gs * v.z, gs * v.w);
     }
     return;
   }
-  const int n = *a.n_uniq, t = threadIdx.x % TPR;
-  for (long long q = (long long)(blockIdx.x - a.user_blocks) * G + threadIdx.x / TPR; q < n; q += (long long)(gridDim.x - a.user_blocks) * G) {
-    const int item = a.uniq[q];
-    if (item == 0) continue;                                    // absent entries
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    float pb = 0.f;
-    for (int s = a.seg[q]; s < a.seg[q + 1]; ++s) {
-      const int at = a.pos[s];
-      const float p = a.coef[at];
-      pb += p;
-      if (t < d4) {
-        const float4 u = ((const float4*)a.U)[(long long)(at / a.K) * d4 + t];
-        acc.x += p * u.x; acc.y += p * u.y; acc.z += p * u.z; acc.w += p * u.w;
+  const int bucket = blockIdx.x, tiles = (a.B + DS_TILE - 1) / DS_TILE;
+  const long long item0 = (long long)bucket << a.shift;
+  for (int t0 = 0, m = 0; t0 < tiles; t0 += m) {
+    const int some = min(16, tiles - t0);
+    __syncthreads();
+    if (tid < 16) {
+      int f = 0, e = 0;
+      if (tid < some) {
+        const int* o = a.offs + (long long)(t0 + tid) * (a.buckets + 1) + bucket;
+        f = o[0];
+        e = o[1];
       }
+      first_s[tid] = f;
+      count_s[tid] = e - f;
     }
-    if (t < d4) {
-      float4* o = (float4*)a.d_table + (long long)item * d4 + t;
-      const float4 v = *o;
-      *o = make_float4(v.x - g * acc.x, v.y - g * acc.y, v.z - g * acc.z, v.w - g * acc.w);
+    __syncthreads();
+    int total = 0;
+    m = 0;
+    while (m < some && (m == 0 || total + count_s[m] <= ROOM)) total += count_s[m++];   // as many tiles as fit
+    if (total == 0) continue;
+    const int lanes = m > 8 ? 8 : m > 4 ? 16 : m > 2 ? 32 : m > 1 ? 64 : 128, tile = tid / lanes;   // threads of a tile
+    const int n_tile = tile < m ? count_s[tile] : 0;
+    const uint2* list = a.list + ((long long)(t0 + tile) * DS_TILE * a.K + (tile < m ? first_s[tile] : 0));
+    const bool fits = total <= ROOM;
+    const unsigned items = 1u << a.shift;
+    for (unsigned w0 = 0; w0 < items; w0 += fits ? items : (unsigned)WINDOW) {
+      const unsigned w1 = fits ? items : w0 + WINDOW;
+      if (tid == 0) n_s = nlong_s = 0;
+      __syncthreads();
+      for (int i = tid % lanes; i < n_tile; i += lanes) {
+        const uint2 v = list[i];
+        const unsigned o = v.x >> 5;
+        if (o >= w0 && o < w1) entry_s[atomicAdd(&n_s, 1)] = ((u64)o << 41) | ((u64)(unsigned)(tile * DS_TILE + (v.x & 31u)) << 32) | v.y;
+      }
+      __syncthreads();
+      const int n = n_s;
+      if (n == 0) { __syncthreads(); continue; }
+      int size = 2;
+      while (size < n) size *= 2;
+      for (int i = n + tid; i < size; i += NT) entry_s[i] = ~0ull;
+      __syncthreads();
+      for (int k = 2; k <= size; k *= 2)
+        for (int j = k / 2; j > 0; j /= 2) {
+          for (int i = tid; i < size / 2; i += NT) {
+            const int x = ((i & ~(j - 1)) << 1) | (i & (j - 1)), y = x | j;
+            const u64 vx = entry_s[x], vy = entry_s[y];
+            if ((vx > vy) == ((x & k) == 0)) { entry_s[x] = vy; entry_s[y] = vx; }
+          }
+          __syncthreads();
+        }
+      if (tid < 64) {
+        int runs = 0;
+        for (int i0 = 0; i0 < n; i0 += 64) {
+          const int i = i0 + tid;
+          const bool head = i < n && (i == 0 || (entry_s[i] >> 41) != (entry_s[i - 1] >> 41));
+          const u64 heads = __ballot(head);
+          if (head) run_s[runs + __popcll(heads & ((1ull << tid) - 1ull))] = (unsigned short)i;
+          runs += __popcll(heads);
+        }
+        if (tid == 0) { run_s[runs] = (unsigned short)n; runs_s = runs; }
+      }
+      __syncthreads();
+      const int runs = runs_s;
+      const float4* U = (const float4*)a.U + (long long)t0 * DS_TILE * d4 + t;
+      const bool on = t < d4;
+      auto sum = [&](int from, int to, int step, float4& acc, float& pb) {
+#pragma unroll 4
+        for (int e = from; e < to; e += step) {
+          const u64 v = entry_s[e];
+          const float p = __uint_as_float((unsigned)v);
+          pb += p;
+          if (on) {
+            const float4 u = U[(long long)((unsigned)(v >> 32) & 511u) * d4];
+            acc.x += p * u.x; acc.y += p * u.y; acc.z += p * u.z; acc.w += p * u.w;
+          }
+        }
+      };
+      auto put = [&](int from, const float4& acc, float pb) {
+        const long long item = item0 + (long long)(entry_s[from] >> 41);
+        if (on) {
+          float4* e = (float4*)a.d_table + item * d4 + t;
+          const float4 v = *e;
+          *e = make_float4(v.x - gs * acc.x, v.y - gs * acc.y, v.z - gs * acc.z, v.w - gs * acc.w);
+        }
+        if (t == 0 && a.d_bias) a.d_bias[item] -= gs * pb;
+      };
+      for (int r = grp; r < runs; r += G) {
+        const int from = run_s[r], to = run_s[r + 1];
+        if (to - from > LONG) {
+          if (t == 0) long_s[atomicAdd(&nlong_s, 1)] = (unsigned short)r;   // (their order is free: an item is its own sum)
+          continue;
+        }
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float pb = 0.f;
+        sum(from, to, 1, acc, pb);
+        put(from, acc, pb);
+      }
+      __syncthreads();
+      const int nl = nlong_s;
+      for (int q = 0; q < nl; ++q) {
+        const int from = run_s[long_s[q]], to = run_s[long_s[q] + 1];
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        float pb = 0.f;
+        sum(from + grp, to, G, acc, pb);
+        acc_s[tid] = acc;
+        if (t == 0) accp_s[grp] = pb;
+        __syncthreads();
+        if (grp == 0) {
+          for (int w = 1; w < G; ++w) {
+            const float4 v = acc_s[w * TPR + t];
+            acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+            pb += accp_s[w];
+          }
+          put(from, acc, pb);
+        }
+        __syncthreads();
+      }
+      __syncthreads();
     }
-    if (t == 0 && a.d_bias) a.d_bias[item] -= g * pb;
   }
 }
 
@@ -731,10 +924,18 @@ static void ds_splits(int B, int d, long long N, int* owner_blocks, int* splits,
   *splits = (int)s;
 }
 
+// items of a bucket of the lists, 2^shift: some 32 to 64 entries a bucket if ids were uniform, and no more buckets than a tile of users can
+// count in LDS.  (512 users x 100, 1 M items: buckets of 128 items left 7 a workgroup, 86 us of workgroups waiting for memory; 400 x 20, 1 682
+// items: 14 workgroups of 610, 21 us)
+static inline int ds_shift(long long N, long long entries) {
+  int s = 0;
+  while (s < 22 && ((entries << s) < 32 * N || ((N - 1) >> s) >= 8192)) ++s;
+  return s;
+}
 struct DistillWs {
-  float *part_m, *part_l, *part_o;                                   // forward
-  int *uniq, *seg, *pos, *n_uniq; char* plan;                       // backward
-  _Float16* img; float* rb_img; int* ky_img;                        // from the forward to the backward
+  float *part_m, *part_l, *part_o, *stat, *coef; int* tid;          // the forward's own
+  _Float16* img; float* rb_img; int* ky_img; int* offs; uint2* list; float* d_unit;   // from the forward to the backward
+  int buckets, shift;
   int64_t bytes;
 };
 static DistillWs ds_carve(int B, int d, long long N, int K, int grad, char* base) {
@@ -748,20 +949,19 @@ static DistillWs ds_carve(int B, int d, long long N, int K, int grad, char* base
   int ob, splits;
   long long per;
   ds_splits(B, d, N, &ob, &splits, &per);
+  w.shift = ds_shift(N, (long long)B * K);
+  w.buckets = (int)(((N - 1) >> w.shift) + 1);
   if (grad) {
     const int64_t ut = cdiv(B, DS_TILE);
     w.img = (_Float16*)take(ut * 4 * DS_TILE * ds_width(d)); w.rb_img = (float*)take(ut * DS_TILE * 4); w.ky_img = (int*)take(ut * 4);
+    w.offs = (int*)take(ut * (w.buckets + 1) * 4); w.list = (uint2*)take((int64_t)B * K * 8);
+    w.d_unit = (float*)take((int64_t)B * d * 4);
   }
-  const int64_t mark = o;
-  w.part_m = (float*)take((int64_t)splits * B * 4);
-  w.part_l = (float*)take((int64_t)splits * B * 4);
+  w.part_m = (float*)take((int64_t)splits * B * 4); w.part_l = (float*)take((int64_t)splits * B * 4);
+  w.stat = (float*)take((int64_t)B * 12);
   if (grad) {
     w.part_o = (float*)take((int64_t)splits * B * d * 4);
-    const int64_t n = (int64_t)B * K, fwd = o;
-    o = mark;                                                       // the backward reuses the forward's partials
-    w.uniq = (int*)take(n * 4); w.seg = (int*)take((n + 1) * 4); w.pos = (int*)take(n * 4); w.n_uniq = (int*)take(4);
-    w.plan = take(ur_rows_plan_workspace_bytes(n));
-    o = std::max(o, fwd);
+    w.coef = (float*)take((int64_t)B * K * 4); w.tid = (int*)take((int64_t)B * K * 4);
   }
   w.bytes = o;
   return w;
@@ -784,8 +984,8 @@ static int ds_launch_fwd(const DistillStream& a, bool grad, bool clip, int nw, i
 #undef GO
 }
 
-static int ds_check(const float* user_emb, const float* table, int64_t N, int B, int d, int K, float tau, float T, const char* who) {
-  UR_REQUIRE(user_emb && table, UR_ERR_ARG, "%s: null pointer", who);
+static int ds_check(const float* table, int64_t N, int B, int d, int K, float tau, float T, const char* who) {
+  UR_REQUIRE(table, UR_ERR_ARG, "%s: null pointer", who);
   UR_REQUIRE(B > 0 && d > 0 && d % 4 == 0 && N > 1 && N < (1LL << 31) && K > 0, UR_ERR_ARG, "%s: shape", who);
   UR_REQUIRE(d <= DS_MAX_D, UR_ERR_UNSUPPORTED, "%s: d=%d (at most %d)", who, d, DS_MAX_D);
   UR_REQUIRE((int64_t)B * K < (1LL << 31), UR_ERR_ARG, "%s: B * K = %lld", who, (long long)B * K);
@@ -804,16 +1004,14 @@ extern "C" int64_t ur_full_distill_workspace_bytes(int32_t B, int32_t d, int64_t
 
 extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_table, int64_t n_items, int32_t B, int32_t d,
                                    const int64_t* teacher_id, const void* teacher_score, int32_t score_type, int32_t K, const float* item_bias,
-                                   float tau, float score_clip, float temperature, float* lse, float* loss_out, float* row_stat, float* coef,
-                                   int64_t* entry_id, float* d_unit, void* ws, void* stream) {
+                                   float tau, float score_clip, float temperature, float* lse, float* loss_out, int32_t need_grad, void* ws,
+                                   void* stream) {
   UR_TRACE_SCOPE();
-  int rc = ds_check(user_emb, item_table, n_items, B, d, K, tau, temperature, "ur_full_distill_fwd");
+  int rc = ds_check(item_table, n_items, B, d, K, tau, temperature, "ur_full_distill_fwd");
   if (rc) return rc;
-  UR_REQUIRE(teacher_id && teacher_score && lse && loss_out && row_stat && ws, UR_ERR_ARG, "ur_full_distill_fwd: null pointer");
+  UR_REQUIRE(user_emb && teacher_id && teacher_score && lse && loss_out && ws, UR_ERR_ARG, "ur_full_distill_fwd: null pointer");
   UR_REQUIRE(score_type == UR_F32 || score_type == UR_F16 || score_type == UR_BF16, UR_ERR_ARG, "ur_full_distill_fwd: score_type=%d", score_type);
-  const bool grad = d_unit != nullptr;
-  UR_REQUIRE(grad == (coef != nullptr) && grad == (entry_id != nullptr), UR_ERR_ARG,
-             "ur_full_distill_fwd: coef, entry_id and d_unit go together (all of them for a backward pass, none without)");
+  const bool grad = need_grad != 0;
   hipStream_t st = as_stream(stream);
   ProfScope ps(PC_LOSS, st, (grad ? 4.0 : 2.0) * B * (double)n_items * d);
   const DistillWs w = ds_carve(B, d, n_items, K, grad, (char*)ws);
@@ -832,7 +1030,7 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   r.part_m = w.part_m; r.part_l = w.part_l; r.part_o = w.part_o;
   r.id = (const long long*)teacher_id; r.score = teacher_score; r.score_type = score_type; r.item_bias = item_bias;
   r.inv_tau = 1.f / tau; r.inv_T = 1.f / temperature; r.clip = score_clip;
-  r.lse = lse; r.stat = row_stat; r.coef = coef; r.tid = (long long*)entry_id; r.d_unit = d_unit; r.guard = id_guard();
+  r.lse = lse; r.stat = w.stat; r.coef = w.coef; r.tid = w.tid; r.d_unit = w.d_unit; r.guard = id_guard();
 #define GO(T) do { if (grad) hipLaunchKernelGGL((distill_row_kernel<T, true>), dim3(B), dim3(256), 0, st, r); \
                    else hipLaunchKernelGGL((distill_row_kernel<T, false>), dim3(B), dim3(256), 0, st, r); } while (0)
   switch (ds_tpr(d)) {
@@ -842,9 +1040,13 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   }
 #undef GO
   UR_LAUNCH_CHECK();
+  DistillLoss l{};
+  l.stat = w.stat; l.B = B; l.d = d; l.K = K; l.T2 = temperature * temperature; l.loss_out = loss_out; l.U = user_emb;
+  l.img = w.img; l.rb_img = w.rb_img; l.ky_img = w.ky_img; l.coef = w.coef; l.tid = w.tid;
+  l.buckets = w.buckets; l.shift = w.shift; l.offs = w.offs; l.list = w.list;
   const int tiles = grad ? cdiv(B, DS_TILE) : 0;
-#define GO(W) hipLaunchKernelGGL((distill_loss_kernel<W>), dim3(1 + tiles), dim3(256), 0, st, row_stat, B, temperature * temperature, loss_out, user_emb, d, \
-                                 w.img, w.rb_img, w.ky_img)
+  const size_t lds = grad ? (size_t)w.buckets * 4 : 0;
+#define GO(W) hipLaunchKernelGGL((distill_loss_kernel<W>), dim3(1 + tiles), dim3(256), lds, st, l)
   switch (ds_width(d)) {
     case 32: GO(32); break;
     case 64: GO(64); break;
@@ -856,19 +1058,16 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   return UR_OK;
 }
 
-extern "C" int ur_full_distill_bwd(const float* user_emb, const float* item_table, int64_t n_items, int32_t B, int32_t d, int32_t K,
-                                   const float* item_bias, float tau, float score_clip, float temperature, const float* loss_out,
-                                   const float* row_stat, const float* coef, const int64_t* entry_id, const float* d_unit, const float* d_loss,
-                                   float* d_user_emb, float* d_item_table, float* d_item_bias, void* ws, void* stream) {
+extern "C" int ur_full_distill_bwd(const float* user_emb, const float* item_table, int64_t n_items, int32_t B, int32_t d, int32_t K, const float* item_bias, float tau,
+                                   float score_clip, float temperature, const float* loss_out, const float* d_loss, float* d_user_emb,
+                                   float* d_item_table, float* d_item_bias, const void* ws, void* stream) {
   UR_TRACE_SCOPE();
-  int rc = ds_check(user_emb, item_table, n_items, B, d, K, tau, temperature, "ur_full_distill_bwd");
+  int rc = ds_check(item_table, n_items, B, d, K, tau, temperature, "ur_full_distill_bwd");
   if (rc) return rc;
-  UR_REQUIRE(loss_out && row_stat && coef && entry_id && d_unit && d_user_emb && d_item_table && ws, UR_ERR_ARG, "ur_full_distill_bwd: null pointer");
+  UR_REQUIRE(user_emb && loss_out && d_user_emb && d_item_table && ws, UR_ERR_ARG, "ur_full_distill_bwd: null pointer");
   UR_REQUIRE(!item_bias || d_item_bias, UR_ERR_ARG, "ur_full_distill_bwd: d_item_bias is required when item_bias is given");
   hipStream_t st = as_stream(stream);
   const DistillWs w = ds_carve(B, d, n_items, K, 1, (char*)ws);
-  rc = ur_rows_plan(nullptr, 0, entry_id, (int64_t)B * K, n_items, w.uniq, w.seg, w.pos, w.n_uniq, w.plan, stream);
-  if (rc) return rc;
   ProfScope ps(PC_LOSS, st, 4.0 * B * (double)n_items * d);
   DistillStream a{};
   a.X = item_table; a.nx = n_items; a.ny = B; a.d = d; a.img = w.img; a.rb_img = w.rb_img; a.ky_img = w.ky_img; a.x_bias = item_bias;
@@ -880,17 +1079,15 @@ extern "C" int ur_full_distill_bwd(const float* user_emb, const float* item_tabl
      : d <= 128 ? ds_launch_stream<128, 4, false, true>(a, clip, grid, st) : ds_launch_stream<256, 4, false, true>(a, clip, grid, st);
   if (rc) return rc;
   DistillApply p{};
-  p.uniq = w.uniq; p.seg = w.seg; p.pos = w.pos; p.n_uniq = w.n_uniq; p.coef = coef; p.U = user_emb; p.d_unit = d_unit;
+  p.offs = w.offs; p.list = w.list; p.buckets = w.buckets; p.shift = w.shift; p.U = user_emb; p.d_unit = w.d_unit;
   p.B = B; p.d = d; p.K = K; p.loss_out = loss_out; p.d_loss = d_loss; p.g_num = temperature / tau;
-  p.d_user = d_user_emb; p.d_table = d_item_table; p.d_bias = d_item_bias; p.user_blocks = cdiv((long long)B * (d / 4), 256);
-  const int tpr = ds_tpr(d), item_blocks = (int)std::min<int64_t>(cdiv((int64_t)B * K, 256 / tpr), 4096);
-#define GO(T) hipLaunchKernelGGL((distill_apply_kernel<T>), dim3(p.user_blocks + item_blocks), dim3(256), 0, st, p)
-  switch (tpr) {
-    case 16: GO(16); break;
-    case 32: GO(32); break;
-    default: GO(64); break;
+  p.d_user = d_user_emb; p.d_table = d_item_table; p.d_bias = d_item_bias;
+  const int blocks = w.buckets + cdiv((long long)B * (d / 4), 128);
+  switch (ds_tpr(d)) {
+    case 16: hipLaunchKernelGGL((distill_apply_kernel<16>), dim3(blocks), dim3(128), 0, st, p); break;
+    case 32: hipLaunchKernelGGL((distill_apply_kernel<32>), dim3(blocks), dim3(128), 0, st, p); break;
+    default: hipLaunchKernelGGL((distill_apply_kernel<64>), dim3(blocks), dim3(128), 0, st, p); break;
   }
-#undef GO
   UR_LAUNCH_CHECK();
   return UR_OK;
 }

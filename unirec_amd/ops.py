@@ -841,8 +841,11 @@ def full_softmax_bwd_shard(user_emb_all, shard_rows, target_row, lse, ws, d_shar
 
 # --------------------------------------------------------------------------------------------- distillation from a teacher's top logits
 class DistillSaved:
-    """What a full_distill_fwd(need_grad=True) leaves for its full_distill_bwd (all device tensors)."""
-    __slots__ = ("row_stat", "coef", "entry_id", "d_unit", "ws")
+    """What a full_distill_fwd(need_grad=True) leaves for its full_distill_bwd: a device buffer, and the sizes (B, d, N, K) it was made for."""
+    __slots__ = ("ws", "sizes")
+
+    def __init__(self, ws, sizes):
+        self.ws, self.sizes = ws, sizes
 
 
 def _distill_check(who, user_emb, item_table, item_bias, tau, temperature):
@@ -884,17 +887,12 @@ def full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias=
     id_guard_check()
     f32 = dict(dtype=torch.float32, device=dev)
     lse, loss_out = torch.empty(B, **f32), torch.empty(4, **f32)
-    sv = DistillSaved()
-    sv.row_stat = torch.empty(3 * B, **f32)
-    sv.coef = torch.empty(B, K, **f32) if need_grad else None
-    sv.entry_id = torch.empty(B, K, dtype=torch.int64, device=dev) if need_grad else None
-    sv.d_unit = torch.empty(B, d, **f32) if need_grad else None
-    sv.ws = torch.empty(check(lib.ur_full_distill_workspace_bytes(B, d, N, K, int(need_grad)), "ur_full_distill_workspace_bytes"),
-                        dtype=torch.uint8, device=dev)
+    ws = torch.empty(check(lib.ur_full_distill_workspace_bytes(B, d, N, K, int(need_grad)), "ur_full_distill_workspace_bytes"),
+                     dtype=torch.uint8, device=dev)
     check(lib.ur_full_distill_fwd(_p(user_emb), _p(item_table), N, B, d, _p(teacher_id), _p(teacher_score), _lib.DTYPE_IDS[teacher_score.dtype], K,
                                   _p(item_bias), float(tau), float(score_clip if score_clip else -1.0), float(temperature), _p(lse), _p(loss_out),
-                                  _p(sv.row_stat), _p(sv.coef), _p(sv.entry_id), _p(sv.d_unit), _p(sv.ws), _stream()), "ur_full_distill_fwd")
-    return loss_out, lse, (sv if need_grad else None)
+                                  int(need_grad), _p(ws), _stream()), "ur_full_distill_fwd")
+    return loss_out, lse, (DistillSaved(ws, (B, d, N, K)) if need_grad else None)
 
 
 def full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, saved, item_bias=None, tau=1.0, score_clip=-1.0, temperature=1.0, d_loss=None):
@@ -904,15 +902,16 @@ def full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, saved, ite
     _distill_check(who, user_emb, item_table, item_bias, tau, temperature)
     _chk(d_loss, torch.float32, "d_loss", allow_none=True)
     B, d = user_emb.shape
-    if saved is None or saved.d_unit.shape != user_emb.shape or saved.coef.shape != teacher_id.shape or loss_out.numel() != 4 or lse.numel() != B:
-        raise _lib.UnirecAmdError(f"{who}: not the results of a full_distill_fwd(need_grad=True) of these inputs")
     K, N, dev = teacher_id.shape[1], item_table.shape[0], user_emb.device
+    if saved is None or saved.sizes != (B, d, N, K) or loss_out.numel() != 4 or lse.numel() != B:
+        raise _lib.UnirecAmdError(f"{who}: not the results of a full_distill_fwd(need_grad=True) of these inputs")
+    _same_device(who, loss_out, saved.ws, d_loss)
     d_user = torch.empty(B, d, dtype=torch.float32, device=dev)
     d_table = torch.empty(N, d, dtype=torch.float32, device=dev)
     d_ib = torch.empty(N, dtype=torch.float32, device=dev) if item_bias is not None else None
     check(lib.ur_full_distill_bwd(_p(user_emb), _p(item_table), N, B, d, K, _p(item_bias), float(tau), float(score_clip if score_clip else -1.0),
-                                  float(temperature), _p(loss_out), _p(saved.row_stat), _p(saved.coef), _p(saved.entry_id), _p(saved.d_unit),
-                                  _p(d_loss), _p(d_user), _p(d_table), _p(d_ib), _p(saved.ws), _stream()), "ur_full_distill_bwd")
+                                  float(temperature), _p(loss_out), _p(d_loss), _p(d_user), _p(d_table), _p(d_ib), _p(saved.ws), _stream()),
+          "ur_full_distill_bwd")
     return d_user, d_table, d_ib
 
 

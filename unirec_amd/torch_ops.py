@@ -322,33 +322,33 @@ def _(user_emb, item_table, k, user_id, hist_ptr, hist_sorted, user_bias, item_b
 # ------------------------------------------------------------------------------------------------ distillation from a teacher's top logits
 @custom_op(f"{NS}::full_distill_fwd", mutates_args=())
 def full_distill_fwd(user_emb: torch.Tensor, item_table: torch.Tensor, teacher_id: torch.Tensor, teacher_score: torch.Tensor,
-                     item_bias: Optional[torch.Tensor], tau: float = 1.0, score_clip: float = -1.0, temperature: float = 1.0) -> Tuple[
-                         torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
-    """-> (loss_out, lse, row_stat, coef, entry_id, d_unit, ws): the last five are full_distill_bwd's"""
+                     item_bias: Optional[torch.Tensor], tau: float = 1.0, score_clip: float = -1.0,
+                     temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """-> (loss_out, lse, ws): full_distill_bwd's"""
     loss_out, lse, sv = ops.full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias, tau, score_clip, temperature)
-    return loss_out, lse, sv.row_stat, sv.coef, sv.entry_id, sv.d_unit, sv.ws
+    return loss_out, lse, sv.ws
 
 
 @full_distill_fwd.register_fake
 def _(user_emb, item_table, teacher_id, teacher_score, item_bias, tau=1.0, score_clip=-1.0, temperature=1.0):
-    B = user_emb.shape[0]
-    return (user_emb.new_empty((4,)), user_emb.new_empty((B,)), user_emb.new_empty((3 * B,)), user_emb.new_empty(teacher_id.shape),
-            torch.empty_like(teacher_id), torch.empty_like(user_emb), user_emb.new_empty((torch.library.get_ctx().new_dynamic_size(),), dtype=torch.uint8))
+    return (user_emb.new_empty((4,)), user_emb.new_empty((user_emb.shape[0],)),
+            user_emb.new_empty((torch.library.get_ctx().new_dynamic_size(),), dtype=torch.uint8))
 
 
-@custom_op(f"{NS}::full_distill_bwd", mutates_args=("ws",))
-def full_distill_bwd(user_emb: torch.Tensor, item_table: torch.Tensor, loss_out: torch.Tensor, lse: torch.Tensor, row_stat: torch.Tensor,
-                     coef: torch.Tensor, entry_id: torch.Tensor, d_unit: torch.Tensor, ws: torch.Tensor, d_loss: Optional[torch.Tensor],
-                     item_bias: Optional[torch.Tensor], tau: float = 1.0, score_clip: float = -1.0,
-                     temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    sv = ops.DistillSaved()
-    sv.row_stat, sv.coef, sv.entry_id, sv.d_unit, sv.ws = row_stat, coef, entry_id, d_unit, ws
-    d_user, d_table, d_ib = ops.full_distill_bwd(user_emb, item_table, entry_id, lse, loss_out, sv, item_bias, tau, score_clip, temperature, d_loss)
+@custom_op(f"{NS}::full_distill_bwd", mutates_args=())
+def full_distill_bwd(user_emb: torch.Tensor, item_table: torch.Tensor, teacher_id: torch.Tensor, loss_out: torch.Tensor, lse: torch.Tensor,
+                     ws: torch.Tensor, d_loss: Optional[torch.Tensor], item_bias: Optional[torch.Tensor], tau: float = 1.0,
+                     score_clip: float = -1.0, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    sizes = (user_emb.shape[0], user_emb.shape[1], item_table.shape[0], teacher_id.shape[1])
+    if ws.dtype != torch.uint8 or ws.numel() != ops.check(ops.lib.ur_full_distill_workspace_bytes(sizes[0], sizes[1], sizes[2], sizes[3], 1), "ws"):
+        raise ops._lib.UnirecAmdError("full_distill_bwd: ws is not that of a full_distill_fwd of these sizes")
+    sv = ops.DistillSaved(ws, sizes)
+    d_user, d_table, d_ib = ops.full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, sv, item_bias, tau, score_clip, temperature, d_loss)
     return d_user, d_table, d_ib if d_ib is not None else user_emb.new_empty((0,))
 
 
 @full_distill_bwd.register_fake
-def _(user_emb, item_table, loss_out, lse, row_stat, coef, entry_id, d_unit, ws, d_loss, item_bias, tau=1.0, score_clip=-1.0, temperature=1.0):
+def _(user_emb, item_table, teacher_id, loss_out, lse, ws, d_loss, item_bias, tau=1.0, score_clip=-1.0, temperature=1.0):
     return torch.empty_like(user_emb), torch.empty_like(item_table), user_emb.new_empty((item_table.shape[0] if item_bias is not None else 0,))
 
 
