@@ -18,7 +18,6 @@
 #include <type_traits>
 
 #include "common.h"
-#include "kernels.h"
 
 namespace ur {
 
@@ -924,12 +923,12 @@ static void ds_splits(int B, int d, long long N, int* owner_blocks, int* splits,
   *splits = (int)s;
 }
 
-// items of a bucket of the lists, 2^shift: some 32 to 64 entries a bucket if ids were uniform, and no more buckets than a tile of users can
+// items of a bucket of the lists, 2^shift: some 8 to 16 entries a bucket if ids were uniform (32 to 64: 512 x 60 K 103 us, these 100), and no more buckets than a tile of users can
 // count in LDS.  (512 users x 100, 1 M items: buckets of 128 items left 7 a workgroup, 86 us of workgroups waiting for memory; 400 x 20, 1 682
 // items: 14 workgroups of 610, 21 us)
 static inline int ds_shift(long long N, long long entries) {
   int s = 0;
-  while (s < 22 && ((entries << s) < 32 * N || ((N - 1) >> s) >= 8192)) ++s;
+  while (s < 22 && ((entries << s) < 8 * N || ((N - 1) >> s) >= 8192)) ++s;
   return s;
 }
 struct DistillWs {
@@ -982,6 +981,15 @@ static int ds_launch_fwd(const DistillStream& a, bool grad, bool clip, int nw, i
   }
   return nw == 1 ? GO(1) : nw == 2 ? GO(2) : GO(4);
 #undef GO
+}
+
+// waves of a workgroup of the backward, 32 items each: one where four would leave most compute units without a workgroup (1 682 items, 400
+// users: step of 55.3 us with one, 57.6 with four; 20 011 items, 333 users: 65.4 and 65.9, and two waves 70.7, so no size takes two)
+static inline int ds_nw_bwd(long long N) { return N <= 256 * 32 ? 1 : 4; }
+template <int D>
+static int ds_launch_bwd(const DistillStream& a, bool clip, hipStream_t st) {
+  const int nw = ds_nw_bwd(a.nx), grid = cdiv(a.nx, 32 * nw);
+  return nw == 1 ? ds_launch_stream<D, 1, false, true>(a, clip, grid, st) : ds_launch_stream<D, 4, false, true>(a, clip, grid, st);
 }
 
 static int ds_check(const float* table, int64_t N, int B, int d, int K, float tau, float T, const char* who) {
@@ -1074,9 +1082,8 @@ extern "C" int ur_full_distill_bwd(const float* user_emb, const float* item_tabl
   a.cz = DS_LOG2E / (tau * temperature); a.clip2 = score_clip > 0.f ? score_clip / temperature * DS_LOG2E : 0.f;
   a.loss_out = loss_out; a.d_loss = d_loss; a.g_num = temperature / tau; a.dX = d_item_table; a.d_bias = d_item_bias;
   const bool clip = score_clip > 0.f;
-  const int grid = cdiv(n_items, 128);
-  rc = d <= 32 ? ds_launch_stream<32, 4, false, true>(a, clip, grid, st) : d <= 64 ? ds_launch_stream<64, 4, false, true>(a, clip, grid, st)
-     : d <= 128 ? ds_launch_stream<128, 4, false, true>(a, clip, grid, st) : ds_launch_stream<256, 4, false, true>(a, clip, grid, st);
+  rc = d <= 32 ? ds_launch_bwd<32>(a, clip, st) : d <= 64 ? ds_launch_bwd<64>(a, clip, st)
+     : d <= 128 ? ds_launch_bwd<128>(a, clip, st) : ds_launch_bwd<256>(a, clip, st);
   if (rc) return rc;
   DistillApply p{};
   p.offs = w.offs; p.list = w.list; p.buckets = w.buckets; p.shift = w.shift; p.U = user_emb; p.d_unit = w.d_unit;
