@@ -565,27 +565,46 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
   float4 u = make_float4(0.f, 0.f, 0.f, 0.f), acc = u;
   if (on) u = ((const float4*)a.U)[(long long)b * d4 + t];
   float loss = 0.f;
-  for (int k = g; k < a.K; k += G) {
-    const long long i = (long long)b * a.K + k, id = a.id[i];
-    const float v = teacher_at(a.score, a.score_type, i) * a.inv_T;
-    const bool there = some && id >= 1 && id < a.N && v > -INFINITY;
-    float p = 0.f;
-    if (there) {
-      float4 e = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (on) e = ((const float4*)a.E)[id * d4 + t];
-      const float dot = group_sum<TPR>((u.x * e.x + u.y * e.y) + (u.z * e.z + u.w * e.w));
-      float s = (dot + (a.item_bias ? a.item_bias[id] : 0.f)) * a.inv_tau;
-      const bool cut = a.clip > 0.f && (s > a.clip || s < -a.clip);
-      if (cut) s = s > 0.f ? a.clip : -a.clip;
-      const float logp = v - tm - log_ts;
-      p = expf(logp);
-      if (t == 0) loss += p * (logp - s * a.inv_T + lse);
-      if (cut) p = 0.f;
-      acc.x -= p * e.x; acc.y -= p * e.y; acc.z -= p * e.z; acc.w -= p * e.w;
+  constexpr int AHEAD = 4;                                       // rows of a group under way at once
+  for (int k0 = g; k0 < a.K; k0 += AHEAD * G) {
+    long long id[AHEAD];
+    float v[AHEAD], bias[AHEAD];
+    bool there[AHEAD];
+    float4 e[AHEAD];
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = k0 + j * G;
+      const long long i = (long long)b * a.K + min(k, a.K - 1);
+      id[j] = a.id[i];
+      v[j] = teacher_at(a.score, a.score_type, i) * a.inv_T;
+      there[j] = k < a.K && some && id[j] >= 1 && id[j] < a.N && v[j] > -INFINITY;
     }
-    if (GRAD && t == 0) {
-      a.coef[i] = p;
-      a.tid[i] = there ? (int)id : 0;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      e[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      bias[j] = 0.f;
+      if (there[j] && on) e[j] = ((const float4*)a.E)[id[j] * d4 + t];
+      if (there[j] && a.item_bias) bias[j] = a.item_bias[id[j]];
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const int k = k0 + j * G;
+      float p = 0.f;
+      if (there[j]) {
+        const float dot = group_sum<TPR>((u.x * e[j].x + u.y * e[j].y) + (u.z * e[j].z + u.w * e[j].w));
+        float s = (dot + bias[j]) * a.inv_tau;
+        const bool cut = a.clip > 0.f && (s > a.clip || s < -a.clip);
+        if (cut) s = s > 0.f ? a.clip : -a.clip;
+        const float logp = v[j] - tm - log_ts;
+        p = expf(logp);
+        if (t == 0) loss += p * (logp - s * a.inv_T + lse);
+        if (cut) p = 0.f;
+        acc.x -= p * e[j].x; acc.y -= p * e[j].y; acc.z -= p * e[j].z; acc.w -= p * e[j].w;
+      }
+      if (GRAD && t == 0 && k < a.K) {
+        a.coef[(long long)b * a.K + k] = p;
+        a.tid[(long long)b * a.K + k] = there[j] ? (int)id[j] : 0;
+      }
     }
   }
   loss = ds_block_sum(loss, red);
@@ -626,6 +645,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
         coef[k] = p;
       }
     }
+#pragma unroll 8
     for (int s = g; s < a.splits; s += G) {
       const long long at = (long long)s * a.B + b;
       const float f = exp2f(a.part_m[at] - lse2);
@@ -654,9 +674,9 @@ struct DistillLoss {
   const float* coef; const int* tid; int buckets, shift; int* offs; uint2* list;
 };
 // Workgroup 0: loss_out = [T^2 / C sum of the rows' losses, C, update guard, -] (fixed order).  The others (a forward pass that will be
-// followed by a backward): what the backward needs of a tile of 32 users.  Its image, that every workgroup streams: one exponent, [hi | lo][32][D]
-// halves in the swizzled order, the row biases -log2(softmax sum) (-inf without a teacher and behind the last user).  And its teacher's
-// entries (item - first item of the bucket, user; p) by bucket of 2^shift items, a counting sort in LDS: the order inside a bucket is free.
+// followed by a backward), two for a tile of 32 users, leave what the backward needs of it.  One the image that every workgroup streams: one
+// exponent, [hi | lo][32][D] halves in the swizzled order, the row biases -log2(softmax sum) (-inf without a teacher and behind the last user).
+// The other its teacher's entries (item - first item of the bucket, user; p) by bucket of 2^shift items, a counting sort in LDS: the order inside a bucket is free.
 template <int D>
 __global__ __launch_bounds__(256) void distill_loss_kernel(DistillLoss a) {
   __shared__ float red[4];
@@ -680,33 +700,36 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillLoss a) {
     }
     return;
   }
-  constexpr int F4 = D / 4, PER = DS_TILE * F4 / 256;
-  const int tile = blockIdx.x - 1;
-  float4 v[PER];
-  float mx = 0.f;
+  const int tile = (blockIdx.x - 1) >> 1;
+  if (blockIdx.x & 1) {
+    constexpr int F4 = D / 4, PER = DS_TILE * F4 / 256;
+    float4 v[PER];
+    float mx = 0.f;
 #pragma unroll
-  for (int p = 0; p < PER; ++p) {
-    const int i = threadIdx.x + 256 * p, b = tile * DS_TILE + i / F4, c = (i % F4) * 4;
-    v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (b < B && c < d) v[p] = *(const float4*)(a.U + (long long)b * d + c);
-    mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(v[p].x), finite_abs(v[p].y)), fmaxf(finite_abs(v[p].z), finite_abs(v[p].w))));
-  }
-  const int ky = group_exponent(ds_block_max(mx, red));
-  const float up = pow2i(ky);
-  _Float16* out = a.img + (long long)tile * 2 * DS_TILE * D;
+    for (int p = 0; p < PER; ++p) {
+      const int i = threadIdx.x + 256 * p, b = tile * DS_TILE + i / F4, c = (i % F4) * 4;
+      v[p] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (b < B && c < d) v[p] = *(const float4*)(a.U + (long long)b * d + c);
+      mx = fmaxf(mx, fmaxf(fmaxf(finite_abs(v[p].x), finite_abs(v[p].y)), fmaxf(finite_abs(v[p].z), finite_abs(v[p].w))));
+    }
+    const int ky = group_exponent(ds_block_max(mx, red));
+    const float up = pow2i(ky);
+    _Float16* out = a.img + (long long)tile * 2 * DS_TILE * D;
 #pragma unroll
-  for (int p = 0; p < PER; ++p) {
-    const int i = threadIdx.x + 256 * p, at = ds_at<D>(i / F4, (i % F4) * 4);
-    half2_t h0, h1, l0, l1;
-    split_pair(v[p].x, v[p].y, up, h0, l0);
-    split_pair(v[p].z, v[p].w, up, h1, l1);
-    *(half4*)(out + at) = (half4){h0[0], h0[1], h1[0], h1[1]};
-    *(half4*)(out + DS_TILE * D + at) = (half4){l0[0], l0[1], l1[0], l1[1]};
-  }
-  if (tid == 0) a.ky_img[tile] = ky;
-  if (tid < DS_TILE) {
-    const int b = tile * DS_TILE + tid;
-    a.rb_img[b] = b < B ? -stat[2 * (long long)B + b] : -INFINITY;
+    for (int p = 0; p < PER; ++p) {
+      const int i = threadIdx.x + 256 * p, at = ds_at<D>(i / F4, (i % F4) * 4);
+      half2_t h0, h1, l0, l1;
+      split_pair(v[p].x, v[p].y, up, h0, l0);
+      split_pair(v[p].z, v[p].w, up, h1, l1);
+      *(half4*)(out + at) = (half4){h0[0], h0[1], h1[0], h1[1]};
+      *(half4*)(out + DS_TILE * D + at) = (half4){l0[0], l0[1], l1[0], l1[1]};
+    }
+    if (tid == 0) a.ky_img[tile] = ky;
+    if (tid < DS_TILE) {
+      const int b = tile * DS_TILE + tid;
+      a.rb_img[b] = b < B ? -stat[2 * (long long)B + b] : -INFINITY;
+    }
+    return;
   }
   // ---- the lists
   const int rows = min(DS_TILE, B - tile * DS_TILE);
@@ -716,10 +739,23 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillLoss a) {
   const float* coef = a.coef + e0;
   for (int i = tid; i < a.buckets; i += 256) count_s[i] = 0u;
   __syncthreads();
-#pragma unroll 4
-  for (unsigned i = tid; i < n; i += 256) {
-    const int item = items[i];
-    if (item > 0 && coef[i] != 0.f) atomicAdd(&count_s[item >> a.shift], 1u);
+  constexpr int AHEAD = 8;                                       // entries of a thread under way at once
+  int item[AHEAD];
+  float p[AHEAD];
+  auto fetch = [&](unsigned i0) {
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      const unsigned i = i0 + tid + 256u * j;
+      item[j] = i < n ? items[i] : 0;
+      p[j] = i < n ? coef[i] : 0.f;
+    }
+  };
+  const unsigned batch = 256u * AHEAD;
+  for (unsigned i0 = 0; i0 < n; i0 += batch) {
+    fetch(i0);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (item[j] > 0 && p[j] != 0.f) atomicAdd(&count_s[item[j] >> a.shift], 1u);
   }
   __syncthreads();
   const int per = (a.buckets + 255) / 256, i0 = min(a.buckets, tid * per), i1 = min(a.buckets, i0 + per);
@@ -747,12 +783,13 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillLoss a) {
   if (tid == 255) offs[a.buckets] = (int)at;
   __syncthreads();
   uint2* list = a.list + e0;
-#pragma unroll 4
-  for (unsigned i = tid; i < n; i += 256) {
-    const int item = items[i];
-    const float p = coef[i];
-    if (item > 0 && p != 0.f)
-      list[atomicAdd(&count_s[item >> a.shift], 1u)] = make_uint2(((unsigned)item & ((1u << a.shift) - 1u)) << 5 | i / (unsigned)a.K, __float_as_uint(p));
+  for (unsigned i0 = 0; i0 < n; i0 += batch) {
+    if (n > batch) fetch(i0);                                    // (else they are still at hand)
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (item[j] > 0 && p[j] != 0.f)
+        list[atomicAdd(&count_s[item[j] >> a.shift], 1u)] =
+            make_uint2(((unsigned)item[j] & ((1u << a.shift) - 1u)) << 5 | (i0 + tid + 256u * j) / (unsigned)a.K, __float_as_uint(p[j]));
   }
 }
 
@@ -1054,7 +1091,7 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   l.buckets = w.buckets; l.shift = w.shift; l.offs = w.offs; l.list = w.list;
   const int tiles = grad ? cdiv(B, DS_TILE) : 0;
   const size_t lds = grad ? (size_t)w.buckets * 4 : 0;
-#define GO(W) hipLaunchKernelGGL((distill_loss_kernel<W>), dim3(1 + tiles), dim3(256), lds, st, l)
+#define GO(W) hipLaunchKernelGGL((distill_loss_kernel<W>), dim3(1 + 2 * tiles), dim3(256), lds, st, l)
   switch (ds_width(d)) {
     case 32: GO(32); break;
     case 64: GO(64); break;
