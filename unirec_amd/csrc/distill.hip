@@ -560,7 +560,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
     if (id >= 1 && id < a.N && v > -INFINITY) ts += expf(v - tm);
   }
   ts = ds_block_sum(ts, red);
-  const float log_ts = logf(ts);
+  const float log_ts = logf(ts), inv_ts = 1.f / ts;
   // ---- its rows
   float4 u = make_float4(0.f, 0.f, 0.f, 0.f), acc = u;
   if (on) u = ((const float4*)a.U)[(long long)b * d4 + t];
@@ -596,7 +596,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
         const bool cut = a.clip > 0.f && (s > a.clip || s < -a.clip);
         if (cut) s = s > 0.f ? a.clip : -a.clip;
         const float logp = v[j] - tm - log_ts;
-        p = expf(logp);
+        p = expf(v[j] - tm) * inv_ts;                            // (not exp(logp): log_ts is rounded, once for all of the row)
         if (t == 0) loss += p * (logp - s * a.inv_T + lse);
         if (cut) p = 0.f;
         acc.x -= p * e[j].x; acc.y -= p * e[j].y; acc.z -= p * e[j].z; acc.w -= p * e[j].w;
