@@ -148,7 +148,7 @@ def test_steps_follow_dense_adam():
     tr.optimizer.flush()
     # (Adam divides by sqrt(v): where a gradient is close to zero its sign decides a whole step of 1e-3, so the tables are compared in the mean)
     for t, ref in ((m.user_embedding, U), (m.item_embedding, E)):
-        assert float((t.weight.double().cpu() - ref).abs().mean()) <= 2e-6
+        assert (t.weight.detach().double().cpu() - ref.detach()).abs().mean() <= 2e-6
     given = dict(batches[0], teacher_id=ids, teacher_score=score)   # a batch that brings its own list
     tr.teacher = None
     assert math.isfinite(float(tr.train_step(given)))
