@@ -946,7 +946,10 @@ __global__ __launch_bounds__(128) void distill_apply_kernel(DistillApply a) {
 }
 
 static inline int ds_tpr(int d) { return d <= 64 ? 16 : d <= 128 ? 32 : 64; }
-static inline int ds_nw(int B, int d) { return B <= 32 ? 1 : B <= 64 ? 2 : B <= 128 || d <= 32 || d > 128 ? 4 : 8; }
+// waves of a workgroup of the forward, 32 users each, the stream's tiles staged once for all of them.  Eight where they have users (512 x 60 K,
+// d 64: 49.8 us with eight, 50.7 with four) and registers; else four, also where some have none: 16 x 500 K, d 128: 147 us with four, 218 with
+// one, 182 with eight; 64 x 500 K: 151, 163 with two, 180 with eight; 128 x 500 K: 157 and 182
+static inline int ds_nw(int B, int d) { return B <= 128 || d <= 32 || d > 128 ? 4 : 8; }
 static inline int ds_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
 static void ds_splits(int B, int d, long long N, int* owner_blocks, int* splits, long long* per) {
@@ -1016,7 +1019,7 @@ static int ds_launch_fwd(const DistillStream& a, bool grad, bool clip, int nw, i
   if constexpr (D == 64 || D == 128) {
     if (nw == 8) return GO(8);
   }
-  return nw == 1 ? GO(1) : nw == 2 ? GO(2) : GO(4);
+  return GO(4);
 #undef GO
 }
 
