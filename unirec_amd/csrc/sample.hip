@@ -813,6 +813,18 @@ __device__ __forceinline__ FourX four_scores(const SampleArgs& a, long long base
   }
   return r;
 }
+// a workgroup's bins added to the row's, up to nine adds of a thread under way.  Every thread waits for its adds' old values: an add without one
+// may still be on its way when the barrier in front of the arrival is passed (that barrier waits for LDS, the arrival for its own wave only), and the
+// workgroup that arrives last would read, and clear, bins that lack it
+template <int FIRST = 0, typename T>
+__device__ __forceinline__ void add_bins(const T* mine, T* row) {
+  const int i = (int)threadIdx.x + FIRST;
+  const T v = i < SBP ? mine[i] : (T)0;
+  T old = 0;
+  if (v) old = __hip_atomic_fetch_add(row + i, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if constexpr (FIRST + 256 < SBP) add_bins<FIRST + 256>(mine, row);
+  asm volatile("" ::"v"(old));
+}
 // the top-k (PHASE 0) or top-p (PHASE 1) selection: counts (and weights) of the steps; the workgroup that arrives last finds the border's step
 // and clears the bins
 template <int PHASE, int TYPE>
@@ -877,10 +889,8 @@ __global__ __launch_bounds__(256) void sample_steps_kernel(SampleArgs a, SampleL
   }
   if (PHASE == 1 && blockIdx.x == 0 && tid == 0 && kc.cut != 0u && kc.ties != 0u) count(above, kc.ties);
   __syncthreads();
-  for (int i = tid; i < SBP; i += 256) {
-    if constexpr (PHASE == 0) { if (hc[i]) atomicAdd(&ghc[i], hc[i]); }
-    else { if (hw[i]) atomicAdd(&ghw[i], hw[i]); }
-  }
+  if constexpr (PHASE == 0) add_bins(hc, ghc);
+  else add_bins(hw, ghw);
   __syncthreads();
   if (tid == 0) last = ur_arrive(&S->arrived, mode) == (unsigned)g.nchunk - 1u;
   __syncthreads();
