@@ -96,7 +96,7 @@ __device__ __forceinline__ u64 exp2_fixed(double z) {
 }
 // a row's parameters
 struct SampleRow {
-  double scale, inv_T, p, min_z; long long k; int type; bool greedy, flat;   // scale: log2(e) / T
+  double scale, inv_T, p, min_z; long long k; int type; bool greedy, tiny, flat;   // scale: log2(e) / T
   float m;
   __device__ __forceinline__ void load(const SampleArgs& a, int b) {
     const double T = a.T_rows ? (double)a.T_rows[b] : a.T;
@@ -105,13 +105,14 @@ struct SampleRow {
     k = a.k_rows ? a.k_rows[b] : a.top_k;
     type = a.type;
     if (k <= 0) k = a.N;
-    greedy = !(T > 1e-300);              // (1 / T stays finite)
-    inv_T = greedy ? 1.0 : 1.0 / T;
-    scale = greedy ? 1.0 : 1.4426950408889634 / T;
+    greedy = !(T > 0.0);                 // the first of the largest
+    tiny = !(T > 1e-300);                // (1 / T stays finite) nothing but the largest has weight: two floats differ by 1e-45 at least
+    inv_T = tiny ? 1.0 : 1.0 / T;
+    scale = tiny ? 1.0 : 1.4426950408889634 / T;
     if (!(min_p < 1.0)) min_p = 1.0;     // (the largest stays)
     min_z = min_p > 0.0 ? log2(min_p) : -INFINITY;
   }
-  __device__ __forceinline__ void set_max(unsigned key) { m = key_value(key, type); flat = greedy || m == INFINITY; }
+  __device__ __forceinline__ void set_max(unsigned key) { m = key_value(key, type); flat = tiny || m == INFINITY; }
   __device__ __forceinline__ double z(unsigned key) const {
     const float x = key_value(key, type);
     if (flat) return x == m ? 0.0 : -INFINITY;
