@@ -146,6 +146,9 @@ struct SampleRow {
 // entries above `cut` stay, and of those equal to it the first `ties` in index order
 struct SampleCut { unsigned cut; unsigned ties; };
 constexpr unsigned ALL_TIES = 0xFFFFFFFFu;
+__device__ __forceinline__ SampleCut inside(SampleCut c, SampleCut outer) {   // a cut made among what `outer` left never lets more in: ties that all
+  return c.cut < outer.cut ? outer : c;                                        // stay are those that `outer` left of them, not all of the row's
+}
 __device__ __forceinline__ SampleCut above_min_p(SampleCut c, unsigned min_key) {   // and what min-p leaves of them
   return min_key > 1u && min_key > c.cut ? SampleCut{min_key - 1u, 0u} : c;
 }
@@ -627,7 +630,7 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
         }
         direct_p(near_k, near_w, (int)s_n, &st, &cut_s);
       }
-      c = cut_s;
+      c = inside(cut_s, c);
       __syncthreads();
     }
   }
@@ -1013,7 +1016,7 @@ __global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, Sampl
     else pick_p<NT>(round, round == rounds - 1, hc, hw, r.p, &st, &cut, tmp64);
   }
   if (tid == 0) {
-    S->cut = cut;
+    S->cut = inside(cut, kc);
     if (PHASE == 0) S->kcut = cut;
   }
 }
