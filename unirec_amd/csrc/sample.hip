@@ -9,8 +9,9 @@
 // comparing up to 128 keys directly, or by radix selection over 11, 11 and 10 bits of the key.
 //
 // Arithmetic.  Which entry a sum's border falls on is a whole number, so sums are exact: a weight is exp in double, rounded down
-// once to a multiple of 2^-57 (2^-53 is a double's own step) and added as integers: 64 of them in 64 bits, more in two 32-bit limbs (the
-// top-p selection sums multiples of 2^-(63 - log2 N) in 64 bits).  No result depends on an order of additions or on how a row was cut into pieces.
+// once to a multiple of 2^-57 (2^-53 is a double's own step) and added as integers: 64 of them in 64 bits, more in two limbs.  (With top-p's sums
+// in 64 bits, log2 N - 6 bits of every weight dropped, the border came out up to 900 entries off among a million equal ones 22 T below one.)  No
+// result depends on an order of additions or on how a row was cut into pieces.
 //
 // Two forms.  A row that fits into LDS (32 768 entries; 65 536 of 16 bits): one workgroup, one read of the row, every pass from LDS.
 // Longer rows: many workgroups a row, a pass over memory each for the maximum, for a selection's histogram and its border's step, and for the
@@ -174,6 +175,9 @@ __device__ __forceinline__ T wave_upto(T v) {
   v += dpp_from<0x143, 0xC>(v);
   return v;
 }
+__device__ __forceinline__ u64 at_lane(u64 v, int lane) {
+  return ((u64)(unsigned)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, lane);
+}
 __device__ __forceinline__ unsigned last_lane(unsigned v) { return (unsigned)__builtin_amdgcn_readlane((int)v, 63); }
 __device__ __forceinline__ u64 last_lane(u64 v) { return ((u64)last_lane((unsigned)(v >> 32)) << 32) | last_lane((unsigned)v); }
 template <typename T>
@@ -202,13 +206,32 @@ __device__ __forceinline__ T block_before(T v, T* tmp, T* total) {
   return base + s - v;
 }
 template <int NT>
-__device__ __forceinline__ WSum block_before(const WSum& v, u64* tmp, WSum* total) {
-  WSum r;
-  r.hi = block_before<NT>(v.hi, tmp, &total->hi);
-  r.lo = block_before<NT>(v.lo, tmp, &total->lo);
+__device__ __forceinline__ WSum block_before(const WSum& v, u64* tmp, WSum* total) {   // tmp[2 NT / 64]: both limbs between the same two barriers
+  constexpr int NW = NT / 64;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const WSum s{wave_upto(v.hi), wave_upto(v.lo)};
+  __syncthreads();
+  if (lane == 63) { tmp[wave] = s.hi; tmp[NW + wave] = s.lo; }
+  __syncthreads();
+  WSum r{s.hi - v.hi, s.lo - v.lo};
+  if constexpr (NW <= 4) {
+    *total = WSum{0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      const WSum t{tmp[w], tmp[NW + w]};
+      if (w < wave) r.add(t);
+      total->add(t);
+    }
+  } else {
+    const WSum t{wave_upto(lane < NW ? tmp[lane] : 0ull), wave_upto(lane < NW ? tmp[NW + lane] : 0ull)};   // the waves' sums, a lane each
+    *total = WSum{at_lane(t.hi, NW - 1), at_lane(t.lo, NW - 1)};
+    if (wave > 0) r.add(WSum{at_lane(t.hi, wave - 1), at_lane(t.lo, wave - 1)});
+  }
   return r;
 }
-__device__ __forceinline__ double wide_to_double(u128 v) { return (double)(u64)(v >> 64) * 18446744073709551616.0 + (double)(u64)v; }
+__device__ __forceinline__ double wide_to_double(u128 v) {     // v < 2^88 (2^31 weights)
+  return fma((double)(unsigned)(v >> 64), 18446744073709551616.0, (double)(u64)v);
+}
 __device__ __forceinline__ u128 double_to_wide(double v) {   // v >= 0
   const u64 hi = (u64)(v * 5.42101086242752217e-20);          // 2^-64
   const double rest = v - (double)hi * 18446744073709551616.0;
@@ -219,12 +242,12 @@ __device__ __forceinline__ u128 sample_goal(float u, u128 W) {
   return double_to_wide((double)u * wide_to_double(W));
 }
 // entries j = 0, 1, .. of one tied weight w stay while above + j w < limit (the first always)
-__device__ __forceinline__ unsigned ties_within(u64 above, u64 w, double limit, unsigned most) {
+__device__ __forceinline__ unsigned ties_within(u128 above, u64 w, double limit, unsigned most) {
   if (w == 0) return most;
   unsigned lo = 1, hi = most;           // the first j in [1, most] that does not stay
   while (lo < hi) {
     const unsigned mid = lo + (hi - lo) / 2;
-    if ((double)(above + w * mid) < limit) lo = mid + 1; else hi = mid;
+    if (wide_to_double(above + (u128)w * mid) < limit) lo = mid + 1; else hi = mid;
   }
   return lo;
 }
@@ -279,7 +302,7 @@ struct Select {   // state of a selection (one per row)
   int step; unsigned lo, hi;            // the border's step, its keys [lo, hi]
   unsigned prefix, count;               // the key's bits so far, and the entries that share them
   unsigned need;                        // top-k: how many of those stay
-  u64 above; double limit;              // top-p: the weight in front of them, p times all of it
+  u128 above; double limit;             // top-p: the weight in front of them, p times all of it
   unsigned done;
 };
 // bins lie in the order of the threads that sum them: thread t of NT takes places t SB / NT .. , place j of them at j (NT + 1) + t (a bank apart:
@@ -288,6 +311,22 @@ template <int NT>
 __device__ __forceinline__ int bin_at(int place) {
   constexpr int PB = SB / NT;
   return (place % PB) * (NT + 1) + place / PB;
+}
+// a bin of weights: 64 bits and, in units of 2^HI, 32 more.  Up to 65 536 entries go in without a carry (HI 42: a weight below 2^64 / entries into the
+// lower part, of a larger one its last 42 bits); any number of them with one (HI 64)
+constexpr int BIN_HI = 42;
+__device__ __forceinline__ unsigned large_from(unsigned entries) { return entries > 128u ? 1u << __clz(entries - 1u) : 1u << 25; }   // 2^(64 - log2), upper word
+__device__ __forceinline__ void add_weight(u64* lo, unsigned* hi, u64 w, unsigned times, unsigned large) {
+  if ((unsigned)(w >> 32) >= large) {
+    atomicAdd(hi, (unsigned)(w >> BIN_HI) * times);
+    w &= (1ull << BIN_HI) - 1ull;
+  }
+  atomicAdd(lo, w * times);
+}
+__device__ __forceinline__ void add_wide(u64* lo, unsigned* hi, u128 v) {
+  const u64 w = (u64)v, old = atomicAdd(lo, w);
+  const unsigned up = (unsigned)(v >> 64) + (old + w < old);
+  if (up) atomicAdd(hi, up);
 }
 // the place that the border falls into, found by the whole workgroup; updates st, sets cut when it is final.
 // `last`: no key of this type has bits below this round's
@@ -326,39 +365,66 @@ __device__ __forceinline__ void pick_k(int round, bool last, const unsigned* hc,
   }
   __syncthreads();
 }
-template <int NT>
-__device__ __forceinline__ void pick_p(int round, bool last, const unsigned* hc, const u64* hw, double p, Select* st, SampleCut* cut, u64* tmp) {
+// the bins' weights in hw and hc (see add_weight)
+template <int NT, int HI>
+__device__ __forceinline__ void pick_p(int round, const unsigned* hc, const u64* hw, double p, Select* st, u64* tmp) {
   constexpr int PB = SB / NT;
   const unsigned prefix = st->prefix;
-  const u64 above = st->above;
+  const u128 above = st->above;
   const double given = st->limit;
-  u64 mine[PB], sum = 0, total;
+  auto in_bin = [&](int j) { return ((u128)hc[j * (NT + 1) + threadIdx.x] << HI) + hw[j * (NT + 1) + threadIdx.x]; };
+  u128 here = 0;
+  WSum total;
 #pragma unroll
-  for (int j = 0; j < PB; ++j) { mine[j] = hw[j * (NT + 1) + threadIdx.x]; sum += mine[j]; }
-  u64 before = block_before<NT>(sum, tmp, &total) + above;
-  const double limit = round < 0 ? p * (double)total : given;
+  for (int j = 0; j < PB; ++j) here += in_bin(j);
+  u128 before = block_before<NT>(WSum{(u64)(here >> 32), (u64)here & 0xFFFFFFFFull}, tmp, &total).all() + above;
+  const double limit = round < 0 ? p * wide_to_double(total.all()) : given;
   // the first entry of exactly one bin is the last whose forerunners weigh less than the limit
-  if ((double)before < limit && !((double)(before + sum) < limit)) {
+  if (wide_to_double(before) < limit && !(wide_to_double(before + here) < limit)) {
+    u128 mine[PB];                      // (read again: not worth registers across the sums)
 #pragma unroll
+    for (int j = 0; j < PB; ++j) mine[j] = in_bin(j);
+    int found = 0;
+#pragma unroll
+    for (int j = 0; j < PB - 1; ++j)
+      if (found == j && wide_to_double(before + mine[j]) < limit) { before += mine[j]; ++found; }
+    const int place = (int)threadIdx.x * PB + found;
+    st->above = before;
+    st->limit = limit;
+    if (round < 0) st->step = place;
+    else st->prefix = round_prefix(prefix, round, place);
+  }
+  __syncthreads();
+}
+// the last round: hc are the entries of one key a bin, weight(key) each
+template <int NT, typename W>
+__device__ __forceinline__ void pick_p_key(int round, const unsigned* hc, const W& weight, Select* st, SampleCut* cut, u64* tmp) {
+  constexpr int PB = SB / NT;
+  const unsigned prefix = st->prefix;
+  const u128 above = st->above;
+  const double limit = st->limit;
+  auto key_of = [&](int j) { return round_prefix(prefix, round, (int)threadIdx.x * PB + j) << round_shift(round); };
+  auto in_bin = [&](int j) -> u128 {
+    const unsigned c = hc[j * (NT + 1) + threadIdx.x];
+    return c ? (u128)weight(key_of(j)) * c : 0;
+  };
+  u128 here = 0;
+#pragma unroll 1
+  for (int j = 0; j < PB; ++j) here += in_bin(j);
+  WSum total;
+  u128 before = block_before<NT>(WSum{(u64)(here >> 32), (u64)here & 0xFFFFFFFFull}, tmp, &total).all() + above;
+  if (wide_to_double(before) < limit && !(wide_to_double(before + here) < limit)) {
+#pragma unroll 1
     for (int j = 0; j < PB; ++j) {
-      if ((double)before < limit && !((double)(before + mine[j]) < limit)) {
-        const int place = (int)threadIdx.x * PB + j;
-        st->above = before;
-        st->limit = limit;
-        if (round < 0) st->step = place;
-        else {
-          const unsigned n = hc[j * (NT + 1) + threadIdx.x];
-          const unsigned q = round_prefix(prefix, round, place);
-          st->prefix = q;
-          if (last) {
-            const unsigned key = q << round_shift(round), t = ties_within(before, mine[j] / n, limit, n);
-            cut->cut = t == n ? key - 1u : key;
-            cut->ties = t == n ? 0u : t;
-            st->done = 1u;
-          }
-        }
+      const u128 mine = in_bin(j);
+      if (!(wide_to_double(before + mine) < limit)) {
+        const unsigned n = hc[j * (NT + 1) + threadIdx.x], key = key_of(j), t = ties_within(before, weight(key), limit, n);
+        cut->cut = t == n ? key - 1u : key;
+        cut->ties = t == n ? 0u : t;
+        st->done = 1u;
+        break;
       }
-      before += mine[j];
+      before += mine;
     }
   }
   __syncthreads();
@@ -399,7 +465,7 @@ __device__ __forceinline__ void direct_p(const unsigned* keys, const u64* wgt, i
   if ((int)threadIdx.x < n) {
     const unsigned mine = keys[threadIdx.x];
     const u64 w = wgt[threadIdx.x];
-    u64 front = st->above;
+    u64 larger = 0;                     // (of at most 127 others, 2^57 each)
     unsigned equal = 0;
     for (int j = 0; j < n; j += 8) {
       const uint4 u = *(const uint4*)(keys + j), v = *(const uint4*)(keys + j + 4);
@@ -408,10 +474,11 @@ __device__ __forceinline__ void direct_p(const unsigned* keys, const u64* wgt, i
 #pragma unroll
       for (int q = 0; q < 8; ++q) x[q] = wgt[j + q];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) { front += k[q] > mine ? x[q] : 0; equal += k[q] == mine; }
+      for (int q = 0; q < 8; ++q) { larger += k[q] > mine ? x[q] : 0; equal += k[q] == mine; }
     }
     const double limit = st->limit;
-    if ((double)front < limit && !((double)(front + w * equal) < limit)) {
+    const u128 front = st->above + larger;
+    if (wide_to_double(front) < limit && !(wide_to_double(front + (u128)w * equal) < limit)) {
       const unsigned t = ties_within(front, w, limit, equal);
       cut->cut = t == equal ? mine - 1u : mine;
       cut->ties = t == equal ? 0u : t;
@@ -425,14 +492,14 @@ constexpr int SLIST = 2048;
 // Thread t owns the entries [t C, (t + 1) C): sums in index order are one scan over the threads.  When top-k leaves few entries they are
 // copied out, in order, and everything behind it works on the copy.  A draw falls to one thread's entries; a wave looks at them together.
 template <int NT, bool RAW>
-__global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse) {
+__global__ __launch_bounds__(NT, 4) void sample_row_kernel(SampleArgs a) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   constexpr int NWV = NT / 64, LAST = RAW ? 1 : 2;
   u64* hw = (u64*)smem;                                          // [SBP]; the copied entries on their way
   unsigned* hc = (unsigned*)(hw + SBP);                          // [SBP]
   unsigned* keys = hc + SBP;                                     // [N] (RAW: 16 bits each); then the copied entries, keys and indices
   unsigned short* keys16 = (unsigned short*)keys;
-  __shared__ u64 tmp64[NWV];
+  __shared__ u64 tmp64[2 * NWV];
   __shared__ unsigned tmp32[NWV], s_min[NWV], s_n;
   __shared__ Select st;
   __shared__ SampleCut cut_s;
@@ -579,12 +646,13 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
       steps.set(r, least, true);
       if (tid == 0) { st = Select{0, 1u, mk, 0u, 0u, 0u, 0, 0.0, 0u}; cut_s = SampleCut{mk, 1u}; s_n = 0u; }   // (p <= 0: the largest alone)
       if (tid < DIRECT) { near_k[tid] = 0u; near_w[tid] = 0; }
+      const unsigned large = large_from((unsigned)n);
       const bool few = n <= DIRECT && copied;                    // no histogram: all of them are compared
       auto gather = [&]() {                                      // the keys of the border's step (few: all), as many as can be compared
         const unsigned lo = st.lo, hi = st.hi;
         auto add = [&](unsigned k) {
           const unsigned q = atomicAdd(&s_n, 1u);
-          if (q < DIRECT) { near_k[q] = k; near_w[q] = r.weight(k) >> coarse; }
+          if (q < DIRECT) { near_k[q] = k; near_w[q] = r.weight(k); }
         };
         for (int i = tid; i < n; i += NT) {
           const unsigned k = key_at(i);
@@ -602,8 +670,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
         auto count = [&](unsigned k, unsigned times) {
           if (round >= 0 && !(k >= lo && k <= hi && round_in(k, round, prefix))) return;
           const int d = bin_at<NT>(round < 0 ? steps.of(k) : round_place(k, round));
-          if (round >= 0) atomicAdd(&hc[d], times);
-          atomicAdd(&hw[d], (r.weight(k) >> coarse) * times);
+          if (round == LAST) atomicAdd(&hc[d], times);
+          else add_weight(hw + d, hc + d, r.weight(k), times, large);
         };
         for (int i = tid; i < n; i += NT) {
           const unsigned k = key_at(i);
@@ -611,7 +679,8 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
         }
         if (tid == 0 && c.cut != 0u && c.ties != 0u) count(c.cut, c.ties);   // the ties that top-k left
         __syncthreads();
-        pick_p<NT>(round, round == LAST, hc, hw, r.p, &st, &cut_s, tmp64);
+        if (round == LAST) pick_p_key<NT>(round, hc, [&](unsigned k) { return r.weight(k); }, &st, &cut_s, tmp64);
+        else pick_p<NT, BIN_HI>(round, hc, hw, r.p, &st, tmp64);
         if (round < 0) {
           step_keys(steps, mk, &st);
           gather();
@@ -623,9 +692,10 @@ __global__ __launch_bounds__(NT) void sample_row_kernel(SampleArgs a, int coarse
       __syncthreads();
       if (r.p > 0.0 && !st.done) {
         if (few) {                                               // the limit: p times all of it
-          u64 total;
-          block_before<NT>(tid < DIRECT ? near_w[tid] : 0, tmp64, &total);
-          if (tid == 0) st.limit = r.p * (double)total;
+          WSum one{0, 0}, total;
+          if (tid < DIRECT) one.add(near_w[tid]);
+          block_before<NT>(one, tmp64, &total);
+          if (tid == 0) st.limit = r.p * wide_to_double(total.all());
           __syncthreads();
         }
         direct_p(near_k, near_w, (int)s_n, &st, &cut_s);
@@ -716,7 +786,7 @@ struct SampleLong {
   SampleState* state; unsigned* hc; u64* hw;   // [B], [B][SBP], [B][SBP]
   unsigned* tb; u64* bs;                       // [B][nblk] ties of a block, [B][2 nblk] kept weight of a block
   unsigned* list;                              // [B][LLIST] keys of the border's step
-  int nblk, nchunk, coarse;
+  int nblk, nchunk;
   int chunk;                                   // entries of a workgroup, a multiple of 4 096
   int uses_k, uses_p;
 };
@@ -829,14 +899,28 @@ __device__ __forceinline__ void add_bins(const T* mine, T* row) {
   if constexpr (FIRST + 256 < SBP) add_bins<FIRST + 256>(mine, row);
   asm volatile("" ::"v"(old));
 }
+// the same of bins of weights (HI 42), into the row's (HI 64)
+template <int FIRST = 0>
+__device__ __forceinline__ void add_bins(const u64* lo, const unsigned* hi, u64* row_lo, unsigned* row_hi) {
+  const int i = (int)threadIdx.x + FIRST;
+  const u128 v = i < SBP ? ((u128)hi[i] << BIN_HI) + lo[i] : 0;
+  const u64 w = (u64)v;
+  u64 old = 0;
+  unsigned up = (unsigned)(v >> 64), old_up = 0;
+  if (w) old = __hip_atomic_fetch_add(row_lo + i, w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if constexpr (FIRST + 256 < SBP) add_bins<FIRST + 256>(lo, hi, row_lo, row_hi);
+  up += old + w < old;
+  if (up) old_up = __hip_atomic_fetch_add(row_hi + i, up, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("" ::"v"(old), "v"(old_up));
+}
 // the top-k (PHASE 0) or top-p (PHASE 1) selection: counts (and weights) of the steps; the workgroup that arrives last finds the border's step
 // and clears the bins
 template <int PHASE, int TYPE>
 __global__ __launch_bounds__(256) void sample_steps_kernel(SampleArgs a, SampleLong g, int mode) {
-  __shared__ unsigned hc[PHASE == 0 ? SBP : 1];
+  __shared__ unsigned hc[SBP];
   __shared__ u64 hw[PHASE == 1 ? SBP : 1];
   __shared__ unsigned tmp32[4], last;
-  __shared__ u64 tmp64[4];
+  __shared__ u64 tmp64[8];
   __shared__ Select st;
   __shared__ SampleCut cut;
   const int b = blockIdx.y, tid = threadIdx.x;
@@ -856,20 +940,19 @@ __global__ __launch_bounds__(256) void sample_steps_kernel(SampleArgs a, SampleL
   u64* ghw = g.hw + (long long)b * SBP;
   const SampleCut kc = S->kcut;
   for (int i = tid; i < SBP; i += 256) {
-    if constexpr (PHASE == 0) hc[i] = 0u;
-    else hw[i] = 0;
+    hc[i] = 0u;
+    if constexpr (PHASE == 1) hw[i] = 0;
   }
   __syncthreads();
   const long long i0 = (long long)blockIdx.x * g.chunk, i1 = min(a.N, i0 + g.chunk);
   const float above = PHASE == 1 ? cut_value(kc.cut, TYPE) : -INFINITY;
   const double m = (double)r.m, scale = r.scale;
-  auto count = [&](float x, unsigned times) {
+  const unsigned large = large_from((unsigned)g.chunk);
+  auto weight = [&](float x) { return exp2_fixed(r.flat ? (x == r.m ? 0.0 : -100.0) : ((double)x - m) * scale); };
+  auto count = [&](float x) {
     const int d = bin_at<256>(steps.of_value(x));
-    if constexpr (PHASE == 0) atomicAdd(&hc[d], times);
-    else {
-      const double z = r.flat ? (x == r.m ? 0.0 : -100.0) : ((double)x - m) * scale;
-      atomicAdd(&hw[d], (exp2_fixed(z) >> g.coarse) * times);
-    }
+    if constexpr (PHASE == 0) atomicAdd(&hc[d], 1u);
+    else add_weight(hw + d, hc + d, weight(x), 1u, large);       // (a chunk is 65 536 entries at most)
   };
   {
     const long long base = (long long)b * a.ld;
@@ -886,15 +969,14 @@ __global__ __launch_bounds__(256) void sample_steps_kernel(SampleArgs a, SampleL
       for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (v[u].x[j] > above) count(v[u].x[j], 1u);
+          if (v[u].x[j] > above) count(v[u].x[j]);
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = w[u];
     }
   }
-  if (PHASE == 1 && blockIdx.x == 0 && tid == 0 && kc.cut != 0u && kc.ties != 0u) count(above, kc.ties);
   __syncthreads();
   if constexpr (PHASE == 0) add_bins(hc, ghc);
-  else add_bins(hw, ghw);
+  else add_bins(hw, hc, ghw, ghc);
   __syncthreads();
   if (tid == 0) last = ur_arrive(&S->arrived, mode) == (unsigned)g.nchunk - 1u;
   __syncthreads();
@@ -903,13 +985,37 @@ __global__ __launch_bounds__(256) void sample_steps_kernel(SampleArgs a, SampleL
     st = Select{0, 1u, mk, 0u, 0u, (unsigned)min((long long)0x7FFFFFFF, r.k), 0, 0.0, 0u};
     cut = S->cut;
   }
+  constexpr int PER = (SBP + 255) / 256;                         // all of a thread's bins under way at once
+  unsigned c[PER];
+  u64 w[PHASE == 1 ? PER : 1];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = min(tid + 256 * j, SBP - 1);
+    c[j] = agent_load(ghc + i);
+    if constexpr (PHASE == 1) w[j] = agent_load(ghw + i);
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    const int i = tid + 256 * j;
+    if (i >= SBP) break;
+    hc[i] = c[j];
+    if constexpr (PHASE == 1) hw[i] = w[j];
+  }
+  __syncthreads();
   for (int i = tid; i < SBP; i += 256) {
-    if constexpr (PHASE == 0) { hc[i] = agent_load(ghc + i); ghc[i] = 0u; }
-    else { hw[i] = agent_load(ghw + i); ghw[i] = 0; }
+    ghc[i] = 0u;
+    if constexpr (PHASE == 1) ghw[i] = 0;
   }
   __syncthreads();
   if constexpr (PHASE == 0) pick_k<256>(-1, false, hc, &st, &cut, tmp32);
-  else pick_p<256>(-1, false, nullptr, hw, r.p, &st, &cut, tmp64);
+  else {
+    if (tid == 0 && kc.cut != 0u && kc.ties != 0u) {             // the ties that top-k left
+      const int d = bin_at<256>(steps.of_value(above));
+      add_wide(hw + d, hc + d, (u128)weight(above) * kc.ties);
+    }
+    __syncthreads();
+    pick_p<256, 64>(-1, hc, hw, r.p, &st, tmp64);
+  }
   step_keys(steps, mk, &st);
   if (tid == 0) {
     S->st = st;
@@ -953,7 +1059,7 @@ __global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, Sampl
   __shared__ __attribute__((aligned(16))) unsigned near_k[DIRECT];
   __shared__ u64 near_w[PHASE == 1 ? DIRECT : 1];
   __shared__ unsigned tmp32[NT / 64];
-  __shared__ u64 tmp64[NT / 64];
+  __shared__ u64 tmp64[2 * NT / 64];
   __shared__ Select st;
   __shared__ SampleCut cut;
   const int b = blockIdx.x, tid = threadIdx.x;
@@ -975,7 +1081,7 @@ __global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, Sampl
     if (tid < DIRECT) {
       const unsigned k = tid < (int)n ? list[tid] : 0u;
       near_k[tid] = k;
-      if constexpr (PHASE == 1) near_w[tid] = k ? r.weight(k) >> g.coarse : 0;
+      if constexpr (PHASE == 1) near_w[tid] = k ? r.weight(k) : 0;
     }
     __syncthreads();
     if constexpr (PHASE == 0) direct_k(near_k, (int)n, &st, &cut);
@@ -994,8 +1100,8 @@ __global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, Sampl
     auto count = [&](unsigned k, unsigned times) {
       if (!round_in(k, round, prefix)) return;
       const int d = bin_at<NT>(round_place(k, round));
-      atomicAdd(&hc[d], times);
-      if constexpr (PHASE == 1) atomicAdd(&hw[d], (r.weight(k) >> g.coarse) * times);
+      if (PHASE == 0 || round == rounds - 1) atomicAdd(&hc[d], times);
+      else add_wide(hw + d, hc + d, (u128)r.weight(k) * times);
     };
     if (listed) {
       for (unsigned i = tid; i < n; i += NT) count(list[i], 1u);
@@ -1013,7 +1119,8 @@ __global__ __launch_bounds__(1024) void sample_border_kernel(SampleArgs a, Sampl
     if (tied && tid == 0) count(kc.cut, kc.ties);
     __syncthreads();
     if constexpr (PHASE == 0) pick_k<NT>(round, round == rounds - 1, hc, &st, &cut, tmp32);
-    else pick_p<NT>(round, round == rounds - 1, hc, hw, r.p, &st, &cut, tmp64);
+    else if (round == rounds - 1) pick_p_key<NT>(round, hc, [&](unsigned k) { return r.weight(k); }, &st, &cut, tmp64);
+    else pick_p<NT, 64>(round, hc, hw, r.p, &st, tmp64);
   }
   if (tid == 0) {
     S->cut = inside(cut, kc);
@@ -1112,7 +1219,7 @@ __global__ __launch_bounds__(256) void sample_sums_kernel(SampleArgs a, SampleLo
 }
 // a workgroup a draw: the block that the goal falls into (a thread takes a run of blocks), then its entry (a thread takes eight)
 __global__ __launch_bounds__(256) void sample_draw_kernel(SampleArgs a, SampleLong g) {
-  __shared__ u64 tmp64[4];
+  __shared__ u64 tmp64[8];
   __shared__ unsigned tmp32[4];
   __shared__ int q_s;
   __shared__ WSum run_s;
@@ -1188,12 +1295,6 @@ __global__ __launch_bounds__(256) void sample_draw_kernel(SampleArgs a, SampleLo
 }
 
 // ---- host
-static inline int log2_up(long long n) {
-  int k = 0;
-  while ((1LL << k) < n) ++k;
-  return k;
-}
-static inline int coarse_bits(long long n) { return std::max(0, log2_up(n) - 6); }   // sums of n weights stay below 2^63
 // what fits into a workgroup's LDS beside the histograms.  Rows in LDS or over many workgroups, k 50 and p 0.9: 256 x 20 000 28 / 144 us, 4 x 30 000
 // 33 / 64
 static inline bool sample_in_lds(long long N, int type) { return N <= (type == UR_F32 ? 32768 : 65536); }
@@ -1208,7 +1309,7 @@ static size_t sample_long_bytes(long long N, int B, char* base, SampleLong* g) {
   // about 2 048 workgroups where there is work for them, of 4 096 to 65 536 entries
   const long long want = (N * (long long)B + 2047) / 2048;
   w.chunk = (int)std::min<long long>(65536, std::max<long long>(4096, (want + 4095) / 4096 * 4096));
-  w.nchunk = cdiv(N, w.chunk); w.nblk = cdiv(N, LBLK); w.coarse = coarse_bits(N);
+  w.nchunk = cdiv(N, w.chunk); w.nblk = cdiv(N, LBLK);
   w.state = (SampleState*)take(sizeof(SampleState) * B);
   w.hc = (unsigned*)take((size_t)B * SBP * 4); w.hw = (u64*)take((size_t)B * SBP * 8);
   w.tb = (unsigned*)take((size_t)B * w.nblk * 4); w.bs = (u64*)take((size_t)B * w.nblk * 16);
@@ -1221,7 +1322,7 @@ static int launch_sample_row(const SampleArgs& a, hipStream_t st) {
   const size_t lds = (size_t)SBP * 12 + (size_t)a.N * (RAW ? 2 : 4) + 16;
   static const hipError_t attr = hipFuncSetAttribute((const void*)sample_row_kernel<NT, RAW>, hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024 - 6144);
   (void)attr;
-  hipLaunchKernelGGL((sample_row_kernel<NT, RAW>), dim3(a.B), dim3(NT), lds, st, a, coarse_bits(a.N));
+  hipLaunchKernelGGL((sample_row_kernel<NT, RAW>), dim3(a.B), dim3(NT), lds, st, a);
   UR_LAUNCH_CHECK();
   return UR_OK;
 }
