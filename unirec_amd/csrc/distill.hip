@@ -671,12 +671,12 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
 struct DistillLoss {
   const float* stat; int B, d, K; float T2; float* loss_out;
   const float* U; _Float16* img; float* rb_img; int* ky_img;
-  const float* coef; const int* tid; int buckets, shift; int* offs; uint2* list;
+  const float* coef; const int* tid; int buckets, log2b; int* offs; uint2* list;
 };
 // Workgroup 0: loss_out = [T^2 / C sum of the rows' losses, C, update guard, -] (fixed order).  The others (a forward pass that will be
 // followed by a backward), two for a tile of 32 users, leave what the backward needs of it.  One the image that every workgroup streams: one
 // exponent, [hi | lo][32][D] halves in the swizzled order, the row biases -log2(softmax sum) (-inf without a teacher and behind the last user).
-// The other its teacher's entries (item - first item of the bucket, user; p) by bucket of 2^shift items, a counting sort in LDS: the order inside a bucket is free.
+// The other its teacher's entries (item / buckets, user; p) by bucket item % buckets, a counting sort in LDS: the order inside a bucket is free.
 template <int D>
 __global__ __launch_bounds__(256) void distill_loss_kernel(DistillLoss a) {
   __shared__ float red[4];
@@ -755,7 +755,7 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillLoss a) {
     fetch(i0);
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)
-      if (item[j] > 0 && p[j] != 0.f) atomicAdd(&count_s[item[j] >> a.shift], 1u);
+      if (item[j] > 0 && p[j] != 0.f) atomicAdd(&count_s[item[j] & (a.buckets - 1)], 1u);
   }
   __syncthreads();
   const int per = (a.buckets + 255) / 256, i0 = min(a.buckets, tid * per), i1 = min(a.buckets, i0 + per);
@@ -788,29 +788,29 @@ __global__ __launch_bounds__(256) void distill_loss_kernel(DistillLoss a) {
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j)
       if (item[j] > 0 && p[j] != 0.f)
-        list[atomicAdd(&count_s[item[j] >> a.shift], 1u)] =
-            make_uint2(((unsigned)item[j] & ((1u << a.shift) - 1u)) << 5 | (i0 + tid + 256u * j) / (unsigned)a.K, __float_as_uint(p[j]));
+        list[atomicAdd(&count_s[item[j] & (a.buckets - 1)], 1u)] =
+            make_uint2(((unsigned)item[j] >> a.log2b) << 5 | (i0 + tid + 256u * j) / (unsigned)a.K, __float_as_uint(p[j]));
   }
 }
 
 struct DistillApply {
-  const int* offs; const uint2* list; int buckets, shift;
+  const int* offs; const uint2* list; int buckets, log2b; unsigned items;   // items: of a bucket, at most
   const float *U, *d_unit;
   int B, d, K;
   const float* loss_out; const float* d_loss; float g_num;
   float *d_user, *d_table, *d_bias;
 };
 // A workgroup per bucket: dE[item] -= g sum p u, d_bias[item] -= g sum p over its lists of up to 16 tiles of users (512 users) at a time, put
-// in the order of (item, user) by a bitonic sort in LDS.  Lists longer than the room there: one tile at a time, 32 items (32 x 32 entries at
-// the most) at a time.  TPR lanes hold a row; a group of them takes an item, all groups one that many list (a popular item).  The
+// in the order of (item, user) by a bitonic sort in LDS.  Lists longer than the room there: one tile at a time, as many items at a time as have
+// their entries in the room, 32 (32 x 32 entries at the most) at least.  TPR lanes hold a row; a group of them takes an item, all groups one that many list (a popular item).  The
 // workgroups behind: d_user = g d_unit.  Latency bound: a chain of range, entries, rows, gradient.
 template <int TPR>
 __global__ __launch_bounds__(128) void distill_apply_kernel(DistillApply a) {
-  constexpr int NT = 128, G = NT / TPR, ROOM = 1024, WINDOW = ROOM / DS_TILE, LONG = 32;
+  constexpr int NT = 128, G = NT / TPR, ROOM = 1024, LONG = 32, AHEAD = 8;
   typedef unsigned long long u64;
   __shared__ u64 entry_s[ROOM];                                  // item of the bucket << 41 | user of the 512 << 32 | p
   __shared__ unsigned short run_s[ROOM + 1], long_s[ROOM];       // where an item's entries begin
-  __shared__ int first_s[16], count_s[16], n_s, runs_s, nlong_s;
+  __shared__ int first_s[16], count_s[16], reach_s[32], n_s, runs_s, nlong_s;
   __shared__ __attribute__((aligned(16))) float4 acc_s[NT];
   __shared__ float accp_s[G];
   const float gs = distill_scale(a.loss_out, a.d_loss, a.g_num);
@@ -824,7 +824,6 @@ __global__ __launch_bounds__(128) void distill_apply_kernel(DistillApply a) {
     return;
   }
   const int bucket = blockIdx.x, tiles = (a.B + DS_TILE - 1) / DS_TILE;
-  const long long item0 = (long long)bucket << a.shift;
   for (int t0 = 0, m = 0; t0 < tiles; t0 += m) {
     const int some = min(16, tiles - t0);
     __syncthreads();
@@ -847,16 +846,37 @@ __global__ __launch_bounds__(128) void distill_apply_kernel(DistillApply a) {
     const int n_tile = tile < m ? count_s[tile] : 0;
     const uint2* list = a.list + ((long long)(t0 + tile) * DS_TILE * a.K + (tile < m ? first_s[tile] : 0));
     const bool fits = total <= ROOM;
-    const unsigned items = 1u << a.shift;
-    for (unsigned w0 = 0; w0 < items; w0 += fits ? items : (unsigned)WINDOW) {
-      const unsigned w1 = fits ? items : w0 + WINDOW;
+    const unsigned items = a.items;
+    auto each = [&](auto f) {                                    // of the entries, AHEAD of a thread on their way at once
+      for (int i0 = tid % lanes; i0 < n_tile; i0 += AHEAD * lanes) {
+        uint2 v[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) v[j] = list[min(i0 + j * lanes, n_tile - 1)];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j)
+          if (i0 + j * lanes < n_tile) f(v[j]);
+      }
+    };
+    for (unsigned w0 = 0, w1 = items; w0 < items; w0 = w1, w1 = items) {
       if (tid == 0) n_s = nlong_s = 0;
+      if (!fits) {                                               // entries by the bits of their distance from w0: the widest 2^bits that fits
+        if (tid < 32) reach_s[tid] = 0;
+        __syncthreads();
+        each([&](const uint2& v) {
+          const unsigned o = v.x >> 5;
+          if (o >= w0) atomicAdd(&reach_s[o == w0 ? 0 : 32 - __clz(o - w0)], 1);
+        });
+        __syncthreads();
+        int bits = 0, sum = reach_s[0];
+        while ((1u << bits) < items && (bits < 5 || sum + reach_s[bits + 1] <= ROOM)) sum += reach_s[++bits];
+        w1 = min(items, w0 + (1u << bits));
+        if (sum == 0) { __syncthreads(); continue; }
+      }
       __syncthreads();
-      for (int i = tid % lanes; i < n_tile; i += lanes) {
-        const uint2 v = list[i];
+      each([&](const uint2& v) {
         const unsigned o = v.x >> 5;
         if (o >= w0 && o < w1) entry_s[atomicAdd(&n_s, 1)] = ((u64)o << 41) | ((u64)(unsigned)(tile * DS_TILE + (v.x & 31u)) << 32) | v.y;
-      }
+      });
       __syncthreads();
       const int n = n_s;
       if (n == 0) { __syncthreads(); continue; }
@@ -901,7 +921,7 @@ __global__ __launch_bounds__(128) void distill_apply_kernel(DistillApply a) {
         }
       };
       auto put = [&](int from, const float4& acc, float pb) {
-        const long long item = item0 + (long long)(entry_s[from] >> 41);
+        const long long item = (long long)(entry_s[from] >> 41) << a.log2b | bucket;
         if (on) {
           float4* e = (float4*)a.d_table + item * d4 + t;
           const float4 v = *e;
@@ -963,18 +983,21 @@ static void ds_splits(int B, int d, long long N, int* owner_blocks, int* splits,
   *splits = (int)s;
 }
 
-// items of a bucket of the lists, 2^shift: some 8 to 16 entries a bucket if ids were uniform (32 to 64: 512 x 60 K 103 us, these 100), and no more buckets than a tile of users can
-// count in LDS.  (512 users x 100, 1 M items: buckets of 128 items left 7 a workgroup, 86 us of workgroups waiting for memory; 400 x 20, 1 682
-// items: 14 workgroups of 610, 21 us)
-static inline int ds_shift(long long N, long long entries) {
-  int s = 0;
+// buckets of the lists, a power of two: some 4 to 16 entries a bucket (32 to 64: 512 x 60 K 103 us, 8 to 16 100), and no more buckets than a tile of
+// users can count in LDS.  (512 users x 100, 1 M items: buckets of 128 items left 7 a workgroup, 86 us of workgroups waiting for memory; 400 x 20,
+// 1 682 items: 14 workgroups of 610, 21 us.)  An item's bucket is its id modulo their number: ids next to each other, which are often alike popular, fall
+// into different ones.  (With ranges of ids, 512 users x 100 entries on 200 neighbours of 1 M items, d 64, had one workgroup do it all: the
+// backward 4 375 us, 508 with lists all over the catalogue; as it is 529 and 523; 120 items with one remainder, which still share a list, 3 617)
+static inline int ds_log2_buckets(long long N, long long entries) {
+  int s = 0, k = 0;
   while (s < 22 && ((entries << s) < 8 * N || ((N - 1) >> s) >= 8192)) ++s;
-  return s;
+  while ((1LL << k) < ((N - 1) >> s) + 1) ++k;
+  return k;
 }
 struct DistillWs {
   float *part_m, *part_l, *part_o, *stat, *coef; int* tid;          // the forward's own
   _Float16* img; float* rb_img; int* ky_img; int* offs; uint2* list; float* d_unit;   // from the forward to the backward
-  int buckets, shift;
+  int buckets, log2b;
   int64_t bytes;
 };
 static DistillWs ds_carve(int B, int d, long long N, int K, int grad, char* base) {
@@ -988,8 +1011,8 @@ static DistillWs ds_carve(int B, int d, long long N, int K, int grad, char* base
   int ob, splits;
   long long per;
   ds_splits(B, d, N, &ob, &splits, &per);
-  w.shift = ds_shift(N, (long long)B * K);
-  w.buckets = (int)(((N - 1) >> w.shift) + 1);
+  w.log2b = ds_log2_buckets(N, (long long)B * K);
+  w.buckets = 1 << w.log2b;
   if (grad) {
     const int64_t ut = cdiv(B, DS_TILE);
     w.img = (_Float16*)take(ut * 4 * DS_TILE * ds_width(d)); w.rb_img = (float*)take(ut * DS_TILE * 4); w.ky_img = (int*)take(ut * 4);
@@ -1091,7 +1114,7 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   DistillLoss l{};
   l.stat = w.stat; l.B = B; l.d = d; l.K = K; l.T2 = temperature * temperature; l.loss_out = loss_out; l.U = user_emb;
   l.img = w.img; l.rb_img = w.rb_img; l.ky_img = w.ky_img; l.coef = w.coef; l.tid = w.tid;
-  l.buckets = w.buckets; l.shift = w.shift; l.offs = w.offs; l.list = w.list;
+  l.buckets = w.buckets; l.log2b = w.log2b; l.offs = w.offs; l.list = w.list;
   const int tiles = grad ? cdiv(B, DS_TILE) : 0;
   const size_t lds = grad ? (size_t)w.buckets * 4 : 0;
 #define GO(W) hipLaunchKernelGGL((distill_loss_kernel<W>), dim3(1 + 2 * tiles), dim3(256), lds, st, l)
@@ -1126,7 +1149,7 @@ extern "C" int ur_full_distill_bwd(const float* user_emb, const float* item_tabl
      : d <= 128 ? ds_launch_bwd<128>(a, clip, st) : ds_launch_bwd<256>(a, clip, st);
   if (rc) return rc;
   DistillApply p{};
-  p.offs = w.offs; p.list = w.list; p.buckets = w.buckets; p.shift = w.shift; p.U = user_emb; p.d_unit = w.d_unit;
+  p.offs = w.offs; p.list = w.list; p.buckets = w.buckets; p.log2b = w.log2b; p.items = (unsigned)((n_items - 1) >> w.log2b) + 1u; p.U = user_emb; p.d_unit = w.d_unit;
   p.B = B; p.d = d; p.K = K; p.loss_out = loss_out; p.d_loss = d_loss; p.g_num = temperature / tau;
   p.d_user = d_user_emb; p.d_table = d_item_table; p.d_bias = d_item_bias;
   const int blocks = w.buckets + cdiv((long long)B * (d / 4), 128);
