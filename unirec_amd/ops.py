@@ -841,11 +841,16 @@ def full_softmax_bwd_shard(user_emb_all, shard_rows, target_row, lse, ws, d_shar
 
 # --------------------------------------------------------------------------------------------- distillation from a teacher's top logits
 class DistillSaved:
-    """What a full_distill_fwd(need_grad=True) leaves for its full_distill_bwd: a device buffer, and the sizes (B, d, N, K) it was made for."""
-    __slots__ = ("ws", "sizes")
+    """What a full_distill_fwd(need_grad=True) leaves for its full_distill_bwd: a device buffer, the sizes (B, d, N, K) and the arguments
+    (item bias given, tau, score_clip, temperature; None: not known) it was made with."""
+    __slots__ = ("ws", "sizes", "args")
 
-    def __init__(self, ws, sizes):
-        self.ws, self.sizes = ws, sizes
+    def __init__(self, ws, sizes, args=None):
+        self.ws, self.sizes, self.args = ws, sizes, args
+
+
+def _distill_args(item_bias, tau, score_clip, temperature):
+    return item_bias is not None, float(tau), float(score_clip if score_clip and score_clip > 0 else -1.0), float(temperature)
 
 
 def _distill_check(who, user_emb, item_table, item_bias, tau, temperature):
@@ -892,7 +897,7 @@ def full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias=
     check(lib.ur_full_distill_fwd(_p(user_emb), _p(item_table), N, B, d, _p(teacher_id), _p(teacher_score), _lib.DTYPE_IDS[teacher_score.dtype], K,
                                   _p(item_bias), float(tau), float(score_clip if score_clip else -1.0), float(temperature), _p(lse), _p(loss_out),
                                   int(need_grad), _p(ws), _stream()), "ur_full_distill_fwd")
-    return loss_out, lse, (DistillSaved(ws, (B, d, N, K)) if need_grad else None)
+    return loss_out, lse, (DistillSaved(ws, (B, d, N, K), _distill_args(item_bias, tau, score_clip, temperature)) if need_grad else None)
 
 
 def full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, saved, item_bias=None, tau=1.0, score_clip=-1.0, temperature=1.0, d_loss=None):
@@ -900,12 +905,21 @@ def full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, saved, ite
     See include/unirec_amd.h: ur_full_distill_bwd."""
     who = "full_distill_bwd"
     _distill_check(who, user_emb, item_table, item_bias, tau, temperature)
+    _chk(teacher_id, torch.int64, "teacher_id")
+    _chk(lse, torch.float32, "lse")
+    _chk(loss_out, torch.float32, "loss_out")
     _chk(d_loss, torch.float32, "d_loss", allow_none=True)
     B, d = user_emb.shape
-    K, N, dev = teacher_id.shape[1], item_table.shape[0], user_emb.device
-    if saved is None or saved.sizes != (B, d, N, K) or loss_out.numel() != 4 or lse.numel() != B:
+    N, dev = item_table.shape[0], user_emb.device
+    if saved is None or teacher_id.dim() != 2 or saved.sizes != (B, d, N, teacher_id.shape[1]) or loss_out.numel() != 4 or lse.numel() != B:
         raise _lib.UnirecAmdError(f"{who}: not the results of a full_distill_fwd(need_grad=True) of these inputs")
-    _same_device(who, loss_out, saved.ws, d_loss)
+    if saved.args is not None and saved.args != _distill_args(item_bias, tau, score_clip, temperature):
+        raise _lib.UnirecAmdError(f"{who}: (item bias, tau, score_clip, temperature) = {_distill_args(item_bias, tau, score_clip, temperature)}, its "
+                                  f"full_distill_fwd had {saved.args}")
+    if d_loss is not None and d_loss.numel() != 1:
+        raise _lib.UnirecAmdError(f"{who}: d_loss has {d_loss.numel()} values (one, or None)")
+    K = teacher_id.shape[1]
+    _same_device(who, teacher_id, lse, loss_out, saved.ws, d_loss)
     d_user = torch.empty(B, d, dtype=torch.float32, device=dev)
     d_table = torch.empty(N, d, dtype=torch.float32, device=dev)
     d_ib = torch.empty(N, dtype=torch.float32, device=dev) if item_bias is not None else None
