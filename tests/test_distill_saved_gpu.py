@@ -1,4 +1,5 @@
-"""What a distillation's forward leaves for its backward: refused where the two calls do not belong together."""
+"""What a distillation's forward leaves for its backward: refused where the two calls do not belong together, safe on another stream than the
+forward's."""
 import pytest
 import torch
 from test_distill_gpu import _inputs
@@ -29,3 +30,25 @@ def test_a_backward_with_other_arguments_is_refused():
         for n in (0, 2):                                          # (an empty tensor's address is null, which is d_loss = 1)
             with pytest.raises(_lib.UnirecAmdError, match="d_loss"):
                 ops.full_distill_bwd(U, E, ids, lse, loss_out, sv, d_loss=torch.ones(n, device="cuda"), **kw)
+
+
+@pytest.mark.gpu
+def test_a_backward_on_another_stream_keeps_what_it_reads():
+    """the results of the forward are dropped while the backward, on another stream, has not begun: their memory is not given out on the first"""
+    from unirec_amd import ops
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(first):
+        (U, E, ids, score, ib), (loss_out, lse, sv) = _forward()
+        want = ops.full_distill_bwd(U, E, ids, lse, loss_out, sv, item_bias=ib)
+    torch.cuda.synchronize()
+    size = sv.ws.numel()
+    with torch.cuda.stream(second):
+        torch.cuda._sleep(100_000_000)                            # some 50 ms
+        got = ops.full_distill_bwd(U, E, ids, lse, loss_out, sv, item_bias=ib)
+        del sv
+    with torch.cuda.stream(first):
+        over = [torch.full((size,), 255, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    torch.cuda.synchronize()
+    del over
+    assert all(torch.equal(x, y) for x, y in zip(got, want))

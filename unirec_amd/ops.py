@@ -842,11 +842,11 @@ def full_softmax_bwd_shard(user_emb_all, shard_rows, target_row, lse, ws, d_shar
 # --------------------------------------------------------------------------------------------- distillation from a teacher's top logits
 class DistillSaved:
     """What a full_distill_fwd(need_grad=True) leaves for its full_distill_bwd: a device buffer, the sizes (B, d, N, K) and the arguments
-    (item bias given, tau, score_clip, temperature; None: not known) it was made with."""
-    __slots__ = ("ws", "sizes", "args")
+    (item bias given, tau, score_clip, temperature; None: not known) it was made with, and the stream it belongs to (an address; None: the caller's matter)."""
+    __slots__ = ("ws", "sizes", "args", "stream")
 
-    def __init__(self, ws, sizes, args=None):
-        self.ws, self.sizes, self.args = ws, sizes, args
+    def __init__(self, ws, sizes, args=None, stream=None):
+        self.ws, self.sizes, self.args, self.stream = ws, sizes, args, stream
 
 
 def _distill_args(item_bias, tau, score_clip, temperature):
@@ -897,7 +897,7 @@ def full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias=
     check(lib.ur_full_distill_fwd(_p(user_emb), _p(item_table), N, B, d, _p(teacher_id), _p(teacher_score), _lib.DTYPE_IDS[teacher_score.dtype], K,
                                   _p(item_bias), float(tau), float(score_clip if score_clip else -1.0), float(temperature), _p(lse), _p(loss_out),
                                   int(need_grad), _p(ws), _stream()), "ur_full_distill_fwd")
-    return loss_out, lse, (DistillSaved(ws, (B, d, N, K), _distill_args(item_bias, tau, score_clip, temperature)) if need_grad else None)
+    return loss_out, lse, (DistillSaved(ws, (B, d, N, K), _distill_args(item_bias, tau, score_clip, temperature), _stream().value or 0) if need_grad else None)
 
 
 def full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, saved, item_bias=None, tau=1.0, score_clip=-1.0, temperature=1.0, d_loss=None):
@@ -920,6 +920,8 @@ def full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, saved, ite
         raise _lib.UnirecAmdError(f"{who}: d_loss has {d_loss.numel()} values (one, or None)")
     K = teacher_id.shape[1]
     _same_device(who, teacher_id, lse, loss_out, saved.ws, d_loss)
+    if saved.stream is not None and saved.stream != (_stream().value or 0):
+        saved.ws.record_stream(torch.cuda.current_stream())      # (its memory stays the forward's stream's: not to be handed out there under this pass)
     d_user = torch.empty(B, d, dtype=torch.float32, device=dev)
     d_table = torch.empty(N, d, dtype=torch.float32, device=dev)
     d_ib = torch.empty(N, dtype=torch.float32, device=dev) if item_bias is not None else None
