@@ -323,16 +323,16 @@ def _(user_emb, item_table, k, user_id, hist_ptr, hist_sorted, user_bias, item_b
 @custom_op(f"{NS}::full_distill_fwd", mutates_args=())
 def full_distill_fwd(user_emb: torch.Tensor, item_table: torch.Tensor, teacher_id: torch.Tensor, teacher_score: torch.Tensor,
                      item_bias: Optional[torch.Tensor], tau: float = 1.0, score_clip: float = -1.0,
-                     temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """-> (loss_out, lse, ws): full_distill_bwd's"""
-    loss_out, lse, sv = ops.full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias, tau, score_clip, temperature)
-    return loss_out, lse, sv.ws
+                     temperature: float = 1.0, need_grad: bool = True) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """-> (loss_out, lse, ws): full_distill_bwd's (need_grad=False, the loss alone: an empty ws)"""
+    loss_out, lse, sv = ops.full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias, tau, score_clip, temperature, need_grad)
+    return loss_out, lse, sv.ws if need_grad else user_emb.new_empty((0,), dtype=torch.uint8)
 
 
 @full_distill_fwd.register_fake
-def _(user_emb, item_table, teacher_id, teacher_score, item_bias, tau=1.0, score_clip=-1.0, temperature=1.0):
+def _(user_emb, item_table, teacher_id, teacher_score, item_bias, tau=1.0, score_clip=-1.0, temperature=1.0, need_grad=True):
     return (user_emb.new_empty((4,)), user_emb.new_empty((user_emb.shape[0],)),
-            user_emb.new_empty((torch.library.get_ctx().new_dynamic_size(),), dtype=torch.uint8))
+            user_emb.new_empty((torch.library.get_ctx().new_dynamic_size() if need_grad else 0,), dtype=torch.uint8))
 
 
 @custom_op(f"{NS}::full_distill_bwd", mutates_args=())
