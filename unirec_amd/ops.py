@@ -889,6 +889,8 @@ def full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias=
         raise _lib.UnirecAmdError(f"{who}: teacher_id {tuple(teacher_id.shape)} / teacher_score {tuple(teacher_score.shape)} for {B} rows")
     _same_device(who, teacher_id, teacher_score)
     K, N, dev = teacher_id.shape[1], item_table.shape[0], user_emb.device
+    if not 1 <= K <= 65536:
+        raise _lib.UnirecAmdError(f"{who}: {K} entries a list (1 to 65536)")
     id_guard_check()
     f32 = dict(dtype=torch.float32, device=dev)
     lse, loss_out = torch.empty(B, **f32), torch.empty(4, **f32)
