@@ -87,7 +87,8 @@ class _DistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, user_emb, model, teacher_id, teacher_score):
         user_emb = user_emb.contiguous()
-        loss_out, lse, saved = model._distill_forward(user_emb, teacher_id, teacher_score)
+        # (under no_grad, a validation loss: the loss alone, half the products and none of the workspace)
+        loss_out, lse, saved = model._distill_forward(user_emb, teacher_id, teacher_score, need_grad=ctx.needs_input_grad[0])
         ctx.model, ctx.saved = model, saved
         ctx.save_for_backward(user_emb, teacher_id, lse, loss_out)
         object.__setattr__(model, "loss_guard", loss_out[2:3])
@@ -215,8 +216,8 @@ class BaseRecommender(AbstractRecommender):
         return dict(item_bias=self.item_bias.data if self.has_item_bias else None, tau=self.tau, score_clip=self.SCORE_CLIP,
                     temperature=self.distill_temperature)
 
-    def _distill_forward(self, user_emb, teacher_id, teacher_score):
-        return ops.full_distill_fwd(user_emb, self.item_embedding.weight.data, teacher_id, teacher_score, **self._distill_args())
+    def _distill_forward(self, user_emb, teacher_id, teacher_score, need_grad=True):
+        return ops.full_distill_fwd(user_emb, self.item_embedding.weight.data, teacher_id, teacher_score, need_grad=need_grad, **self._distill_args())
 
     def _distill_backward(self, user_emb, teacher_id, lse, loss_out, saved, d_loss):
         d_user, d_table, d_ib = ops.full_distill_bwd(user_emb, self.item_embedding.weight.data, teacher_id, lse, loss_out, saved, d_loss=d_loss,
@@ -445,6 +446,7 @@ class BaseRecommender(AbstractRecommender):
         """Items drawn from the softmax over the k best of a batch of users (k <= 1024; topk's scores, candidates and user_hist), one for
         every random number in [0, 1): rand float32 [B] or [B, S].  temperature 0: always the best item; top_p: of the k, best first, every
         item before which less than top_p of the weight lies; min_p: items with at least min_p of the best one's weight.  Each of the three
-        may be a tensor [B].  -> (ids int64, log-probabilities float32), shaped like rand; (-1, -inf) for a user with no item left."""
+        may be a tensor [B].  Draws are with replacement: a user's S items may repeat.  -> (ids int64, log-probabilities float32), shaped
+        like rand; (-1, -inf) for a user with no item left."""
         scores, ids = self.topk(interaction, k, user_hist=user_hist)
         return ops.sample_scores(scores, rand, temperature=temperature, top_p=top_p, min_p=min_p, ids=ids)
