@@ -109,3 +109,16 @@ def test_sums_of_many_whole_weights(N, dtype):
     u[:, 0], u[:, 1] = 0.0, 1 - 2.0 ** -24
     for f in (dict(p=0.5), dict(p=0.3), dict(p=0.75, T=0.5), dict(k=N - 1, p=0.625), dict(k=(N + 1) // 2, p=0.99, T=3.0)):
         _check(x.to(getattr(torch, dtype)), u, **f)
+
+
+@pytest.mark.gpu
+def test_a_top_k_beyond_32_bits():
+    from unirec_amd import _lib, ops
+    x, u = (t.cuda() for t in _scores(4, 300, 32))
+    want = ops.sample_scores(x, u)
+    for k in (300, 2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, 10 ** 30):
+        got = ops.sample_scores(x, u, top_k=k)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), k
+    for k in (-1, -2 ** 31, -2 ** 32 + 5):
+        with pytest.raises(_lib.UnirecAmdError):
+            ops.sample_scores(x, u, top_k=k)

@@ -973,7 +973,7 @@ def sample_scores(scores, rand, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     nbytes = check(lib.ur_sample_scores_workspace_bytes(_lib.DTYPE_IDS[scores.dtype], N, B), "ur_sample_scores_workspace_bytes")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=scores.device) if nbytes else None
     check(lib.ur_sample_scores(_p(scores), _lib.DTYPE_IDS[scores.dtype], N, ld, B, _p(rand), rand.numel() // B,
-                               1.0 if rows[0] is not None else float(temperature), 0 if rows[1] is not None else int(top_k),
+                               1.0 if rows[0] is not None else float(temperature), 0 if rows[1] is not None else max(-1, min(int(top_k), N)),
                                1.0 if rows[2] is not None else float(top_p), 0.0 if rows[3] is not None else float(min_p),
                                _p(rows[0]), _p(rows[1]), _p(rows[2]), _p(rows[3]), _p(ids), N, _p(index), _p(logp), _p(ws), _stream()), "ur_sample_scores")
     return index, logp
