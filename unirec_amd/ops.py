@@ -853,7 +853,7 @@ def _distill_args(item_bias, tau, score_clip, temperature):
     return item_bias is not None, float(tau), float(score_clip if score_clip and score_clip > 0 else -1.0), float(temperature)
 
 
-def _distill_check(who, user_emb, item_table, item_bias, tau, temperature):
+def _distill_check(who, user_emb, item_table, item_bias, tau, temperature, *others):
     _chk(user_emb, torch.float32, "user_emb")
     _chk(item_table, torch.float32, "item_table")
     _chk(item_bias, torch.float32, "item_bias", allow_none=True)
@@ -863,7 +863,7 @@ def _distill_check(who, user_emb, item_table, item_bias, tau, temperature):
         raise _lib.UnirecAmdError(f"{who}: item_bias has {item_bias.numel()} entries for {item_table.shape[0]} items")
     if not (tau > 0 and temperature > 0):
         raise _lib.UnirecAmdError(f"{who}: tau={tau} and temperature={temperature} must be positive")
-    _same_device(who, user_emb, item_table, item_bias)
+    _same_device(who, user_emb, item_table, item_bias, *others)   # (one pass over all of them: a small step is bound by the host)
 
 
 def _same_device(who, *tensors):
@@ -879,56 +879,54 @@ def full_distill_fwd(user_emb, item_table, teacher_id, teacher_score, item_bias=
     guard, -], lse float32[B], DistillSaved | None).  teacher_id int64 [B,K] / teacher_score [B,K] (float32, float16 or bfloat16): what
     full_topk returns; -1 / -inf entries are absent.  See include/unirec_amd.h: ur_full_distill_fwd."""
     who = "full_distill_fwd"
-    _distill_check(who, user_emb, item_table, item_bias, tau, temperature)
     _chk(teacher_id, torch.int64, "teacher_id")
     if teacher_score.dtype not in _lib.DTYPE_IDS:
         raise _lib.UnirecAmdError(f"teacher_score: expected float32 / float16 / bfloat16, got {teacher_score.dtype}")
     _chk(teacher_score, teacher_score.dtype, "teacher_score")
+    _distill_check(who, user_emb, item_table, item_bias, tau, temperature, teacher_id, teacher_score)
     B, d = user_emb.shape
     if teacher_id.dim() != 2 or teacher_id.shape[0] != B or teacher_score.shape != teacher_id.shape:
         raise _lib.UnirecAmdError(f"{who}: teacher_id {tuple(teacher_id.shape)} / teacher_score {tuple(teacher_score.shape)} for {B} rows")
-    _same_device(who, teacher_id, teacher_score)
     K, N, dev = teacher_id.shape[1], item_table.shape[0], user_emb.device
     if not 1 <= K <= 65536:
         raise _lib.UnirecAmdError(f"{who}: {K} entries a list (1 to 65536)")
     id_guard_check()
-    f32 = dict(dtype=torch.float32, device=dev)
+    f32, stream = dict(dtype=torch.float32, device=dev), _stream()
     lse, loss_out = torch.empty(B, **f32), torch.empty(4, **f32)
     ws = torch.empty(check(lib.ur_full_distill_workspace_bytes(B, d, N, K, int(need_grad)), "ur_full_distill_workspace_bytes"),
                      dtype=torch.uint8, device=dev)
     check(lib.ur_full_distill_fwd(_p(user_emb), _p(item_table), N, B, d, _p(teacher_id), _p(teacher_score), _lib.DTYPE_IDS[teacher_score.dtype], K,
                                   _p(item_bias), float(tau), float(score_clip if score_clip else -1.0), float(temperature), _p(lse), _p(loss_out),
-                                  int(need_grad), _p(ws), _stream()), "ur_full_distill_fwd")
-    return loss_out, lse, (DistillSaved(ws, (B, d, N, K), _distill_args(item_bias, tau, score_clip, temperature), _stream().value or 0) if need_grad else None)
+                                  int(need_grad), _p(ws), stream), "ur_full_distill_fwd")
+    return loss_out, lse, (DistillSaved(ws, (B, d, N, K), _distill_args(item_bias, tau, score_clip, temperature), stream.value or 0) if need_grad else None)
 
 
 def full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, saved, item_bias=None, tau=1.0, score_clip=-1.0, temperature=1.0, d_loss=None):
     """-> (d_user [B,d], d_table [N,d] dense, d_item_bias [N] | None) of a full_distill_fwd(need_grad=True) with the same arguments.
     See include/unirec_amd.h: ur_full_distill_bwd."""
     who = "full_distill_bwd"
-    _distill_check(who, user_emb, item_table, item_bias, tau, temperature)
     _chk(teacher_id, torch.int64, "teacher_id")
     _chk(lse, torch.float32, "lse")
     _chk(loss_out, torch.float32, "loss_out")
     _chk(d_loss, torch.float32, "d_loss", allow_none=True)
+    _distill_check(who, user_emb, item_table, item_bias, tau, temperature, teacher_id, lse, loss_out, d_loss)
     B, d = user_emb.shape
     N, dev = item_table.shape[0], user_emb.device
     if saved is None or teacher_id.dim() != 2 or saved.sizes != (B, d, N, teacher_id.shape[1]) or loss_out.numel() != 4 or lse.numel() != B:
         raise _lib.UnirecAmdError(f"{who}: not the results of a full_distill_fwd(need_grad=True) of these inputs")
-    if saved.args is not None and saved.args != _distill_args(item_bias, tau, score_clip, temperature):
-        raise _lib.UnirecAmdError(f"{who}: (item bias, tau, score_clip, temperature) = {_distill_args(item_bias, tau, score_clip, temperature)}, its "
-                                  f"full_distill_fwd had {saved.args}")
+    args = _distill_args(item_bias, tau, score_clip, temperature)
+    if saved.args is not None and saved.args != args:
+        raise _lib.UnirecAmdError(f"{who}: (item bias, tau, score_clip, temperature) = {args}, its full_distill_fwd had {saved.args}")
     if d_loss is not None and d_loss.numel() != 1:
         raise _lib.UnirecAmdError(f"{who}: d_loss has {d_loss.numel()} values (one, or None)")
-    K = teacher_id.shape[1]
-    _same_device(who, teacher_id, lse, loss_out, saved.ws, d_loss)
-    if saved.stream is not None and saved.stream != (_stream().value or 0):
+    K, stream = teacher_id.shape[1], _stream()
+    if saved.stream is not None and saved.stream != (stream.value or 0):
         saved.ws.record_stream(torch.cuda.current_stream())      # (its memory stays the forward's stream's: not to be handed out there under this pass)
     d_user = torch.empty(B, d, dtype=torch.float32, device=dev)
     d_table = torch.empty(N, d, dtype=torch.float32, device=dev)
     d_ib = torch.empty(N, dtype=torch.float32, device=dev) if item_bias is not None else None
     check(lib.ur_full_distill_bwd(_p(user_emb), _p(item_table), N, B, d, K, _p(item_bias), float(tau), float(score_clip if score_clip else -1.0),
-                                  float(temperature), _p(loss_out), _p(d_loss), _p(d_user), _p(d_table), _p(d_ib), _p(saved.ws), _stream()),
+                                  float(temperature), _p(loss_out), _p(d_loss), _p(d_user), _p(d_table), _p(d_ib), _p(saved.ws), stream),
           "ur_full_distill_bwd")
     return d_user, d_table, d_ib
 

@@ -340,7 +340,7 @@ def full_distill_bwd(user_emb: torch.Tensor, item_table: torch.Tensor, teacher_i
                      ws: torch.Tensor, d_loss: Optional[torch.Tensor], item_bias: Optional[torch.Tensor], tau: float = 1.0,
                      score_clip: float = -1.0, temperature: float = 1.0) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     sizes = (user_emb.shape[0], user_emb.shape[1], item_table.shape[0], teacher_id.shape[1])
-    if ws.dtype != torch.uint8 or ws.numel() != ops.check(ops.lib.ur_full_distill_workspace_bytes(sizes[0], sizes[1], sizes[2], sizes[3], 1), "ws"):
+    if ws.dtype != torch.uint8 or ws.device != user_emb.device or ws.numel() != ops.check(ops.lib.ur_full_distill_workspace_bytes(sizes[0], sizes[1], sizes[2], sizes[3], 1), "ws"):
         raise ops._lib.UnirecAmdError("full_distill_bwd: ws is not that of a full_distill_fwd of these sizes")
     sv = ops.DistillSaved(ws, sizes)
     d_user, d_table, d_ib = ops.full_distill_bwd(user_emb, item_table, teacher_id, lse, loss_out, sv, item_bias, tau, score_clip, temperature, d_loss)
