@@ -208,7 +208,7 @@ __device__ __forceinline__ T block_before(T v, T* tmp, T* total) {
 template <int NT>
 __device__ __forceinline__ WSum block_before(const WSum& v, u64* tmp, WSum* total) {   // tmp[2 NT / 64]: both limbs between the same two barriers
   constexpr int NW = NT / 64;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, wave = NW <= 4 ? (int)(threadIdx.x >> 6) : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const WSum s{wave_upto(v.hi), wave_upto(v.lo)};
   __syncthreads();
   if (lane == 63) { tmp[wave] = s.hi; tmp[NW + wave] = s.lo; }
@@ -219,7 +219,7 @@ __device__ __forceinline__ WSum block_before(const WSum& v, u64* tmp, WSum* tota
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
       const WSum t{tmp[w], tmp[NW + w]};
-      if (w < wave) r.add(t);
+      r.add(WSum{w < wave ? t.hi : 0, w < wave ? t.lo : 0});
       total->add(t);
     }
   } else {
@@ -385,9 +385,12 @@ __device__ __forceinline__ void pick_p(int round, const unsigned* hc, const u64*
 #pragma unroll
     for (int j = 0; j < PB; ++j) mine[j] = in_bin(j);
     int found = 0;
+    u128 upto = before;
 #pragma unroll
-    for (int j = 0; j < PB - 1; ++j)
-      if (found == j && wide_to_double(before + mine[j]) < limit) { before += mine[j]; ++found; }
+    for (int j = 0; j < PB - 1; ++j) {
+      upto += mine[j];
+      if (wide_to_double(upto) < limit) { before = upto; ++found; }
+    }
     const int place = (int)threadIdx.x * PB + found;
     st->above = before;
     st->limit = limit;
