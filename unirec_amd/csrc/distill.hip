@@ -311,7 +311,9 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && NW >= 4 ? 2 : 1) void distill_
       for (int cb = 0; cb < 2; ++cb) {
         float m2 = fmaxf(tmax[cb], __shfl_xor(tmax[cb], 16, 64));
         m2 = fmaxf(m2, __shfl_xor(m2, 32, 64));
-        const float Mn = m2 > M[cb] + 8.f ? m2 : M[cb];
+        // (a whole number, so that what is added to M or taken off it is hardly rounded: that would be in all the weights of a row alike.  By adding
+        // and taking off 1.5 2^23: rintf here costs D = 128 four registers that it spills, 377 -> 382 us at 512 x 200 K)
+        const float Mn = m2 > M[cb] + 8.f ? (m2 + 12582912.f) - 12582912.f : M[cb];
         const float f = __builtin_amdgcn_exp2f(M[cb] - Mn), fk = f * exp2f((float)(kn - kappa));
         l[cb] *= f;
         if constexpr (GRAD) {
@@ -479,8 +481,11 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && NW >= 4 ? 2 : 1) void distill_
       out = a.part_o + at * a.d;
     } else {
       const float gs = distill_scale(a.loss_out, a.d_loss, a.g_num), e = CLIP ? 0.f : xb[cb];
-      if (g == 0 && a.d_bias) a.d_bias[own] = lt * exp2f(M[cb] + e) * gs;
-      down = exp2f(M[cb] + e - (float)kappa) * gs;
+      // 2^(M + e), M + e in two pieces: its rounding would be in every term of the item's sums
+      const float at = M[cb] + e, back = at - M[cb], rest = at > -1e30f ? (M[cb] - (at - back)) + (e - back) : 0.f;
+      const float scale = exp2f(at) * fmaf(rest, DS_LN2, 1.f);
+      if (g == 0 && a.d_bias) a.d_bias[own] = lt * scale * gs;
+      down = ldexpf(scale, -kappa) * gs;
       out = a.dX + own * a.d;
     }
     if constexpr (GRAD) {
@@ -507,7 +512,7 @@ struct DistillRow {
   const float *part_m, *part_l, *part_o;
   const long long* id; const void* score; int score_type;
   const float* item_bias;
-  float inv_tau, inv_T, clip;
+  float inv_tau, inv_T, T, clip;
   float* lse;
   float* stat;                         // [0, B) loss of the row, [B, 2B) 1 = has a teacher, [2B, 3B) log2 of the softmax sum (+inf without a teacher)
   float* coef; int* tid;               // [B, K]: p (0 where the gradient is cut), item (0: absent; negative: a second time)
@@ -546,21 +551,22 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
   float l = 0.f;
   for (int s = tid; s < a.splits; s += 256) l += a.part_l[(long long)s * a.B + b] * exp2f(a.part_m[(long long)s * a.B + b] - m);
   l = ds_block_sum(l, red);
-  const float lse2 = m + log2f(l), lse = lse2 * DS_LN2;
+  // (log2f is 0.46 of a step low on average, and every q of the row would be as much too large: one step of Newton's, in the residual)
+  const float lg = log2f(l), lse2 = m + fmaf(fmaf(l, exp2f(-lg), -1.f), DS_LOG2E, lg), lse = lse2 * DS_LN2;
   // ---- the teacher's softmax
   float tm = -INFINITY, ts = 0.f;
   for (int k = tid; k < a.K; k += 256) {
     const long long i = (long long)b * a.K + k;
     long long id = a.id[i];
     if (id < -1 || id >= a.N) id = ur_guard_id(id, a.N, a.guard);   // not an item at all: the guard goes up, the entry is absent
-    const float v = teacher_at(a.score, a.score_type, i) * a.inv_T;
+    const float v = teacher_at(a.score, a.score_type, i) / a.T;
     if (id >= 1 && v > -INFINITY) tm = fmaxf(tm, v);
   }
   tm = ds_block_max(tm, red);
   const bool some = tm > -INFINITY;
   for (int k = tid; k < a.K; k += 256) {
     const long long i = (long long)b * a.K + k, id = a.id[i];
-    const float v = teacher_at(a.score, a.score_type, i) * a.inv_T;
+    const float v = teacher_at(a.score, a.score_type, i) / a.T;
     if (id >= 1 && id < a.N && v > -INFINITY) ts += expf(v - tm);
   }
   ts = ds_block_sum(ts, red);
@@ -580,7 +586,7 @@ __global__ __launch_bounds__(256) void distill_row_kernel(DistillRow a) {
       const int k = k0 + j * G;
       const long long i = (long long)b * a.K + min(k, a.K - 1);
       id[j] = a.id[i];
-      v[j] = teacher_at(a.score, a.score_type, i) * a.inv_T;
+      v[j] = teacher_at(a.score, a.score_type, i) / a.T;
       there[j] = k < a.K && some && id[j] >= 1 && id[j] < a.N && v[j] > -INFINITY;
     }
 #pragma unroll
@@ -972,7 +978,8 @@ __global__ __launch_bounds__(128) void distill_apply_kernel(DistillApply a) {
 static inline int ds_tpr(int d) { return d <= 64 ? 16 : d <= 128 ? 32 : 64; }
 // waves of a workgroup of the forward, 32 users each, the stream's tiles staged once for all of them.  Eight where they have users (512 x 60 K,
 // d 64: 49.8 us with eight, 50.7 with four) and registers; else four, also where some have none: 16 x 500 K, d 128: 147 us with four, 218 with
-// one, 182 with eight; 64 x 500 K: 151, 163 with two, 180 with eight; 128 x 500 K: 157 and 182
+// one, 182 with eight; 64 x 500 K: 151, 163 with two, 180 with eight; 128 x 500 K: 157 and 182; above, eight also where many have none: 130 x 500 K 189 and
+// 234 with four, 260 x 500 K 340 and 492, 400 x 500 K 356 and 434 (d 64: 145 and 150, 224 and 267, 223 and 242)
 static inline int ds_nw(int B, int d) { return B <= 128 || d <= 32 || d > 128 ? 4 : 8; }
 static inline int ds_width(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
@@ -1062,6 +1069,13 @@ static int ds_launch_bwd(const DistillStream& a, bool clip, hipStream_t st) {
   return nw == 1 ? ds_launch_stream<D, 1, false, true>(a, clip, grid, st) : ds_launch_stream<D, 4, false, true>(a, clip, grid, st);
 }
 
+// (rounded once: a scale that is off is off for every score of the batch, and what is off the same way everywhere stays in sums over the users)
+static inline void ds_scales(DistillStream& a, float tau, float score_clip, float temperature) {
+  constexpr double log2e = 1.4426950408889634074;
+  a.cz = (float)(log2e / ((double)tau * (double)temperature));
+  a.clip2 = score_clip > 0.f ? (float)((double)score_clip / (double)temperature * log2e) : 0.f;
+}
+
 static int ds_check(const float* table, int64_t N, int B, int d, int K, float tau, float T, const char* who) {
   UR_REQUIRE(table, UR_ERR_ARG, "%s: null pointer", who);
   UR_REQUIRE(B > 0 && d > 0 && d % 4 == 0 && N > 1 && N < (1LL << 31) && K > 0, UR_ERR_ARG, "%s: shape", who);
@@ -1096,7 +1110,7 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   const DistillWs w = ds_carve(B, d, n_items, K, grad, (char*)ws);
   DistillStream a{};
   a.X = user_emb; a.nx = B; a.Y = item_table; a.ny = n_items; a.d = d; a.y_bias = item_bias;
-  a.cz = DS_LOG2E / (tau * temperature); a.clip2 = score_clip > 0.f ? score_clip / temperature * DS_LOG2E : 0.f;
+  ds_scales(a, tau, score_clip, temperature);
   ds_splits(B, d, n_items, &a.owner_blocks, &a.splits, &a.tiles_per_split);
   a.part_m = w.part_m; a.part_l = w.part_l; a.part_o = w.part_o;
   const int nw = ds_nw(B, d), grid = a.owner_blocks * a.splits;
@@ -1108,7 +1122,7 @@ extern "C" int ur_full_distill_fwd(const float* user_emb, const float* item_tabl
   r.U = user_emb; r.E = item_table; r.N = n_items; r.B = B; r.d = d; r.K = K; r.splits = a.splits;
   r.part_m = w.part_m; r.part_l = w.part_l; r.part_o = w.part_o;
   r.id = (const long long*)teacher_id; r.score = teacher_score; r.score_type = score_type; r.item_bias = item_bias;
-  r.inv_tau = 1.f / tau; r.inv_T = 1.f / temperature; r.clip = score_clip;
+  r.inv_tau = 1.f / tau; r.inv_T = 1.f / temperature; r.T = temperature; r.clip = score_clip;
   r.lse = lse; r.stat = w.stat; r.coef = w.coef; r.tid = w.tid; r.d_unit = w.d_unit; r.guard = id_guard();
 #define GO(T) do { if (grad) hipLaunchKernelGGL((distill_row_kernel<T, true>), dim3(B), dim3(256), 0, st, r); \
                    else hipLaunchKernelGGL((distill_row_kernel<T, false>), dim3(B), dim3(256), 0, st, r); } while (0)
@@ -1150,7 +1164,7 @@ extern "C" int ur_full_distill_bwd(const float* user_emb, const float* item_tabl
   ProfScope ps(PC_LOSS, st, 4.0 * B * (double)n_items * d);
   DistillStream a{};
   a.X = item_table; a.nx = n_items; a.ny = B; a.d = d; a.img = w.img; a.rb_img = w.rb_img; a.ky_img = w.ky_img; a.x_bias = item_bias;
-  a.cz = DS_LOG2E / (tau * temperature); a.clip2 = score_clip > 0.f ? score_clip / temperature * DS_LOG2E : 0.f;
+  ds_scales(a, tau, score_clip, temperature);
   a.loss_out = loss_out; a.d_loss = d_loss; a.g_num = temperature / tau; a.dX = d_item_table; a.d_bias = d_item_bias;
   const bool clip = score_clip > 0.f;
   rc = d <= 32 ? ds_launch_bwd<32>(a, clip, st) : d <= 64 ? ds_launch_bwd<64>(a, clip, st)
