@@ -747,7 +747,10 @@ int ur_rows_scatter_add(const int32_t* uniq_idx, const int32_t* n_uniq_dev, int6
  *   bwd: d_user_emb[B,d]; d_item_table [n_items,d] DENSE and overwritten (row 0 = 0: padding_idx); d_item_bias [n_items] (required iff
  *        item_bias); a per-user bias would cancel in q: it has none.  d_loss: device scalar (nullable = 1).  No gradient where the score was clipped.
  * tau, temperature > 0; d % 4 == 0, d <= 256.  Nothing of size [B, n_items] exists; results are bit-reproducible.
- * A score within rounding of +-score_clip may be taken as cut or as not.
+ * A score within rounding of +-score_clip may be taken as cut or as not, and not alike everywhere: q's share of d_user, q's share of d_item_table and
+ * the teacher's share of both are decided by three roundings, so such an entry may lose one share and keep the others.
+ * A teacher_score of +inf leaves no softmax: the loss is NaN and the update guard is up.
+ * Sums over items and users are fp32 (over items in runs of 8 192 at most): d_user is the difference of two of them, q's and the teacher's.
  * ws: ur_full_distill_workspace_bytes of the same sizes and need_grad, from the forward to its backward, which only reads it. */
 enum { UR_F32 = 0, UR_F16 = 1, UR_BF16 = 2 }; /* element types of teacher_score and of ur_sample_scores' scores */
 int64_t ur_full_distill_workspace_bytes(int32_t B, int32_t d, int64_t n_items, int32_t K, int32_t need_grad);

@@ -15,9 +15,10 @@
 //
 // Two forms.  A row that fits into LDS (32 768 entries; 65 536 of 16 bits): one workgroup, one read of the row, every pass from LDS.
 // Longer rows: many workgroups a row, a pass over memory each for the maximum, for a selection's histogram and its border's step, and for the
-// kept sums.  Bound: short rows by the latency of the passes (1 x 1 000: 16 us, 512 x 1 000: 16 us), long rows with top-p by vector
-// instructions, 48 an entry for a weight and its sum, 0.76 of the cycles (64 x 1 M fp32: 378 us, without selections 169 us; 256 x 60 K bf16
-// with all three: 64 us, a workgroup a row and its passes over LDS).
+// kept sums.  Bound: short rows by the latency of the passes (1 x 1 000: 16 us, 512 x 1 000: 17 us), long rows with top-p by vector
+// instructions, 48 an entry for a weight and its sum: 0.76 of the cycles of the kept sums, 0.66 of the steps', whose weights also go through 64-bit
+// LDS atomics (64 x 1 M fp32: 371 - 376 us, without selections 168 us); 256 x 60 K bf16 with all three filters: 65 us, a workgroup a row and its passes
+// over LDS, one key a read (vector instructions in 0.50 of the cycles, the waves wait 0.59 of theirs).
 #include <math.h>
 
 #include <algorithm>
@@ -1298,8 +1299,8 @@ __global__ __launch_bounds__(256) void sample_draw_kernel(SampleArgs a, SampleLo
 }
 
 // ---- host
-// what fits into a workgroup's LDS beside the histograms.  Rows in LDS or over many workgroups, k 50 and p 0.9: 256 x 20 000 28 / 144 us, 4 x 30 000
-// 33 / 64
+// what fits into a workgroup's LDS beside the histograms.  Rows in LDS or over many workgroups, k 50 and p 0.9: 256 x 20 000 28 / 135 us, 4 x 30 000
+// 34 / 51
 static inline bool sample_in_lds(long long N, int type) { return N <= (type == UR_F32 ? 32768 : 65536); }
 static size_t sample_long_bytes(long long N, int B, char* base, SampleLong* g) {
   size_t o = 0;
@@ -1361,8 +1362,9 @@ extern "C" int ur_sample_scores(const void* scores, int32_t score_type, int64_t 
   a.ids = (const long long*)ids; a.ld_ids = ld_ids; a.out_id = (long long*)out_id; a.out_logp = out_logp;
   if (lds) {
     // (threads: about 8 entries each for short rows, whose passes are latency; 1 024 where the row is most of a CU's LDS anyway)
+    // threads for a row, 256 / 512 / 1 024, p 0.9: fp32 512 x 1 000 17.3 / 17.5 / 25.7 us, 256 x 6 000 31.0 / 23.5 / 22.3, 256 x 20 000 73 / 49 / 40;
+    // bf16 20.0 / 19.9 / 28.5, 39.0 / 28.0 / 25.8, 99 / 62 / 48 (one rule for both)
     if (score_type == UR_F32)
-      // threads for a row, 256 / 512 / 1 024 (same draws): 512 x 1 000 17.1 / 17.4 / 32.8 us, 256 x 6 000 24.5 / 20.4 / 20.3, 256 x 20 000 47 / 34 / 28
       return n <= 2048 ? launch_sample_row<256, false>(a, st) : n <= 8192 ? launch_sample_row<512, false>(a, st) : launch_sample_row<1024, false>(a, st);
     return n <= 2048 ? launch_sample_row<256, true>(a, st) : n <= 8192 ? launch_sample_row<512, true>(a, st) : launch_sample_row<1024, true>(a, st);
   }
