@@ -311,9 +311,9 @@ __global__ __launch_bounds__(NW * 64, D <= 128 && NW >= 4 ? 2 : 1) void distill_
       for (int cb = 0; cb < 2; ++cb) {
         float m2 = fmaxf(tmax[cb], __shfl_xor(tmax[cb], 16, 64));
         m2 = fmaxf(m2, __shfl_xor(m2, 32, 64));
-        // (a whole number, so that what is added to M or taken off it is hardly rounded: that would be in all the weights of a row alike.  By adding
-        // and taking off 1.5 2^23: rintf here costs D = 128 four registers that it spills, 377 -> 382 us at 512 x 200 K)
-        const float Mn = m2 > M[cb] + 8.f ? (m2 + 12582912.f) - 12582912.f : M[cb];
+        // (a whole number, so that what is added to M or taken off it is hardly rounded: that would be in all the weights of a row alike.  Not floorf or
+        // rintf: with those D = 128 spills four registers more, 377 -> 382 us at 512 x 200 K)
+        const float Mn = m2 > M[cb] + 8.f ? m2 - __builtin_amdgcn_fractf(m2) : M[cb];
         const float f = __builtin_amdgcn_exp2f(M[cb] - Mn), fk = f * exp2f((float)(kn - kappa));
         l[cb] *= f;
         if constexpr (GRAD) {
